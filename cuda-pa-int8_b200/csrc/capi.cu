@@ -282,10 +282,12 @@ int decode_impl(int mode, int kv_i8, void* out, float* part_out, const void* q,
     return fail(PA_ERR_INVALID_ARG, "null pointer argument");
   if (mode == pa::kModePartial ? part_out == nullptr : out == nullptr)
     return fail(PA_ERR_INVALID_ARG, "null output pointer");
-  if (kv_i8 && (k_scales == nullptr || v_scales == nullptr))
+  const bool fp4 = kv_i8 == 3;  // scales inside the cache, untiled bulk copies: no tensor maps
+  const bool scaled = kv_i8 != 0 && !fp4;
+  if (scaled && (k_scales == nullptr || v_scales == nullptr))
     return fail(PA_ERR_INVALID_ARG, "int8 cache needs k_scales and v_scales");
   if (!aligned(q, 16) || (out && !aligned(out, 16)) || !aligned(k_cache, 16) ||
-      !aligned(v_cache, 16) || (kv_i8 && (!aligned(k_scales, 16) || !aligned(v_scales, 16))) ||
+      !aligned(v_cache, 16) || (scaled && (!aligned(k_scales, 16) || !aligned(v_scales, 16))) ||
       !aligned(workspace, 256) || (part_out && !aligned(part_out, 16)))
     return fail(PA_ERR_INVALID_ARG, "tensors must be 16-byte aligned (workspace 256-byte)");
   if (!(scale == scale)) return fail(PA_ERR_INVALID_ARG, "scale is NaN");
@@ -299,10 +301,12 @@ int decode_impl(int mode, int kv_i8, void* out, float* part_out, const void* q,
 
   CUtensorMap maps[4];
   memset(maps, 0, sizeof(maps));
-  rc = get_map({k_cache, kv_i8 ? kMapKI8 : kMapKF16, NB, KVH, bs, D}, &maps[0]);
-  if (rc != PA_OK) return rc;
+  if (!fp4) {
+    rc = get_map({k_cache, kv_i8 ? kMapKI8 : kMapKF16, NB, KVH, bs, D}, &maps[0]);
+    if (rc != PA_OK) return rc;
+  }
   const bool bulk = (bs == pa::kSubTokens);
-  if (!bulk) {
+  if (!bulk && !fp4) {
     rc = get_map({v_cache, kv_i8 ? kMapVI8 : kMapVF16, NB, KVH, bs, D}, &maps[1]);
     if (rc != PA_OK) return rc;
     if (kv_i8) {
@@ -326,11 +330,15 @@ int decode_impl(int mode, int kv_i8, void* out, float* part_out, const void* q,
   const bool fuse = sw != nullptr && sw->fused && s.HT == 1 && sw->dtype != PA_DTYPE_F32 &&
                     aligned(sw->k, 16) && aligned(sw->v, 16) && (sw->stride * 2) % 16 == 0;
   if (sw != nullptr && !fuse) {
-    cudaError_t e = pa::launch_step_rows(
-        sw->dtype, row_kind, sw->k, sw->v, sw->stride, block_table, context_lens, max_blocks, B,
-        KVH, const_cast<void*>(k_cache), const_cast<void*>(v_cache),
-        const_cast<float*>(k_scales), const_cast<float*>(v_scales), NB, bs, sw->kfix, sw->vfix,
-        status, st);
+    cudaError_t e =
+        fp4 ? pa::launch_step_fp4(sw->dtype, sw->k, sw->v, sw->stride, block_table, context_lens,
+                                  max_blocks, B, KVH, const_cast<void*>(k_cache),
+                                  const_cast<void*>(v_cache), NB, bs, status, st)
+            : pa::launch_step_rows(
+                  sw->dtype, row_kind, sw->k, sw->v, sw->stride, block_table, context_lens,
+                  max_blocks, B, KVH, const_cast<void*>(k_cache), const_cast<void*>(v_cache),
+                  const_cast<float*>(k_scales), const_cast<float*>(v_scales), NB, bs, sw->kfix,
+                  sw->vfix, status, st);
     if (e != cudaSuccess) return cuda_fail(e, "step write launch");
   }
   const size_t new_es = sw == nullptr ? 0 : (sw->dtype == PA_DTYPE_F32 ? 4 : 2);
@@ -343,6 +351,7 @@ int decode_impl(int mode, int kv_i8, void* out, float* part_out, const void* q,
     a.q = static_cast<const __half*>(q) + (size_t)c0 * H * D;
     a.block_table = block_table + (size_t)c0 * max_blocks;
     a.context_lens = context_lens + c0;
+    a.k_base = static_cast<const uint8_t*>(k_cache);
     a.v_base = static_cast<const uint8_t*>(v_cache);
     a.ks_base = k_scales;
     a.vs_base = v_scales;
@@ -437,11 +446,34 @@ int check_row_write(int in_dtype, const void* k, const void* v, int64_t token_st
     return fail(PA_ERR_INVALID_ARG, "misaligned input or cache pointer");
   return PA_OK;
 }
-// Cache kind of the decode kernels: 0 fp16, 1 int8, 2 fp8 e4m3 (-1: not a cache dtype).
+// Cache kind of the decode kernels: 0 fp16, 1 int8, 2 fp8 e4m3, 3 fp4 (-1: not a cache dtype).
 int kv_kind(int kv_dtype) {
   return kv_dtype == PA_DTYPE_F16 ? 0
          : kv_dtype == PA_DTYPE_I8 ? 1
-         : kv_dtype == PA_DTYPE_FP8E4M3 ? 2 : -1;
+         : kv_dtype == PA_DTYPE_FP8E4M3 ? 2
+         : kv_dtype == PA_DTYPE_FP4E2M1 ? 3 : -1;
+}
+
+// Checks shared by the 4-bit cache's row write and read (rows in 16-byte units).
+int check_fp4_rows(int dt, const void* k, const void* v, int64_t token_stride,
+                   const int32_t* slot_mapping, int num_tokens, int num_kv_heads, int head_dim,
+                   const void* k_cache, const void* v_cache, int num_blocks, int block_size) {
+  if (num_tokens < 0 || num_kv_heads <= 0 || num_blocks <= 0)
+    return fail(PA_ERR_INVALID_ARG, "invalid sizes");
+  if (head_dim != 128) return fail(PA_ERR_UNSUPPORTED, "head_dim %d unsupported", head_dim);
+  if (block_size <= 0 || block_size % 16 != 0)
+    return fail(PA_ERR_INVALID_ARG, "block_size must be a multiple of 16");
+  if (k == nullptr || v == nullptr || slot_mapping == nullptr || k_cache == nullptr ||
+      v_cache == nullptr)
+    return fail(PA_ERR_INVALID_ARG, "null pointer argument");
+  if (token_stride < (int64_t)num_kv_heads * head_dim)
+    return fail(PA_ERR_INVALID_ARG, "token_stride smaller than num_kv_heads*head_dim");
+  if (!aligned(k, 16) || !aligned(v, 16) || (token_stride * elem_size(dt)) % 16 != 0 ||
+      !aligned(k_cache, 16) || !aligned(v_cache, 16))
+    return fail(PA_ERR_INVALID_ARG, "rows and caches must be 16-byte aligned");
+  if ((long long)num_tokens * num_kv_heads > (1LL << 34))
+    return fail(PA_ERR_UNSUPPORTED, "too many rows for one call");
+  return PA_OK;
 }
 
 }  // namespace
@@ -476,6 +508,9 @@ const char* pa_status_string(int status) {
   if (status & PA_ERR_TIMEOUT) return "device wait timed out";
   if (status & PA_ERR_SLOT) return "slot_mapping entry outside the cache";
   if (status & PA_ERR_Q_RANGE) return "bf16 q value outside the fp16 range (saturated)";
+  if (status & PA_ERR_FREE_BLOCKS) return "not enough room in the free-block stack";
+  if (status & PA_ERR_TOKENS) return "more new tokens than max_tokens";
+  if (status & PA_ERR_POSITION) return "position outside the rotation table";
   return "unknown status";
 }
 
@@ -589,7 +624,8 @@ int pa_decode_bf16q(void* out, const void* q, const void* k_cache, const void* v
   const NvtxRange nvtx_range("pa_decode_bf16q");
   if (kv_kind(kv_dtype) < 0)
     return fail(PA_ERR_UNSUPPORTED,
-                "kv_dtype must be PA_DTYPE_F16, PA_DTYPE_I8 or PA_DTYPE_FP8E4M3");
+                "kv_dtype must be PA_DTYPE_F16, PA_DTYPE_I8, PA_DTYPE_FP8E4M3 or "
+                "PA_DTYPE_FP4E2M1");
   int rc = check_common(num_seqs, num_heads, num_kv_heads, head_dim, num_blocks, block_size,
                         max_blocks_per_seq);
   if (rc != PA_OK) return rc;
@@ -659,6 +695,30 @@ int pa_splitk_fp8(void* out, const void* q, const void* k_cache, const void* v_c
                      workspace_bytes, stream);
 }
 
+int pa_decode_fp4(void* out, const void* q, const void* k_cache, const void* v_cache,
+                  const int32_t* block_table, const int32_t* context_lens, int num_seqs,
+                  int num_heads, int num_kv_heads, int head_dim, int num_blocks, int block_size,
+                  int max_blocks_per_seq, float scale, void* workspace, size_t workspace_bytes,
+                  void* stream) {
+  const NvtxRange nvtx_range("pa_decode_fp4");
+  return decode_impl(pa::kModeStream, 3, out, nullptr, q, k_cache, v_cache, nullptr, nullptr,
+                     block_table, context_lens, num_seqs, num_heads, num_kv_heads, head_dim,
+                     num_blocks, block_size, max_blocks_per_seq, scale, workspace,
+                     workspace_bytes, stream);
+}
+
+int pa_splitk_fp4(void* out, const void* q, const void* k_cache, const void* v_cache,
+                  const int32_t* block_table, const int32_t* context_lens, int num_seqs,
+                  int num_heads, int num_kv_heads, int head_dim, int num_blocks, int block_size,
+                  int max_blocks_per_seq, float scale, void* workspace, size_t workspace_bytes,
+                  void* stream) {
+  const NvtxRange nvtx_range("pa_splitk_fp4");
+  return decode_impl(pa::kModeSplit, 3, out, nullptr, q, k_cache, v_cache, nullptr, nullptr,
+                     block_table, context_lens, num_seqs, num_heads, num_kv_heads, head_dim,
+                     num_blocks, block_size, max_blocks_per_seq, scale, workspace,
+                     workspace_bytes, stream);
+}
+
 int pa_decode_step(int kv_dtype, void* out, const void* q, const void* new_k,
                    const void* new_v, int new_dtype, int64_t new_token_stride, void* k_cache,
                    void* v_cache, float* k_scales, float* v_scales, const float* k_fixed_scale,
@@ -671,7 +731,8 @@ int pa_decode_step(int kv_dtype, void* out, const void* q, const void* new_k,
   const int kind = kv_kind(kv_dtype);
   if (kind < 0)
     return fail(PA_ERR_UNSUPPORTED,
-                "kv_dtype must be PA_DTYPE_F16, PA_DTYPE_I8 or PA_DTYPE_FP8E4M3");
+                "kv_dtype must be PA_DTYPE_F16, PA_DTYPE_I8, PA_DTYPE_FP8E4M3 or "
+                "PA_DTYPE_FP4E2M1");
   int rc = check_in_dtype(new_dtype);
   if (rc != PA_OK) return rc;
   if (num_seqs == 0) return PA_OK;
@@ -682,6 +743,9 @@ int pa_decode_step(int kv_dtype, void* out, const void* q, const void* new_k,
   const size_t es = (size_t)elem_size(new_dtype);
   if (!aligned(new_k, es * 4) || !aligned(new_v, es * 4) || new_token_stride % 4 != 0)
     return fail(PA_ERR_INVALID_ARG, "misaligned new-token rows");
+  if (kind == 3 && (!aligned(new_k, 16) || !aligned(new_v, 16) ||
+                    (new_token_stride * (int64_t)es) % 16 != 0))
+    return fail(PA_ERR_INVALID_ARG, "new-token rows of an fp4 cache must be 16-byte aligned");
   if ((k_fixed_scale != nullptr || v_fixed_scale != nullptr) &&
       (kind != 1 || k_fixed_scale == nullptr || v_fixed_scale == nullptr))
     return fail(PA_ERR_INVALID_ARG, "fixed scales need an int8 cache and both of k and v");
@@ -708,7 +772,7 @@ int pa_decode_partial(int kv_dtype, float* partials, const void* q, const void* 
                       size_t workspace_bytes, void* stream) {
   const NvtxRange nvtx_range("pa_decode_partial");
   if (kv_kind(kv_dtype) < 0)
-    return fail(PA_ERR_UNSUPPORTED, "kv dtype must be fp16, int8 or fp8 e4m3");
+    return fail(PA_ERR_UNSUPPORTED, "kv dtype must be fp16, int8, fp8 e4m3 or fp4");
   return decode_impl(pa::kModePartial, kv_kind(kv_dtype), nullptr, partials, q,
                      k_cache, v_cache, k_scales, v_scales, block_table, context_lens, num_seqs,
                      num_heads, num_kv_heads, head_dim, num_blocks, block_size,
@@ -789,6 +853,209 @@ int pa_quantize_into_cache_fp8(const void* k, const void* v, int in_dtype, int64
                                         k_scales, v_scales, num_blocks, block_size, nullptr,
                                         nullptr, status, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "fp8 quantize launch");
+  return PA_OK;
+}
+
+int pa_quantize_into_cache_fp4(const void* k, const void* v, int in_dtype, int64_t token_stride,
+                               const int32_t* slot_mapping, int num_tokens, int num_kv_heads,
+                               int head_dim, void* k_cache, void* v_cache, int num_blocks,
+                               int block_size, int* status, void* stream) {
+  const NvtxRange nvtx_range("pa_quantize_into_cache_fp4");
+  int rc = check_in_dtype(in_dtype);
+  if (rc != PA_OK) return rc;
+  if (num_tokens == 0) return PA_OK;
+  rc = check_fp4_rows(in_dtype, k, v, token_stride, slot_mapping, num_tokens, num_kv_heads,
+                      head_dim, k_cache, v_cache, num_blocks, block_size);
+  if (rc != PA_OK) return rc;
+  cudaError_t e = pa::launch_write_fp4(in_dtype, k, v, token_stride, slot_mapping, num_tokens,
+                                       num_kv_heads, k_cache, v_cache, num_blocks, block_size,
+                                       status, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "fp4 quantize launch");
+  return PA_OK;
+}
+
+int pa_read_from_cache_fp4(void* k_out, void* v_out, int out_dtype, const void* k_cache,
+                           const void* v_cache, const int32_t* slot_mapping, int num_tokens,
+                           int num_kv_heads, int head_dim, int num_blocks, int block_size,
+                           int* status, void* stream) {
+  const NvtxRange nvtx_range("pa_read_from_cache_fp4");
+  int rc = check_in_dtype(out_dtype);
+  if (rc != PA_OK) return rc;
+  if (num_tokens == 0) return PA_OK;
+  rc = check_fp4_rows(out_dtype, k_out, v_out, (int64_t)num_kv_heads * head_dim, slot_mapping,
+                      num_tokens, num_kv_heads, head_dim, k_cache, v_cache, num_blocks,
+                      block_size);
+  if (rc != PA_OK) return rc;
+  cudaError_t e = pa::launch_read_fp4(out_dtype, k_out, v_out, k_cache, v_cache, slot_mapping,
+                                      num_tokens, num_kv_heads, num_blocks, block_size, status,
+                                      static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "fp4 read launch");
+  return PA_OK;
+}
+
+// Norm and rotation: the checks of both forms, then the launch. kind: the cache's RowKind, or
+// -1 for k rows to k_out.
+static int norm_rope(const char* what, int dtype, int kind, const pa::RopeArgs& a, int head_dim,
+                     void* stream) {
+  int rc = check_in_dtype(dtype);
+  if (rc != PA_OK) return rc;
+  if (a.N == 0) return PA_OK;
+  if (a.N < 0 || a.H < 0 || a.KVH < 0 || a.H > (1 << 20) || a.KVH > (1 << 20) ||
+      (a.H == 0 && a.KVH == 0) || a.table_len <= 0)
+    return fail(PA_ERR_INVALID_ARG, "invalid sizes");
+  if (head_dim != 128) return fail(PA_ERR_UNSUPPORTED, "head_dim %d unsupported", head_dim);
+  if (a.rot <= 0 || a.rot > 128 || a.rot % 16 != 0)
+    return fail(PA_ERR_UNSUPPORTED, "rot_dim %d unsupported (a multiple of 16 up to 128)", a.rot);
+  if (!(a.eps >= 0.f)) return fail(PA_ERR_INVALID_ARG, "eps must be >= 0");
+  const int64_t es = elem_size(dtype);
+  auto rows = [&](const void* p, long long stride, int heads) {
+    return heads == 0 || (p != nullptr && aligned(p, 16) && (stride * es) % 16 == 0 &&
+                          stride >= (long long)heads * head_dim);
+  };
+  if (a.positions == nullptr || a.table == nullptr ||
+      !rows(a.q, a.q_stride, a.H) || !rows(a.q_out, a.qo_stride, a.H) ||
+      !rows(a.k, a.k_stride, a.KVH))
+    return fail(PA_ERR_INVALID_ARG,
+                "q, k and out rows must be non-null, 16-byte aligned and contiguous per token");
+  if (!aligned(a.table, 16)) return fail(PA_ERR_INVALID_ARG, "table must be 16-byte aligned");
+  if ((a.q_weight && !aligned(a.q_weight, 16)) || (a.k_weight && !aligned(a.k_weight, 16)))
+    return fail(PA_ERR_INVALID_ARG, "weights must be 16-byte aligned");
+  if (kind < 0) {
+    if (!rows(a.k_out, a.ko_stride, a.KVH))
+      return fail(PA_ERR_INVALID_ARG,
+                  "k_out rows must be non-null, 16-byte aligned and contiguous per token");
+  } else {
+    if (a.KVH == 0 || a.NB <= 0 || a.bs <= 0) return fail(PA_ERR_INVALID_ARG, "invalid sizes");
+    if (kind == pa::kRowsFP4 && a.bs % 16 != 0)
+      return fail(PA_ERR_INVALID_ARG, "block_size must be a multiple of 16");
+    if (!rows(a.v, a.v_stride, a.KVH))
+      return fail(PA_ERR_INVALID_ARG,
+                  "v rows must be non-null, 16-byte aligned and contiguous per token");
+    if (a.slots == nullptr || a.k_cache == nullptr || a.v_cache == nullptr ||
+        ((kind == pa::kRowsI8 || kind == pa::kRowsFP8) &&
+         (a.k_scales == nullptr || a.v_scales == nullptr)))
+      return fail(PA_ERR_INVALID_ARG, "null pointer argument");
+    if (!aligned(a.k_cache, 16) || !aligned(a.v_cache, 16))
+      return fail(PA_ERR_INVALID_ARG, "caches must be 16-byte aligned");
+  }
+  const int sms = num_sms_current(nullptr);
+  if (sms <= 0) return fail(PA_ERR_CUDA, "cannot query the current device");
+  cudaError_t e = pa::launch_norm_rope(dtype, kind, a, sms, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  return PA_OK;
+}
+
+int pa_qk_norm_rope(void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride,
+                    const void* q, int64_t q_stride, const void* k, int64_t k_stride, int dtype,
+                    const void* q_weight, const void* k_weight, float eps,
+                    const int32_t* positions, const float* table, int table_len, int rot_dim,
+                    int interleaved, int num_tokens, int num_heads, int num_kv_heads,
+                    int head_dim, int* status, void* stream) {
+  const NvtxRange nvtx_range("pa_qk_norm_rope");
+  pa::RopeArgs a;
+  memset(&a, 0, sizeof(a));
+  a.q = q; a.k = k; a.q_weight = q_weight; a.k_weight = k_weight;
+  a.positions = positions; a.table = table; a.q_out = q_out; a.k_out = k_out;
+  a.q_stride = q_stride; a.k_stride = k_stride;
+  a.qo_stride = q_out_stride; a.ko_stride = k_out_stride;
+  a.N = num_tokens; a.H = num_heads; a.KVH = num_kv_heads;
+  a.table_len = table_len; a.rot = rot_dim; a.interleaved = interleaved != 0; a.eps = eps;
+  a.status = status;
+  return norm_rope("norm and rotation launch", dtype, -1, a, head_dim, stream);
+}
+
+int pa_norm_rope_into_cache(void* q_out, int64_t q_out_stride, const void* q, int64_t q_stride,
+                            const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                            int dtype, const void* q_weight, const void* k_weight, float eps,
+                            const int32_t* positions, const float* table, int table_len,
+                            int rot_dim, int interleaved, const int32_t* slot_mapping,
+                            int num_tokens, int num_heads, int num_kv_heads, int head_dim,
+                            int cache_dtype, void* k_cache, void* v_cache, float* k_scales,
+                            float* v_scales, int num_blocks, int block_size, int* status,
+                            void* stream) {
+  const NvtxRange nvtx_range("pa_norm_rope_into_cache");
+  const int kind = cache_dtype == PA_DTYPE_F16      ? pa::kRowsF16
+                   : cache_dtype == PA_DTYPE_I8      ? pa::kRowsI8
+                   : cache_dtype == PA_DTYPE_FP8E4M3 ? pa::kRowsFP8
+                   : cache_dtype == PA_DTYPE_FP4E2M1 ? pa::kRowsFP4
+                                                     : -1;
+  if (kind < 0)
+    return fail(PA_ERR_UNSUPPORTED, "cache dtype must be fp16, int8, fp8 e4m3 or fp4");
+  pa::RopeArgs a;
+  memset(&a, 0, sizeof(a));
+  a.q = q; a.k = k; a.v = v; a.q_weight = q_weight; a.k_weight = k_weight;
+  a.positions = positions; a.table = table; a.q_out = q_out;
+  a.q_stride = q_stride; a.k_stride = k_stride; a.v_stride = v_stride;
+  a.qo_stride = q_out_stride;
+  a.N = num_tokens; a.H = num_heads; a.KVH = num_kv_heads;
+  a.table_len = table_len; a.rot = rot_dim; a.interleaved = interleaved != 0; a.eps = eps;
+  a.slots = slot_mapping;
+  a.k_cache = k_cache; a.v_cache = v_cache; a.k_scales = k_scales; a.v_scales = v_scales;
+  a.NB = num_blocks; a.bs = block_size; a.status = status;
+  return norm_rope("norm, rotation and cache write launch", dtype, kind, a, head_dim, stream);
+}
+
+// Checks shared by the two block-table calls.
+static int check_tables(const pa::TableArgs& a) {
+  if (a.S < 0 || a.max_blocks <= 0 || a.bs <= 0 || a.pool < 0)
+    return fail(PA_ERR_INVALID_ARG, "invalid sizes");
+  if ((long long)a.max_blocks * a.bs > 0x7fffffffLL)
+    return fail(PA_ERR_UNSUPPORTED, "max_blocks_per_seq * block_size must be below 2^31");
+  if ((a.S > 0 && (a.table == nullptr || a.lens == nullptr || a.flags == nullptr ||
+                   a.lens_out == nullptr)) ||
+      (a.pool > 0 && a.free_blocks == nullptr) || a.free_count == nullptr ||
+      a.count_out == nullptr)
+    return fail(PA_ERR_INVALID_ARG, "null pointer argument");
+  return PA_OK;
+}
+
+int pa_release_blocks(const int32_t* block_table, const int32_t* context_lens,
+                      const int32_t* finished, int32_t* free_blocks, const int32_t* free_count,
+                      int32_t* context_lens_out, int32_t* free_count_out, int num_seqs,
+                      int max_blocks_per_seq, int block_size, int pool_size, int* status,
+                      void* stream) {
+  const NvtxRange nvtx_range("pa_release_blocks");
+  pa::TableArgs a;
+  memset(&a, 0, sizeof(a));
+  a.table = const_cast<int32_t*>(block_table);
+  a.lens = context_lens; a.flags = finished;
+  a.free_blocks = free_blocks; a.free_count = free_count;
+  a.lens_out = context_lens_out; a.count_out = free_count_out;
+  a.S = num_seqs; a.max_blocks = max_blocks_per_seq; a.bs = block_size; a.pool = pool_size;
+  int rc = check_tables(a);
+  if (rc != PA_OK) return rc;
+  a.status = status;
+  cudaError_t e = pa::launch_release(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "block release launch");
+  return PA_OK;
+}
+
+int pa_extend_block_tables(int32_t* block_table, const int32_t* context_lens,
+                           const int32_t* new_lens, const int32_t* free_blocks,
+                           const int32_t* free_count, int32_t* context_lens_out,
+                           int32_t* free_count_out, int32_t* slot_mapping, int32_t* positions,
+                           int32_t* query_start, int num_seqs, int max_blocks_per_seq,
+                           int block_size, int pool_size, int num_blocks, int max_tokens,
+                           int* status, void* stream) {
+  const NvtxRange nvtx_range("pa_extend_block_tables");
+  pa::TableArgs a;
+  memset(&a, 0, sizeof(a));
+  a.table = block_table; a.lens = context_lens; a.flags = new_lens;
+  a.free_blocks = const_cast<int32_t*>(free_blocks); a.free_count = free_count;
+  a.lens_out = context_lens_out; a.count_out = free_count_out;
+  a.slots = slot_mapping; a.positions = positions; a.starts = query_start;
+  a.S = num_seqs; a.max_blocks = max_blocks_per_seq; a.bs = block_size; a.pool = pool_size;
+  a.NB = num_blocks; a.max_tokens = max_tokens;
+  int rc = check_tables(a);
+  if (rc != PA_OK) return rc;
+  if (num_blocks <= 0 || max_tokens < 0) return fail(PA_ERR_INVALID_ARG, "invalid sizes");
+  if ((long long)num_blocks * block_size > 0x80000000LL)
+    return fail(PA_ERR_UNSUPPORTED, "num_blocks * block_size must be at most 2^31 slots");
+  if (query_start == nullptr || (max_tokens > 0 && (slot_mapping == nullptr || positions == nullptr)))
+    return fail(PA_ERR_INVALID_ARG, "null pointer argument");
+  a.status = status;
+  cudaError_t e = pa::launch_extend(a, static_cast<cudaStream_t>(stream));
+  if (e != cudaSuccess) return cuda_fail(e, "block table launch");
   return PA_OK;
 }
 

@@ -34,6 +34,7 @@
 // split merge  m = max m_s,  l = sum l_s e^{m_s - m},  o = sum o_s e^{m_s - m} / l.
 // Scores are kept in log2 units (scale * log2 e) so the exponentials are exp2.
 
+#include "fp4.cuh"
 #include "pa_common.cuh"
 #include "pa_internal.h"
 #include "pa_rows.cuh"
@@ -65,10 +66,11 @@ template <int KVK, int D, int GT, int DEPTH, int WARPS>
 struct Tile {
   static constexpr bool I8 = KVK == 1;    // int8 values, per-token scales
   static constexpr bool F8 = KVK == 2;    // fp8 e4m3 values, per-token scales
-  static constexpr bool BYTE = KVK != 0;  // one-byte elements (the INT8 page layout)
+  static constexpr bool F4 = KVK == 3;    // fp4 e2m1 values, a scale per 16 (fp4.cuh)
+  static constexpr bool BYTE = I8 || F8;  // one-byte elements (the INT8 page layout)
   static constexpr int ELEM = BYTE ? 1 : 2;
-  static constexpr int KT = D * kSubTokens * ELEM;  // K tile bytes
-  static constexpr int VT = D * kSubTokens * ELEM;  // V tile bytes
+  static constexpr int KT = F4 ? fp4::kGroupBytes : D * kSubTokens * ELEM;  // K tile bytes
+  static constexpr int VT = KT;                                             // V tile bytes
   // Scale tiles: 16 K scales at +0 and 16 V scales at +128 (tensor-copy destinations are
   // kept 128-byte aligned); 128 bytes of them are transferred per stage.
   static constexpr int ST = BYTE ? 256 : 0;
@@ -359,8 +361,37 @@ __device__ __noinline__ void stage_new_token(const uint8_t* rk, uint8_t* kt, uin
                                              const float* vfix, void* kc, void* vc, float* ks,
                                              float* vs, int bs) {
   static_assert(D == 128, "one lane per four head_dim values");
-  constexpr bool BYTE = KVK != 0;
+  constexpr bool BYTE = KVK == 1 || KVK == 2;
   constexpr int KIND = KVK == 1 ? kRowsI8 : (KVK == 2 ? kRowsFP8 : kRowsF16);
+  if constexpr (KVK == 3) {
+    // The staged tile and the cache hold the group in the same layout.
+    uint8_t* kg = static_cast<uint8_t*>(kc) + fp4::group_offset((size_t)row, off, bs);
+    uint8_t* vg = static_cast<uint8_t*>(vc) + fp4::group_offset((size_t)row, off, bs);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float x[4];
+      const uint8_t* src = rk + which * D * 2;
+      if (new_dtype == PA_DTYPE_BF16) {
+        load_vals<__nv_bfloat16, 4>(reinterpret_cast<const __nv_bfloat16*>(src) + 4 * lane, x);
+      } else {
+        load_vals<__half, 4>(reinterpret_cast<const __half*>(src) + 4 * lane, x);
+      }
+      uint32_t sb;
+      const uint32_t w = fp4::warp_quantize4<false>(x, sb);
+      uint8_t* tile = which ? vt : kt;
+      uint8_t* grp = which ? vg : kg;
+      const int co = t * fp4::kCodeRow + 2 * lane;
+      const int so = fp4::scale_offset(which != 0, t, lane >> 2);
+      *reinterpret_cast<uint16_t*>(tile + co) = (uint16_t)w;
+      *reinterpret_cast<uint16_t*>(grp + co) = (uint16_t)w;
+      if ((lane & 3) == 0) {
+        tile[so] = (uint8_t)sb;
+        grp[so] = (uint8_t)sb;
+      }
+    }
+    __syncwarp();
+    return;
+  }
   RowQ<KIND, D> qk, qv;
   if (new_dtype == PA_DTYPE_BF16) {
     qk = warp_quantize_row<__nv_bfloat16, KIND, D>(reinterpret_cast<const __nv_bfloat16*>(rk),
@@ -408,6 +439,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   using C = Tile<KVK, D, GT, DEPTH, WARPS>;
   constexpr bool I8 = C::I8;
   constexpr bool F8 = C::F8;
+  constexpr bool F4 = C::F4;
   constexpr bool BYTE = C::BYTE;
   constexpr int NS = C::NS;
   constexpr int MT = C::MT;
@@ -462,8 +494,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       prefetch_l2_share(a.new_k, nb, blockIdx.x, gridDim.x);
       prefetch_l2_share(a.new_v, nb, blockIdx.x, gridDim.x);
     }
-    prefetch_tensormap(&tm_k);
-    if (!a.bulk) {
+    if constexpr (!F4) prefetch_tensormap(&tm_k);
+    if (!F4 && !a.bulk) {
       prefetch_tensormap(&tm_v);
       if constexpr (BYTE) {
         prefetch_tensormap(&tm_ks);
@@ -621,7 +653,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     const __half* qrow = a.q + ((size_t)b * a.H + (size_t)kvh * a.G + hl) * D;
 #pragma unroll
     for (int si = 0; si < NS; ++si) {
-      const int c = BYTE ? chunk_i8(r, si) : chunk_f16(r, si);
+      const int c = F4 ? 4 * r + si : (BYTE ? chunk_i8(r, si) : chunk_f16(r, si));
       ra[si] = (hl < a.G) ? __ldg(reinterpret_cast<const uint4*>(qrow + 8 * c))
                           : make_uint4(0u, 0u, 0u, 0u);
       if constexpr (GT == 16) {
@@ -795,6 +827,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         }
       }
       // The cache pages stream through L2 marked evict-first.
+      if constexpr (F4) {  // a group of 16 tokens is contiguous, whatever the block size
+        const size_t o = ((size_t)row * a.subs + sub) * C::KT;
+        bulk_g2s_hint(kd, a.k_base + o, C::KT, bar, pol);
+        bulk_g2s_hint(vd, a.v_base + o, C::VT, bar, pol);
+        return;
+      }
       if constexpr (BYTE) {
         tma_load_3d_hint(kd, &tm_k, bar, sub * 128, 0, row, pol);
       } else {
@@ -833,7 +871,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
     for (int jt = 0; jt < 2; ++jt) {
       const int tau = 4 * (g >> 1) + (g & 1) + 2 * jt;
-      if constexpr (BYTE) {
+      if constexpr (F4) {
+        koff[si][jt] = 0;  // one 16-byte load a token, addressed directly
+      } else if constexpr (BYTE) {
         const int c = chunk_i8(r, si);
         koff[si][jt] = c * 128 + ((((tau >> 1) ^ (c & 7)) << 4) | ((tau & 1) << 3));
       } else {
@@ -860,6 +900,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 
   float m0 = neg_inf(), l0 = 0.f, m1 = neg_inf(), l1 = 0.f;
   float oacc[MT][NT][4];
+  // head_dim of O's row g (hi = 0) and g + 8 (hi = 1) of m-tile i.
+  auto drow = [&](int i, int hi) { return F4 ? 16 * g + 2 * i + hi : 16 * i + g + 8 * hi; };
 
   int jfail = -1;
   int s = 0;        // ring stage of page j
@@ -925,6 +967,22 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     uint32_t v8[MT][2];
     uint2 v16[MT][2];
     float4 ksv = make_float4(0.f, 0.f, 0.f, 0.f), vsv = ksv;
+    // FP4: tokens 4 (g / 2) + g % 2 + 2 jt of K (values 32 r .. 32 r + 31: one block scale a
+    // half), tokens 4r .. 4r + 3 of V (values 16 g .. 16 g + 15: one block scale a token).
+    uint4 k4[2];
+    uint2 v4[4];
+    uint32_t k4s[2], v4s = 0u;
+    if constexpr (F4) {
+#pragma unroll
+      for (int jt = 0; jt < 2; ++jt) {
+        const int tau = 4 * (g >> 1) + (g & 1) + 2 * jt;
+        k4[jt] = lds128(kb + tau * fp4::kCodeRow + 16 * r);
+        k4s[jt] = lds16(kb + fp4::kCodes + tau * 8 + 2 * r);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v4[e] = lds64(vb + (4 * r + e) * fp4::kCodeRow + 8 * g);
+      v4s = lds32(vb + fp4::kCodes + 16 * g + 4 * r);
+    } else {
 #pragma unroll
     for (int si = 0; si < NS; ++si) {
 #pragma unroll
@@ -942,6 +1000,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         v16[i][0] = lds64(vb + voff + i * 512);
         v16[i][1] = lds64(vb + voff + i * 512 + 256);
       }
+    }
     }
     if constexpr (BYTE) {
       ksv = lds128f(sb + 16 * r);
@@ -1035,6 +1094,24 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
               e4m3x4_to_f16x2x2(k8[si][jt].x, k16[si][jt].x, k16[si][jt].y);
               e4m3x4_to_f16x2x2(k8[si][jt].y, k16[si][jt].z, k16[si][jt].w);
             }
+        }
+        if constexpr (F4) {
+          // Codes -> fp16, times the block scale: exact (fp4.cuh).
+#pragma unroll
+          for (int jt = 0; jt < 2; ++jt) {
+            const uint32_t w[4] = {k4[jt].x, k4[jt].y, k4[jt].z, k4[jt].w};
+            const uint32_t sc[2] = {(k4s[jt] & 0xffu) * 0x00800080u,
+                                    (k4s[jt] >> 8) * 0x00800080u};
+#pragma unroll
+            for (int si = 0; si < NS; ++si) {
+              uint4& h = k16[si][jt];
+              fp4::codes_to_f16x2(w[si], h.x, h.y, h.z, h.w);
+              h.x = fp4::hmul2(h.x, sc[si >> 1]);
+              h.y = fp4::hmul2(h.y, sc[si >> 1]);
+              h.z = fp4::hmul2(h.z, sc[si >> 1]);
+              h.w = fp4::hmul2(h.w, sc[si >> 1]);
+            }
+          }
         }
         // Two accumulation chains per n-tile (even / odd si) shorten the MMA dependency.
         float sacc[2][2][4];
@@ -1175,6 +1252,51 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         split_f16x2(py[2], py[3], pc1, pm1);
       }
 
+      // FP4: the lane's V scales of tokens (4r, 4r + 1) and (4r + 2, 4r + 3); zero past the
+      // context, where the bytes may be anything (a finite code times zero is zero).
+      uint32_t vs01 = 0u, vs23 = 0u;
+      uint32_t vlo01[2], vhi01[2], vlo23[2], vhi23[2];
+      if constexpr (F4) {
+        vs01 = prmt(v4s, 0u, 0x4140u) << 7;
+        vs23 = prmt(v4s, 0u, 0x4342u) << 7;
+        if (valid < kSubTokens) {
+          vs01 &= ((4 * r < valid) ? 0x0000ffffu : 0u) | ((4 * r + 1 < valid) ? 0xffff0000u : 0u);
+          vs23 &= ((4 * r + 2 < valid) ? 0x0000ffffu : 0u) |
+                  ((4 * r + 3 < valid) ? 0xffff0000u : 0u);
+        }
+        // The MMA pairs tokens: the even and odd head_dim codes of two tokens, a byte each.
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w0 = h ? v4[0].y : v4[0].x, w1 = h ? v4[1].y : v4[1].x;
+          const uint32_t w2 = h ? v4[2].y : v4[2].x, w3 = h ? v4[3].y : v4[3].x;
+          vlo01[h] = (w0 & 0x0f0f0f0fu) | ((w1 << 4) & 0xf0f0f0f0u);
+          vhi01[h] = ((w0 >> 4) & 0x0f0f0f0fu) | (w1 & 0xf0f0f0f0u);
+          vlo23[h] = (w2 & 0x0f0f0f0fu) | ((w3 << 4) & 0xf0f0f0f0u);
+          vhi23[h] = ((w2 >> 4) & 0x0f0f0f0fu) | (w3 & 0xf0f0f0f0u);
+        }
+        // O^T rows g and g + 8 of m-tile 4h + j are head_dim 16 g + 8 h + 2 j and the next.
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t A0[4], A1[4], A2[4], A3[4];
+          fp4::codes_to_f16x2(vlo01[h], A0[0], A0[1], A0[2], A0[3]);
+          fp4::codes_to_f16x2(vhi01[h], A1[0], A1[1], A1[2], A1[3]);
+          fp4::codes_to_f16x2(vlo23[h], A2[0], A2[1], A2[2], A2[3]);
+          fp4::codes_to_f16x2(vhi23[h], A3[0], A3[1], A3[2], A3[3]);
+#pragma unroll
+          for (int jj = 0; jj < 4; ++jj) {
+            const int i = 4 * h + jj;
+            const uint32_t a0 = fp4::hmul2(A0[jj], vs01), a1 = fp4::hmul2(A1[jj], vs01);
+            const uint32_t a2 = fp4::hmul2(A2[jj], vs23), a3 = fp4::hmul2(A3[jj], vs23);
+            mma_16816(oacc[i][0], a0, a1, a2, a3, pb0, pb1);
+            mma_16816(oacc[i][0], a0, a1, a2, a3, pl0, pl1);
+            if constexpr (NT == 2) {
+              mma_16816(oacc[i][1], a0, a1, a2, a3, pc0, pc1);
+              mma_16816(oacc[i][1], a0, a1, a2, a3, pm0, pm1);
+            }
+          }
+        }
+      }
+
       // O^T += V^T P^T : rows = head_dim (16 per m-tile), columns = heads.
       uint32_t mlo = 0xffffffffu, mhi = 0xffffffffu;
       if (!I8 && valid < kSubTokens) {
@@ -1182,7 +1304,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         mhi = ((4 * r + 2 < valid) ? 0x0000ffffu : 0u) | ((4 * r + 3 < valid) ? 0xffff0000u : 0u);
       }
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
+      for (int i = 0; i < (F4 ? 0 : MT); ++i) {
         uint32_t a0, a1, a2, a3;
         if constexpr (I8) {
           i8x4_to_f16x2x2(v8[i][0], a0, a2);
@@ -1241,9 +1363,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         for (int i = 0; i < MT; ++i) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            *reinterpret_cast<float2*>(slot + (16 * i + g) * GT + nt * 8 + 2 * r) =
+            *reinterpret_cast<float2*>(slot + drow(i, 0) * GT + nt * 8 + 2 * r) =
                 make_float2(oacc[i][nt][0] * kUnscale, oacc[i][nt][1] * kUnscale);
-            *reinterpret_cast<float2*>(slot + (16 * i + g + 8) * GT + nt * 8 + 2 * r) =
+            *reinterpret_cast<float2*>(slot + drow(i, 1) * GT + nt * 8 + 2 * r) =
                 make_float2(oacc[i][nt][2] * kUnscale, oacc[i][nt][3] * kUnscale);
           }
         }
@@ -1280,12 +1402,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
               const float fa = nt ? ic : ia;
               const float fb = nt ? id : ib;
               if (h < hcnt) {
-                ob[(size_t)h * D + 16 * i + g] = __float2half_rn(oacc[i][nt][0] * fa);
-                ob[(size_t)h * D + 16 * i + g + 8] = __float2half_rn(oacc[i][nt][2] * fa);
+                ob[(size_t)h * D + drow(i, 0)] = __float2half_rn(oacc[i][nt][0] * fa);
+                ob[(size_t)h * D + drow(i, 1)] = __float2half_rn(oacc[i][nt][2] * fa);
               }
               if (h + 1 < hcnt) {
-                ob[(size_t)(h + 1) * D + 16 * i + g] = __float2half_rn(oacc[i][nt][1] * fb);
-                ob[(size_t)(h + 1) * D + 16 * i + g + 8] = __float2half_rn(oacc[i][nt][3] * fb);
+                ob[(size_t)(h + 1) * D + drow(i, 0)] = __float2half_rn(oacc[i][nt][1] * fb);
+                ob[(size_t)(h + 1) * D + drow(i, 1)] = __float2half_rn(oacc[i][nt][3] * fb);
               }
             }
           }
@@ -1492,6 +1614,14 @@ template <> struct Shape<1, 16> { static constexpr int W = 8, DP = 4; };
 template <> struct Shape<0, 16> { static constexpr int W = 8, DP = 3; };
 template <> struct Shape<2, 8> { static constexpr int W = 12, DP = 3; };
 template <> struct Shape<2, 16> { static constexpr int W = 8, DP = 4; };
+#ifndef PA_F4_WARPS
+#define PA_F4_WARPS 12
+#endif
+#ifndef PA_F4_DEPTH
+#define PA_F4_DEPTH 4
+#endif
+template <> struct Shape<3, 8> { static constexpr int W = PA_F4_WARPS, DP = PA_F4_DEPTH; };
+template <> struct Shape<3, 16> { static constexpr int W = 8, DP = 6; };
 
 template <int KVK, int GT>
 cudaError_t launch_one(const DecodeArgs& a, const CUtensorMap* maps, int grid,
@@ -1522,6 +1652,7 @@ cudaError_t launch_one(const DecodeArgs& a, const CUtensorMap* maps, int grid,
 }  // namespace
 
 int decode_warps_per_cta(int kv_i8, int gt) {
+  if (kv_i8 == 3) return gt == 8 ? Shape<3, 8>::W : Shape<3, 16>::W;
   if (kv_i8 == 2) return gt == 8 ? Shape<2, 8>::W : Shape<2, 16>::W;
   if (kv_i8) return gt == 8 ? Shape<1, 8>::W : Shape<1, 16>::W;
   return gt == 8 ? Shape<0, 8>::W : Shape<0, 16>::W;
@@ -1529,6 +1660,10 @@ int decode_warps_per_cta(int kv_i8, int gt) {
 
 cudaError_t launch_decode(int kv_i8, int gt, const DecodeArgs& a, const CUtensorMap* maps,
                           int grid, cudaStream_t stream) {
+  if (kv_i8 == 3) {
+    return gt == 8 ? launch_one<3, 8>(a, maps, grid, stream)
+                   : launch_one<3, 16>(a, maps, grid, stream);
+  }
   if (kv_i8 == 2) {
     return gt == 8 ? launch_one<2, 8>(a, maps, grid, stream)
                    : launch_one<2, 16>(a, maps, grid, stream);

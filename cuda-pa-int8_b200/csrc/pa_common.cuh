@@ -236,6 +236,11 @@ __device__ __forceinline__ void prefetch_tensormap(const CUtensorMap* map) {
 // ------------------------------------------------------------------------------------------
 // Shared-memory loads
 // ------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t lds16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(addr));
+  return v;
+}
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));

@@ -59,6 +59,7 @@ struct DecodeArgs {
   void* vc_w;
   float* ks_w;
   float* vs_w;
+  const uint8_t* k_base;       // K cache base (fp4: its groups are untiled bulk copies)
 };
 
 struct ReduceArgs {
@@ -82,6 +83,7 @@ enum RowKind {
   kRowsF16 = 0,  // fp16 copy
   kRowsI8 = 1,   // int8, per-token or fixed scale
   kRowsFP8 = 2,  // fp8 e4m3, per-token scale
+  kRowsFP4 = 3,  // fp4 e2m1, a scale per 16 values (fp4.cuh)
 };
 cudaError_t launch_write_rows(int in_dtype, int kind, int D, const void* k, const void* v,
                               long long token_stride, const int* slots, int N, int KVH,
@@ -102,6 +104,61 @@ cudaError_t launch_prefill(int in_dtype, bool i8, const void* k, const void* v, 
 cudaError_t launch_absmax_scale(int in_dtype, const void* x, long long n, float* scale_out,
                                 int semantics, unsigned int* scratch, int num_sms,
                                 cudaStream_t st);
+
+// The 4-bit cache: slot-mapped write, the decode step's write, rows read back (fp4.cu).
+cudaError_t launch_write_fp4(int in_dtype, const void* k, const void* v, long long token_stride,
+                             const int* slots, int N, int KVH, void* kc, void* vc, int NB, int bs,
+                             int* status, cudaStream_t st);
+cudaError_t launch_step_fp4(int in_dtype, const void* k, const void* v, long long token_stride,
+                            const int* block_table, const int* context_lens, int max_blocks,
+                            int B, int KVH, void* kc, void* vc, int NB, int bs, int* status,
+                            cudaStream_t st);
+cudaError_t launch_read_fp4(int out_dtype, void* k, void* v, const void* kc, const void* vc,
+                            const int* slots, int N, int KVH, int NB, int bs, int* status,
+                            cudaStream_t st);
+
+// Norm and rotation of q and k rows (rope.cu). Strides are elements per token; rows of a token
+// are contiguous. kind: the RowKind of the cache k and v go into, or -1 for k rows to k_out.
+struct RopeArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* q_weight;  // [128] or null: no norm
+  const void* k_weight;
+  const int* positions;  // [N]; negative: the token is skipped
+  const float* table;    // [table_len, rot]: cosines, then sines
+  void* q_out;
+  void* k_out;
+  long long q_stride, k_stride, v_stride, qo_stride, ko_stride;
+  int N, H, KVH, table_len, rot, interleaved;
+  float eps;
+  const int* slots;  // cache forms: [N]; negative: K and V are not written
+  void* k_cache;
+  void* v_cache;
+  float* k_scales;
+  float* v_scales;
+  int NB, bs;
+  int* status;
+};
+cudaError_t launch_norm_rope(int dtype, int kind, const RopeArgs& a, int sms, cudaStream_t st);
+
+// Block tables of a step (tables.cu).
+struct TableArgs {
+  int* table;             // [S, max_blocks]
+  const int* lens;        // [S]
+  const int* flags;       // release: finished flags; extend: tokens to add
+  int* free_blocks;       // [pool], the stack
+  const int* free_count;  // [1]
+  int* lens_out;          // [S], may be lens
+  int* count_out;         // [1], may be free_count
+  int* slots;             // extend: [max_tokens]
+  int* positions;         // [max_tokens]
+  int* starts;            // [S + 1]
+  int* status;
+  int S, max_blocks, bs, pool, NB, max_tokens;
+};
+cudaError_t launch_release(const TableArgs& a, cudaStream_t st);
+cudaError_t launch_extend(const TableArgs& a, cudaStream_t st);
 
 // bf16 <-> fp16 activation conversions (n a multiple of 8, 16-byte aligned buffers).
 cudaError_t launch_bf16_to_f16(const void* in, void* out, long long n, int* status, int num_sms,

@@ -23,12 +23,16 @@ PA_ERR_BLOCK_ID = 64
 PA_ERR_TIMEOUT = 128
 PA_ERR_SLOT = 256
 PA_ERR_Q_RANGE = 512
+PA_ERR_FREE_BLOCKS = 1024
+PA_ERR_TOKENS = 2048
+PA_ERR_POSITION = 4096
 
 PA_DTYPE_F16 = 0
 PA_DTYPE_BF16 = 1
 PA_DTYPE_F32 = 2
 PA_DTYPE_I8 = 3
 PA_DTYPE_FP8E4M3 = 4
+PA_DTYPE_FP4E2M1 = 5
 
 PA_SCALE_CLAMP_THEN_DIVIDE = 0
 PA_SCALE_DIVIDE_THEN_CLAMP = 1
@@ -68,6 +72,21 @@ SIGNATURES = {
                            _vp, _sz, _vp]),
     "pa_quantize_into_cache_fp8": (_i, [_vp, _vp, _i, _i64, _vp, _i, _i, _i, _vp, _vp, _vp, _vp,
                                         _i, _i, _vp, _vp]),
+    "pa_decode_fp4": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _vp,
+                           _sz, _vp]),
+    "pa_splitk_fp4": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _vp,
+                           _sz, _vp]),
+    "pa_quantize_into_cache_fp4": (_i, [_vp, _vp, _i, _i64, _vp, _i, _i, _i, _vp, _vp, _i, _i,
+                                        _vp, _vp]),
+    "pa_read_from_cache_fp4": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp]),
+    "pa_qk_norm_rope": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i, _vp, _vp, _f, _vp,
+                             _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp]),
+    "pa_norm_rope_into_cache": (_i, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _i, _vp, _vp, _f,
+                                     _vp, _vp, _i, _i, _i, _vp, _i, _i, _i, _i, _i, _vp, _vp,
+                                     _vp, _vp, _i, _i, _vp, _vp]),
+    "pa_release_blocks": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]),
+    "pa_extend_block_tables": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i,
+                                    _i, _i, _i, _vp, _vp]),
     "pa_decode_step": (_i, [_i, _vp, _vp, _vp, _vp, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                             _vp, _i, _i, _i, _i, _i, _i, _i, _f, _i, _i, _vp, _sz, _vp]),
     "pa_partial_floats": (_i, [_i, _i, _i]),

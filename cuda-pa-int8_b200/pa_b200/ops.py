@@ -105,16 +105,22 @@ def _require(cond, msg):
 
 
 _FP8 = getattr(torch, "float8_e4m3fn", None)
+FP4_GROUP_TOKENS = 16    # tokens of a group of the 4-bit cache
+FP4_GROUP_BYTES = 1152   # its codes (16 x 64 bytes) and scales (16 x 8)
 
 
 def _kv_kind(k_cache, k_scales):
-    """'f8' for an fp8 e4m3 cache, 'i8' for int8 (or whenever scales are given), else 'f16'."""
+    """'f4' for a 4-bit cache (uint8), 'f8' for an fp8 e4m3 cache, 'i8' for int8 (or whenever
+    scales are given), else 'f16'."""
+    if k_cache.dtype == torch.uint8:
+        return "f4"
     if _FP8 is not None and k_cache.dtype == _FP8:
         return "f8"
     return "i8" if (k_scales is not None or k_cache.dtype == torch.int8) else "f16"
 
 
-_KV_CODE = {"f16": _lib.PA_DTYPE_F16, "i8": _lib.PA_DTYPE_I8, "f8": _lib.PA_DTYPE_FP8E4M3}
+_KV_CODE = {"f16": _lib.PA_DTYPE_F16, "i8": _lib.PA_DTYPE_I8, "f8": _lib.PA_DTYPE_FP8E4M3,
+            "f4": _lib.PA_DTYPE_FP4E2M1}
 
 
 def _check_lengths(context_lens, capacity, host_context_lens=None):
@@ -136,9 +142,20 @@ def _check_lengths(context_lens, capacity, host_context_lens=None):
     _require(int(a.max()) <= capacity, "context_lens exceeds max_blocks_per_seq * block_size")
 
 
+def _check_fp4_caches(k_cache, v_cache, block_size):
+    """(num_blocks, kv_heads) of 4-bit caches [num_blocks, kv_heads, block_size/16, 1152]."""
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
+        _require(t.dtype == torch.uint8 and t.dim() == 4 and t.shape[3] == FP4_GROUP_BYTES and
+                 t.shape[2] * FP4_GROUP_TOKENS == block_size and t.shape == k_cache.shape,
+                 f"{name} of a 4-bit cache must be uint8 [num_blocks, kv_heads, block_size/16, "
+                 f"{FP4_GROUP_BYTES}]; got {t.dtype} {tuple(t.shape)}")
+    return k_cache.shape[0], k_cache.shape[1]
+
+
 def _check_decode_args(out, q, k_cache, v_cache, block_table, context_lens, block_size,
                        kind, k_scales, v_scales, act_dtype=torch.float16):
-    scaled = kind != "f16"  # one-byte cache with per-token scales (int8 or fp8)
+    scaled = kind in ("i8", "f8")  # one-byte cache with per-token scales
+    fp4 = kind == "f4"
     _require(q.is_cuda and (out is None or out.is_cuda), "tensors must be on CUDA")
     act_name = "fp16" if act_dtype == torch.float16 else "bf16"
     _require(q.dtype == act_dtype, f"q must be {act_name}")
@@ -153,6 +170,10 @@ def _check_decode_args(out, q, k_cache, v_cache, block_table, context_lens, bloc
                  "k_scales must be fp32")
         _require(v_scales is not None and v_scales.dtype == torch.float32,
                  "v_scales must be fp32")
+    elif fp4:
+        _require(k_cache.dtype == torch.uint8 and v_cache.dtype == torch.uint8,
+                 "a 4-bit cache is uint8, K and V")
+        _require(k_scales is None and v_scales is None, "a 4-bit cache holds its own scales")
     else:
         _require(k_cache.dtype == torch.float16, "k_cache must be fp16")
         _require(v_cache.dtype == torch.float16, "v_cache must be fp16")
@@ -172,19 +193,25 @@ def _check_decode_args(out, q, k_cache, v_cache, block_table, context_lens, bloc
     if out is not None:
         _require(tuple(out.shape) == (B, H, D) and out.dtype == act_dtype,
                  f"out must be {act_name} with the shape of q")
-    _require(k_cache.dim() == 5,
-             "k_cache must be [num_blocks, kv_heads, head_dim/x, block_size, x]")
-    NB, KVH, DX, BS, x = k_cache.shape
-    if scaled:
-        _require(x == 8, "int8 K cache requires x == 8")
-    _require(x == X, "K cache requires x == 8")
-    _require(D == HEAD_DIM, f"head_dim {D} unsupported (this build: {HEAD_DIM})")
-    _require(DX * x == D, "k_cache head_dim/x does not match q")
-    _require(block_size % 16 == 0 and 128 % block_size == 0,
-             "block_size must divide TILE (multiple of 16)")
-    _require(BS == block_size, f"k_cache block dimension {BS} != block_size {block_size}")
-    _require(tuple(v_cache.shape) == (NB, KVH, D, block_size),
-             "v_cache must be [num_blocks, kv_heads, head_dim, block_size]")
+    if fp4:
+        _require(D == HEAD_DIM, f"head_dim {D} unsupported (this build: {HEAD_DIM})")
+        _require(block_size > 0 and block_size % 16 == 0 and 128 % block_size == 0,
+                 "block_size must divide TILE (multiple of 16)")
+        NB, KVH = _check_fp4_caches(k_cache, v_cache, block_size)
+    else:
+        _require(k_cache.dim() == 5,
+                 "k_cache must be [num_blocks, kv_heads, head_dim/x, block_size, x]")
+        NB, KVH, DX, BS, x = k_cache.shape
+        if scaled:
+            _require(x == 8, "int8 K cache requires x == 8")
+        _require(x == X, "K cache requires x == 8")
+        _require(D == HEAD_DIM, f"head_dim {D} unsupported (this build: {HEAD_DIM})")
+        _require(DX * x == D, "k_cache head_dim/x does not match q")
+        _require(block_size % 16 == 0 and 128 % block_size == 0,
+                 "block_size must divide TILE (multiple of 16)")
+        _require(BS == block_size, f"k_cache block dimension {BS} != block_size {block_size}")
+        _require(tuple(v_cache.shape) == (NB, KVH, D, block_size),
+                 "v_cache must be [num_blocks, kv_heads, head_dim, block_size]")
     if scaled:
         _require(tuple(k_scales.shape) == (NB, KVH, block_size) and
                  tuple(v_scales.shape) == (NB, KVH, block_size),
@@ -203,11 +230,12 @@ def decode(out, q, k_cache, v_cache, block_table, context_lens, scale, block_siz
     """Paged decode attention into `out` (fp16 [num_seqs, num_heads, head_dim]).
 
     The cache type follows the tensors: fp16; int8 or float8_e4m3fn, each with per-token fp32
-    k_scales/v_scales (an int8 cache is assumed whenever scales are given). splitk
+    k_scales/v_scales (an int8 cache is assumed whenever scales are given); uint8 for a 4-bit
+    cache (fp4_cache), which holds its own scales. splitk
     selects the partition + LSE-reduce kernel pair (512-token splits); otherwise the
     single-pass kernel with the fused combine runs. validate=False skips the one host sync
     that checks context_lens (the kernels still flag bad lengths in the status word).
-    kv_kind ('f16', 'i8' or 'f8') pins the cache type instead of inferring it from the
+    kv_kind ('f16', 'i8', 'f8' or 'f4') pins the cache type instead of inferring it from the
     tensors, so a cache of another type is rejected (the reference-named ops use this).
     host_context_lens, a CPU tensor holding the same lengths (for instance the pinned copy the
     lengths were uploaded from), moves that check to the host: the call then does not
@@ -227,7 +255,7 @@ def decode(out, q, k_cache, v_cache, block_table, context_lens, scale, block_siz
         _require(need > 0, "unsupported decode shape: " + _lib.last_error())
         ws = workspace(q.device, need)
         stream = _stream(q.device)
-        if kind != "f16":
+        if kind in ("i8", "f8"):
             if kind == "f8":
                 fn = L.pa_splitk_fp8 if splitk else L.pa_decode_fp8
             else:
@@ -237,7 +265,10 @@ def decode(out, q, k_cache, v_cache, block_table, context_lens, scale, block_siz
                     context_lens.data_ptr(), B, H, KVH, D, NB, block_size, max_blocks,
                     float(scale), ws.data_ptr(), ws.numel(), stream)
         else:
-            fn = L.pa_splitk_f16 if splitk else L.pa_decode_f16
+            if kind == "f4":
+                fn = L.pa_splitk_fp4 if splitk else L.pa_decode_fp4
+            else:
+                fn = L.pa_splitk_f16 if splitk else L.pa_decode_f16
             args = (out.data_ptr(), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                     block_table.data_ptr(), context_lens.data_ptr(), B, H, KVH, D, NB,
                     block_size, max_blocks, float(scale), ws.data_ptr(), ws.numel(), stream)
@@ -276,9 +307,11 @@ class DecodePlan:
             self.fn = L.pa_splitk_fp8 if splitk else L.pa_decode_fp8
         elif kind == "i8":
             self.fn = L.pa_splitk_i8 if splitk else L.pa_decode_i8
+        elif kind == "f4":
+            self.fn = L.pa_splitk_fp4 if splitk else L.pa_decode_fp4
         else:
             self.fn = L.pa_splitk_f16 if splitk else L.pa_decode_f16
-        self.scaled = kind != "f16"
+        self.scaled = kind in ("i8", "f8")
         self.device = q.device
         self.sizes = (B, H, KVH, D, NB, block_size, self.max_blocks, float(scale))
         self.caches = ((k_cache.data_ptr(), v_cache.data_ptr()) +
@@ -325,8 +358,8 @@ def decode_step(out, q, new_k, new_v, k_cache, v_cache, block_table, context_len
     context_lens already counts the new token: new_k / new_v [num_seqs, kv_heads, head_dim]
     (fp16, bf16 or fp32 rows) go to position context_lens[b] - 1 of sequence b through
     block_table, written like quantize_into_cache (int8 cache, per-token scales or the
-    per-tensor k_scale / v_scale), its FP8 counterpart or write_into_cache (fp16 cache); then
-    the decode of decode() runs over the whole context. This is the bridge's
+    per-tensor k_scale / v_scale), its FP8 and 4-bit counterparts or write_into_cache (fp16
+    cache); then the decode of decode() runs over the whole context. This is the bridge's
     PagedKVCache.decode_append + split-K op (benchmarks/int8_bridge/paged_cache.py:132-156,
     qwen_paged_attn.py:61-73) for a whole batch in one call. With fused=True (and at most 16 q
     heads per kv head) the decode kernel writes each token itself just before reading its
@@ -380,15 +413,15 @@ def decode_step(out, q, new_k, new_v, k_cache, v_cache, block_table, context_len
 
 def decode_bf16(out, q, k_cache, v_cache, block_table, context_lens, scale, block_size=16, *,
                 k_scales=None, v_scales=None, splitk=False, validate=True):
-    """decode() with bf16 activations: q and out are bf16, the cache fp16, per-token INT8 or
-    per-token FP8 (e4m3).
+    """decode() with bf16 activations: q and out are bf16, the cache fp16, per-token INT8,
+    per-token FP8 (e4m3) or 4-bit.
 
     q is converted to fp16 on the device (exact for magnitudes in the fp16 normal range; larger
     values saturate and set the PA_ERR_Q_RANGE status bit), the fp16 decode runs, and the output
     is rounded once to bf16.
     """
     kind = _kv_kind(k_cache, k_scales)
-    int8 = kind != "f16"
+    int8 = kind in ("i8", "f8")
     B, H, KVH, D, NB = _check_decode_args(out, q, k_cache, v_cache, block_table, context_lens,
                                           block_size, kind, k_scales, v_scales,
                                           act_dtype=torch.bfloat16)
@@ -617,6 +650,303 @@ def prefill_into_cache(k, v, k_cache, v_cache, block_table, context_lens, block_
             v_cache.data_ptr(), _ptr(k_scales), _ptr(v_scales), k_cache.shape[0], block_size,
             _ptr(k_scale), _ptr(v_scale), ws.data_ptr(), _stream(k.device))
         _lib.check(rc, "prefill_into_cache")
+
+
+def fp4_cache(num_blocks, num_kv_heads, block_size=16, device="cuda"):
+    """A zeroed 4-bit K/V cache: (k_cache, v_cache), each uint8 [num_blocks, num_kv_heads,
+    block_size/16, 1152]. The layout is include/pa_b200.h's; 72 bytes hold K or V of one token
+    and kv head (4.5 bits a value), against 132 in an int8 cache and 256 in an fp16 one."""
+    _require(block_size > 0 and block_size % FP4_GROUP_TOKENS == 0 and 128 % block_size == 0,
+             "block_size must divide TILE (multiple of 16)")
+    return tuple(torch.zeros(num_blocks, num_kv_heads, block_size // FP4_GROUP_TOKENS,
+                             FP4_GROUP_BYTES, dtype=torch.uint8, device=device)
+                 for _ in range(2))
+
+
+def _check_slots(slot_mapping, num_tokens, device):
+    _require(slot_mapping.dtype == torch.int32 and slot_mapping.is_cuda,
+             "slot_mapping must be int32 on CUDA")
+    _require(slot_mapping.numel() == num_tokens and slot_mapping.is_contiguous() and
+             slot_mapping.device == device,
+             "slot_mapping must be contiguous, with one entry per token, on the rows' device")
+
+
+def quantize_into_cache_fp4(key, value, k_cache, v_cache, slot_mapping, block_size=16):
+    """Write key/value [num_tokens, kv_heads, 128] (fp16, bf16 or fp32) into a 4-bit cache
+    (fp4_cache) at slot_mapping (int32, block*block_size+offset; negative = skip).
+
+    Sixteen neighbouring values share a scale: the nearest representable to amax / 6, ties to
+    even; a value becomes the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 times it, ties to the even
+    code. A block holding a NaN or an infinity reads back as NaN. Two tokens with the same slot
+    in one call leave a mixture of their blocks there."""
+    _check_rows(key, value)
+    N, KVH, D = key.shape
+    _require(D == HEAD_DIM, f"head_dim {D} unsupported (this build: {HEAD_DIM})")
+    _check_slots(slot_mapping, N, key.device)
+    NB, kvh = _check_fp4_caches(k_cache, v_cache, block_size)
+    _require(kvh == KVH, f"the cache has {kvh} kv heads, the rows {KVH}")
+    for t in (value, k_cache, v_cache):
+        _require(t.device == key.device, "all tensors must be on the same CUDA device")
+    for t in (k_cache, v_cache):
+        _require(t.is_contiguous(), "cache tensors must be contiguous")
+    with _Guard(key.device):
+        ws = workspace(key.device, 256)
+        rc = _lib.lib().pa_quantize_into_cache_fp4(
+            key.data_ptr(), value.data_ptr(), _DTYPE_CODE[key.dtype], key.stride(0),
+            slot_mapping.data_ptr(), N, KVH, D, k_cache.data_ptr(), v_cache.data_ptr(), NB,
+            block_size, ws.data_ptr(), _stream(key.device))
+        _lib.check(rc, "quantize_into_cache (fp4)")
+
+
+def read_from_cache_fp4(k_cache, v_cache, slot_mapping, block_size=16, *, dtype=torch.float16,
+                        out=None):
+    """Rows read back from a 4-bit cache: (key, value) [num_tokens, kv_heads, 128] of the tokens
+    at slot_mapping, for instance a cached prefix for the attention of a prompt's next chunk.
+    Held values are exact in fp16, bf16 and fp32. Rows of negative slots are not written: they
+    keep what `out`, a pair of tensors to write into, held, and are undefined without it."""
+    _require(k_cache.is_cuda and v_cache.is_cuda, "tensors must be on CUDA")
+    NB, KVH = _check_fp4_caches(k_cache, v_cache, block_size)
+    N = slot_mapping.numel()
+    _check_slots(slot_mapping, N, k_cache.device)
+    _require(v_cache.device == k_cache.device and k_cache.is_contiguous() and
+             v_cache.is_contiguous(), "cache tensors must be contiguous and on one device")
+    if out is None:
+        _require(dtype in _DTYPE_CODE, "dtype must be fp16, bf16 or fp32")
+        out = tuple(torch.empty(N, KVH, HEAD_DIM, dtype=dtype, device=k_cache.device)
+                    for _ in range(2))
+    key, value = out
+    for t in (key, value):
+        _require(t.dtype in _DTYPE_CODE and t.dtype == key.dtype and t.device == k_cache.device and
+                 tuple(t.shape) == (N, KVH, HEAD_DIM) and t.is_contiguous(),
+                 f"out must be two contiguous [{N}, {KVH}, {HEAD_DIM}] tensors of one type on the "
+                 "cache's device")
+    with _Guard(k_cache.device):
+        ws = workspace(k_cache.device, 256)
+        rc = _lib.lib().pa_read_from_cache_fp4(
+            key.data_ptr(), value.data_ptr(), _DTYPE_CODE[key.dtype], k_cache.data_ptr(),
+            v_cache.data_ptr(), slot_mapping.data_ptr(), N, KVH, HEAD_DIM, NB, block_size,
+            ws.data_ptr(), _stream(k_cache.device))
+        _lib.check(rc, "read_from_cache (fp4)")
+    return key, value
+
+
+# ---------------------------------------------------------------------------------------
+# Norm and position rotation
+# ---------------------------------------------------------------------------------------
+def rope_table(num_positions, rot_dim=HEAD_DIM, base=10000.0, device="cuda"):
+    """Rotation table [num_positions, rot_dim] fp32: cos(p * base^(-2i/rot_dim)) for i <
+    rot_dim/2, then the sines. Angles are formed in 64 bits (far positions lose them in 32)."""
+    inv = float(base) ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) /
+                          rot_dim)
+    ang = torch.arange(num_positions, dtype=torch.float64, device=device)[:, None] * inv
+    return torch.cat([ang.cos(), ang.sin()], 1).float()
+
+
+def _check_head_rows(name, t, like, heads=None):
+    """[num_tokens, heads, 128] rows, contiguous per token; like: a tensor whose tokens, type
+    and device they share."""
+    _require(t.is_cuda, "tensors must be on CUDA")
+    _require(t.dim() == 3 and t.shape[2] == HEAD_DIM and t.shape[0] == like.shape[0] and
+             (heads is None or t.shape[1] == heads),
+             f"{name} must be [{like.shape[0]}, {heads or 'heads'}, {HEAD_DIM}]; "
+             f"got {tuple(t.shape)}")
+    _require(t.dtype == like.dtype and t.device == like.device,
+             f"{name} must have q's type and device")
+    _require(t.numel() == 0 or (t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == HEAD_DIM)
+                                and (t.shape[0] == 1 or t.stride(0) >= t.shape[1] * HEAD_DIM)),
+             f"{name} rows must be contiguous per token")
+
+
+def _token_stride(t):
+    return max(t.stride(0), t.shape[1] * HEAD_DIM)
+
+
+def _check_norm_rope(q, k, q_weight, k_weight, positions, table, eps):
+    _require(q.is_cuda and q.dtype in _DTYPE_CODE, "q must be fp16, bf16 or fp32 on CUDA")
+    _require(q.dim() == 3, "q must be [num_tokens, num_heads, head_dim]")
+    _check_head_rows("q", q, q)
+    _check_head_rows("k", k, q)
+    for w in (q_weight, k_weight):
+        _require(w is None or (w.dtype == q.dtype and w.device == q.device and
+                               tuple(w.shape) == (HEAD_DIM,) and w.is_contiguous()),
+                 f"weights must be [{HEAD_DIM}] of q's type, on q's device")
+    _require(positions.dtype == torch.int32 and positions.device == q.device and
+             positions.is_contiguous() and positions.numel() == q.shape[0],
+             "positions must be int32, one per token, on q's device")
+    _require(table.dtype == torch.float32 and table.device == q.device and table.dim() == 2 and
+             table.is_contiguous() and table.shape[0] > 0, "table must be fp32 [positions, rot_dim]")
+    _require(0 < table.shape[1] <= HEAD_DIM and table.shape[1] % 16 == 0,
+             "rot_dim must be a multiple of 16 up to 128")
+    _require(eps >= 0, "eps must be >= 0")
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, positions, table, *, eps=1e-6, interleaved=False,
+                 q_out=None, k_out=None):
+    """RMS norm of every q and k head and the position rotation, in one launch.
+
+    q [num_tokens, heads, 128] and k [num_tokens, kv_heads, 128] (fp16, bf16 or fp32; views into
+    one projection are fine, each token's rows contiguous); weights [128] of the same type, or
+    None for no norm; positions int32 [num_tokens]; table [positions, rot_dim] fp32 as rope_table
+    makes it: the first rot_dim values of a head turn, value i with i + rot_dim/2, or 2i with
+    2i + 1 when interleaved. fp32 arithmetic, rounded once. Rows of tokens with a negative
+    position (extend_block_tables' padding) are not written: they keep what q_out and k_out held,
+    and are undefined where those are not given. q_out may be q and k_out k. Returns
+    (q_out, k_out)."""
+    _check_norm_rope(q, k, q_weight, k_weight, positions, table, eps)
+    N, H, D = q.shape
+    KVH = k.shape[1]
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
+    _check_head_rows("q_out", q_out, q, H)
+    _check_head_rows("k_out", k_out, q, KVH)
+    with _Guard(q.device):
+        ws = workspace(q.device, 256)
+        rc = _lib.lib().pa_qk_norm_rope(
+            q_out.data_ptr(), _token_stride(q_out), k_out.data_ptr(), _token_stride(k_out),
+            q.data_ptr(), _token_stride(q), k.data_ptr(), _token_stride(k),
+            _DTYPE_CODE[q.dtype], _ptr(q_weight), _ptr(k_weight), float(eps),
+            positions.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1],
+            1 if interleaved else 0, N, H, KVH, D, ws.data_ptr(), _stream(q.device))
+        _lib.check(rc, "qk_norm_rope")
+    return q_out, k_out
+
+
+def norm_rope_into_cache(q, k, v, q_weight, k_weight, positions, table, k_cache, v_cache,
+                         slot_mapping, block_size=16, *, eps=1e-6, interleaved=False,
+                         q_out=None, k_scales=None, v_scales=None):
+    """qk_norm_rope with the new K and the V rows going straight into the paged cache at
+    slot_mapping, in one launch: bit for bit what qk_norm_rope followed by the cache's write
+    (write_into_cache, quantize_into_cache with per-token scales, or quantize_into_cache_fp4)
+    gives. The cache is fp16, int8 or float8_e4m3fn (with k_scales and v_scales), or 4-bit. A
+    negative slot writes nothing to the cache, a negative position skips the token. Returns
+    q_out [num_tokens, heads, 128]; it may be q."""
+    _check_norm_rope(q, k, q_weight, k_weight, positions, table, eps)
+    N, H, D = q.shape
+    KVH = k.shape[1]
+    _check_head_rows("v", v, q, KVH)
+    _check_slots(slot_mapping, N, q.device)
+    kind = _kv_kind(k_cache, k_scales)
+    if kind == "f4":
+        NB, kvh = _check_fp4_caches(k_cache, v_cache, block_size)
+        _require(kvh == KVH, f"the cache has {kvh} kv heads, the rows {KVH}")
+        _require(k_scales is None and v_scales is None, "a 4-bit cache holds its own scales")
+    else:
+        want = {"f16": torch.float16, "i8": torch.int8, "f8": _FP8}[kind]
+        _require(k_cache.dtype == want and v_cache.dtype == want,
+                 "cache must be fp16, int8, float8_e4m3fn or 4-bit, K and V alike")
+        if kind != "f16":
+            _require(k_scales is not None and v_scales is not None and
+                     k_scales.dtype == torch.float32 and v_scales.dtype == torch.float32,
+                     "scales must be fp32")
+        NB = _check_cache_layout(k_cache, v_cache, KVH, D, block_size, k_scales, v_scales)
+    for t in (k_cache, v_cache, k_scales, v_scales):
+        _require(t is None or (t.is_contiguous() and t.device == q.device),
+                 "cache tensors must be contiguous and on q's device")
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
+    _check_head_rows("q_out", q_out, q, H)
+    with _Guard(q.device):
+        ws = workspace(q.device, 256)
+        rc = _lib.lib().pa_norm_rope_into_cache(
+            q_out.data_ptr(), _token_stride(q_out), q.data_ptr(), _token_stride(q),
+            k.data_ptr(), _token_stride(k), v.data_ptr(), _token_stride(v),
+            _DTYPE_CODE[q.dtype], _ptr(q_weight), _ptr(k_weight), float(eps),
+            positions.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1],
+            1 if interleaved else 0, slot_mapping.data_ptr(), N, H, KVH, D, _KV_CODE[kind],
+            k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scales), _ptr(v_scales), NB,
+            block_size, ws.data_ptr(), _stream(q.device))
+        _lib.check(rc, "norm_rope_into_cache")
+    return q_out
+
+
+# ---------------------------------------------------------------------------------------
+# Block tables of a step
+# ---------------------------------------------------------------------------------------
+def _check_tables(block_table, context_lens, per_seq, free_blocks, free_count, block_size):
+    _require(block_table.is_cuda and block_table.dim() == 2,
+             "block_table must be [num_seqs, max_blocks_per_seq] on CUDA")
+    S, max_blocks = block_table.shape
+    _require(max_blocks > 0 and block_size > 0, "max_blocks_per_seq and block_size must be > 0")
+    for name, t, n in (("context_lens", context_lens, S), ("per-sequence values", per_seq, S),
+                       ("free_blocks", free_blocks, None), ("free_count", free_count, 1),
+                       ("block_table", block_table, None)):
+        _require(t.dtype == torch.int32 and t.device == block_table.device and
+                 t.is_contiguous() and (n is None or t.numel() == n),
+                 f"{name} must be contiguous int32 on block_table's device"
+                 + (f", {n} entries" if n is not None else ""))
+    return S, max_blocks
+
+
+def _out_like(t, out, name):
+    out = torch.empty_like(t) if out is None else out
+    _require(out.dtype == torch.int32 and out.shape == t.shape and out.device == t.device and
+             out.is_contiguous(), f"{name} must match its input")
+    return out
+
+
+def release_blocks(block_table, context_lens, finished, free_blocks, free_count, block_size=16,
+                   *, context_lens_out=None, free_count_out=None):
+    """Push the blocks of finished sequences (finished[b] != 0, int32) onto the free stack.
+
+    free_blocks (int32 buffer) holds the free block ids in [0, free_count[0]); blocks go on top in
+    sequence order, by block index. Returns (context_lens, free_count): new tensors, or the given
+    ones, which may be the inputs. Finished sequences get length 0. A call that does not fit
+    (a length past the table, no room in the buffer) changes nothing and sets a status bit
+    (check_status)."""
+    S, max_blocks = _check_tables(block_table, context_lens, finished, free_blocks, free_count,
+                                  block_size)
+    dev = block_table.device
+    lens = _out_like(context_lens, context_lens_out, "context_lens_out")
+    count = _out_like(free_count, free_count_out, "free_count_out")
+    with _Guard(dev):
+        ws = workspace(dev, 256)
+        rc = _lib.lib().pa_release_blocks(
+            block_table.data_ptr(), context_lens.data_ptr(), finished.data_ptr(),
+            free_blocks.data_ptr(), free_count.data_ptr(), lens.data_ptr(), count.data_ptr(), S,
+            max_blocks, block_size, free_blocks.numel(), ws.data_ptr(), _stream(dev))
+        _lib.check(rc, "release_blocks")
+    return lens, count
+
+
+def extend_block_tables(block_table, context_lens, new_lens, free_blocks, free_count, num_blocks,
+                        block_size=16, *, max_tokens, slot_mapping=None, positions=None,
+                        query_start=None, context_lens_out=None, free_count_out=None):
+    """Grow sequence b by new_lens[b] tokens (int32, >= 0): pop the blocks it needs from the free
+    stack (see release_blocks) into its row of block_table, and lay out the step's packed batch.
+
+    Returns (slot_mapping, positions, query_start, context_lens, free_count): for token i of the
+    batch, sequences in order, its cache slot and its position, -1 in both past the last token
+    (both int32 [max_tokens], what the cache writes and qk_norm_rope take); sequence b's tokens
+    are [query_start[b], query_start[b + 1]). context_lens counts the new tokens, as the decodes
+    expect. Nothing is read on the host, so the call can be captured in a CUDA graph. A call that
+    does not fit (lengths past the table, more than max_tokens tokens, too few free blocks)
+    changes nothing, gives slots and positions of -1 and query_start of 0, and sets a status bit
+    (check_status)."""
+    S, max_blocks = _check_tables(block_table, context_lens, new_lens, free_blocks, free_count,
+                                  block_size)
+    dev = block_table.device
+    max_tokens = int(max_tokens)
+    _require(max_tokens >= 0, "max_tokens must be >= 0")
+
+    def int_out(t, n, name):
+        t = torch.empty(n, dtype=torch.int32, device=dev) if t is None else t
+        _require(t.dtype == torch.int32 and t.device == dev and t.is_contiguous() and
+                 t.numel() == n, f"{name} must be contiguous int32 [{n}] on block_table's device")
+        return t
+
+    slot_mapping = int_out(slot_mapping, max_tokens, "slot_mapping")
+    positions = int_out(positions, max_tokens, "positions")
+    query_start = int_out(query_start, S + 1, "query_start")
+    lens = _out_like(context_lens, context_lens_out, "context_lens_out")
+    count = _out_like(free_count, free_count_out, "free_count_out")
+    with _Guard(dev):
+        ws = workspace(dev, 256)
+        rc = _lib.lib().pa_extend_block_tables(
+            block_table.data_ptr(), context_lens.data_ptr(), new_lens.data_ptr(),
+            free_blocks.data_ptr(), free_count.data_ptr(), lens.data_ptr(), count.data_ptr(),
+            slot_mapping.data_ptr(), positions.data_ptr(), query_start.data_ptr(), S, max_blocks,
+            block_size, free_blocks.numel(), num_blocks, max_tokens, ws.data_ptr(), _stream(dev))
+        _lib.check(rc, "extend_block_tables")
+    return slot_mapping, positions, query_start, lens, count
 
 
 def absmax_scale(x, semantics=_lib.PA_SCALE_CLAMP_THEN_DIVIDE):

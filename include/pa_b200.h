@@ -15,6 +15,12 @@
  *   block_table  [num_seqs, max_blocks_per_seq] int32
  *   context_lens [num_seqs] int32
  *   q, out [num_seqs, num_heads, head_dim] fp16 (bf16 with pa_decode_bf16q)
+ *   An fp4 cache (PA_DTYPE_FP4E2M1) holds its scales itself:
+ *   k_cache, v_cache [num_blocks, num_kv_heads, block_size/16, 1152] bytes: a group of 16 tokens
+ *     is 16 rows of 64 code bytes (byte j: head_dim 2j in the low half, 2j + 1 in the high half;
+ *     e2m1 codes 0 .5 1 1.5 2 3 4 6, bit 3 the sign), then a scale byte per 16 head_dim values,
+ *     [16 tokens][8] in the K cache and [8][16 tokens] in the V cache (five exponent bits, bias
+ *     15, three mantissa bits: byte << 7 is its fp16 pattern); value = code * scale.
  * Supported: head_dim 128, block_size a multiple of 16 dividing 128, x = 8, num_heads a
  * multiple of num_kv_heads, num_blocks * num_kv_heads below 2^28 page rows.
  *
@@ -47,6 +53,9 @@ extern "C" {
 #define PA_ERR_TIMEOUT 128      /* device: a bounded wait gave up (about one second) */
 #define PA_ERR_SLOT 256         /* device: a slot_mapping entry outside the cache */
 #define PA_ERR_Q_RANGE 512      /* device: a bf16 q value outside the fp16 range (saturated) */
+#define PA_ERR_FREE_BLOCKS 1024 /* device: too few free blocks, or no room to push more */
+#define PA_ERR_TOKENS 2048      /* device: more new tokens than max_tokens */
+#define PA_ERR_POSITION 4096    /* device: a position outside the rotation table */
 
 /* ---- dtype codes ---- */
 #define PA_DTYPE_F16 0
@@ -54,6 +63,7 @@ extern "C" {
 #define PA_DTYPE_F32 2
 #define PA_DTYPE_I8 3
 #define PA_DTYPE_FP8E4M3 4 /* fp8 e4m3 cache values with per-token fp32 scales */
+#define PA_DTYPE_FP4E2M1 5 /* fp4 e2m1 cache values with a scale byte per 16 values */
 
 /* ---- per-tensor scale semantics for pa_absmax_scale ---- */
 /* quantize_per_tensor (tests/paged_decode_attn.py:115-121): clamp_min(1e-8) in the input
@@ -69,7 +79,7 @@ const char* pa_status_string(int status);
 
 /* ------------------------------------------------------------------------------------
  * Decode workspace size for one call shape on the current device (0 for an unsupported
- * shape). kv_dtype is PA_DTYPE_F16, PA_DTYPE_I8 or PA_DTYPE_FP8E4M3; splitk selects the
+ * shape). kv_dtype is PA_DTYPE_F16, _I8, _FP8E4M3 or _FP4E2M1; splitk selects the
  * split-K partition/reduce pair (nonzero) or the single-pass op (zero).
  * ---------------------------------------------------------------------------------- */
 size_t pa_decode_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads, int head_dim,
@@ -138,6 +148,21 @@ int pa_splitk_fp8(void* out, const void* q, const void* k_cache, const void* v_c
                   const int32_t* context_lens, int num_seqs, int num_heads, int num_kv_heads,
                   int head_dim, int num_blocks, int block_size, int max_blocks_per_seq,
                   float scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* FP4 KV cache (layout above; written by pa_quantize_into_cache_fp4). Same arguments as
+ * pa_decode_f16 / pa_splitk_f16. The other decode entry points (pa_decode_step, pa_decode_bf16q,
+ * pa_decode_partial) take it as kv_dtype PA_DTYPE_FP4E2M1, without scales. No counterpart in the
+ * reference. */
+int pa_decode_fp4(void* out, const void* q, const void* k_cache, const void* v_cache,
+                  const int32_t* block_table, const int32_t* context_lens, int num_seqs,
+                  int num_heads, int num_kv_heads, int head_dim, int num_blocks, int block_size,
+                  int max_blocks_per_seq, float scale, void* workspace, size_t workspace_bytes,
+                  void* stream);
+int pa_splitk_fp4(void* out, const void* q, const void* k_cache, const void* v_cache,
+                  const int32_t* block_table, const int32_t* context_lens, int num_seqs,
+                  int num_heads, int num_kv_heads, int head_dim, int num_blocks, int block_size,
+                  int max_blocks_per_seq, float scale, void* workspace, size_t workspace_bytes,
+                  void* stream);
 
 /* ------------------------------------------------------------------------------------
  * Decode step: append every sequence's new token to the cache, then decode over the whole
@@ -264,6 +289,96 @@ int pa_quantize_into_cache_fp8(const void* k, const void* v, int in_dtype, int64
                                int head_dim, void* k_cache, void* v_cache, float* k_scales,
                                float* v_scales, int num_blocks, int block_size, int* status,
                                void* stream);
+
+/* FP4 write, same rows and slots; rows and caches 16-byte aligned, block_size a multiple of 16.
+ * Per 16 head_dim values:
+ *   scale = the nearest scale byte's value to amax / 6, ties to even, at most 10240
+ *   code  = the nearest e2m1 to x / scale, ties to the even code, magnitudes above 6 as 6
+ * (a zero may carry either sign). A block with a zero scale holds zeros; one with a NaN or an
+ * infinity gets a NaN scale and reads as NaN. No counterpart in the reference. */
+int pa_quantize_into_cache_fp4(const void* k, const void* v, int in_dtype, int64_t token_stride,
+                               const int32_t* slot_mapping, int num_tokens, int num_kv_heads,
+                               int head_dim, void* k_cache, void* v_cache, int num_blocks,
+                               int block_size, int* status, void* stream);
+
+/* Rows read back from an fp4 cache (for instance a cached prefix, for the attention of a prompt's
+ * next chunk): k_out, v_out [num_tokens, num_kv_heads, head_dim] in out_dtype (F16, BF16 or F32; held
+ * values are exact in each). Rows of tokens with a negative slot are left as they are; so are
+ * rows of slots outside the cache, which set PA_ERR_SLOT. */
+int pa_read_from_cache_fp4(void* k_out, void* v_out, int out_dtype, const void* k_cache,
+                           const void* v_cache, const int32_t* slot_mapping, int num_tokens,
+                           int num_kv_heads, int head_dim, int num_blocks, int block_size,
+                           int* status, void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * RMS norm of each q and k head and the position rotation, in one pass:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight        (a null weight: no norm of those rows)
+ *   (a, b) -> (a cos - b sin, b cos + a sin)       over the first rot_dim values of a head
+ * pairing value i with i + rot_dim/2, or 2i with 2i + 1 when interleaved is nonzero. fp32
+ * arithmetic, one rounding to dtype (F16, BF16 or F32; weights have it too).
+ * q [num_tokens, num_heads, head_dim], k [num_tokens, num_kv_heads, head_dim]: rows of a token
+ * contiguous, token strides in elements, all 16-byte aligned; out may be in itself (same rows
+ * and strides), no other overlap. table [table_len, rot_dim] fp32: the cosines of the rot_dim/2
+ * angles of each position, then the sines; rot_dim a multiple of 16 up to 128. positions[i]:
+ * negative skips the token (its outputs are left as they are); one outside the table does too and
+ * sets PA_ERR_POSITION. The reference has no such op: its cache takes K after the rotation.
+ * ---------------------------------------------------------------------------------- */
+int pa_qk_norm_rope(void* q_out, int64_t q_out_stride, void* k_out, int64_t k_out_stride,
+                    const void* q, int64_t q_stride, const void* k, int64_t k_stride, int dtype,
+                    const void* q_weight, const void* k_weight, float eps,
+                    const int32_t* positions, const float* table, int table_len, int rot_dim,
+                    int interleaved, int num_tokens, int num_heads, int num_kv_heads,
+                    int head_dim, int* status, void* stream);
+
+/* The same, with the new K rows and the V rows written into the paged cache at slot_mapping instead of
+ * k_out: cache_dtype F16, I8 (per-token scales), FP8E4M3 or FP4E2M1, bit for bit what
+ * pa_qk_norm_rope followed by that cache's write gives, in one launch. A negative slot writes
+ * nothing to the cache (q_out is still written). */
+int pa_norm_rope_into_cache(void* q_out, int64_t q_out_stride, const void* q, int64_t q_stride,
+                            const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+                            int dtype, const void* q_weight, const void* k_weight, float eps,
+                            const int32_t* positions, const float* table, int table_len,
+                            int rot_dim, int interleaved, const int32_t* slot_mapping,
+                            int num_tokens, int num_heads, int num_kv_heads, int head_dim,
+                            int cache_dtype, void* k_cache, void* v_cache, float* k_scales,
+                            float* v_scales, int num_blocks, int block_size, int* status,
+                            void* stream);
+
+/* ------------------------------------------------------------------------------------
+ * Block tables, slot maps and positions of a serving step, from the requests' lengths, on the
+ * GPU (so that a captured step needs no lengths on the host). The free blocks are a stack,
+ * free_blocks[0 .. free_count[0]) of a buffer of pool_size ids. Both calls change nothing but
+ * their status word (and what they say of refusals below) when the call as a whole does not
+ * fit. status (nullable) receives the refusal's bits.
+ *
+ * Release: the blocks of every sequence with finished[b] != 0 are pushed, in sequence order and
+ * by block index; context_lens_out[b] is 0 for those and context_lens[b] for the others. Refused
+ * with PA_ERR_CONTEXT_RANGE (a finished sequence's length outside its table) or
+ * PA_ERR_FREE_BLOCKS (no room in the buffer).
+ *
+ * Extend: sequence b grows by new_lens[b] >= 0 tokens; blocks are popped from the top in sequence
+ * order and written into its table. Token i of the packed batch (sequence order; sequence b's
+ * are [query_start[b], query_start[b + 1])) gets its position and slot = block * block_size +
+ * position % block_size; entries up to max_tokens past the last are -1 in both. context_lens_out =
+ * context_lens + new_lens. Refused, with slots and positions -1 and query_start 0 throughout, with
+ * PA_ERR_CONTEXT_RANGE (a negative length, or one past the table), PA_ERR_TOKENS (more than
+ * max_tokens) or PA_ERR_FREE_BLOCKS. A block id outside [0, num_blocks) sets PA_ERR_BLOCK_ID and
+ * its tokens' slots are -1.
+ *
+ * context_lens_out and free_count_out may be context_lens and free_count themselves.
+ * ---------------------------------------------------------------------------------- */
+int pa_release_blocks(const int32_t* block_table, const int32_t* context_lens,
+                      const int32_t* finished, int32_t* free_blocks, const int32_t* free_count,
+                      int32_t* context_lens_out, int32_t* free_count_out, int num_seqs,
+                      int max_blocks_per_seq, int block_size, int pool_size, int* status,
+                      void* stream);
+int pa_extend_block_tables(int32_t* block_table, const int32_t* context_lens,
+                           const int32_t* new_lens, const int32_t* free_blocks,
+                           const int32_t* free_count, int32_t* context_lens_out,
+                           int32_t* free_count_out, int32_t* slot_mapping, int32_t* positions,
+                           int32_t* query_start, int num_seqs, int max_blocks_per_seq,
+                           int block_size, int pool_size, int num_blocks, int max_tokens,
+                           int* status, void* stream);
 
 /* FP16 copy-into-cache (no quantisation), same slot semantics: the fp16 cache write of
  * PagedKVCache.decode_append / build_paged_kv_cache (paged_cache.py:147-150,

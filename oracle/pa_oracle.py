@@ -416,3 +416,147 @@ class BridgeCacheOracle:
             self.v_scales[blk, :, off] = vs
         self.length = t + 1
         return t + 1
+
+
+# ---------------------------------------------------------------------------------------
+# The 4-bit cache (no counterpart in the reference): e2m1 codes, a scale byte per 16 values
+# ---------------------------------------------------------------------------------------
+FP4_VALUES = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+FP4_SCALE_MAX = 0xE2  # 10240
+FP4_SCALE_NAN = 0xFF
+FP4_GROUP_BYTES = 1152
+
+
+def fp4_scale_values():
+    """Values of all 256 scale bytes: five exponent bits (bias 15), three mantissa bits."""
+    b = np.arange(256, dtype=np.uint16)
+    return (b << 7).view(np.float16).astype(np.float64)
+
+
+def _nearest_even(t, grid):
+    """Index of the nearest entry of the ascending grid to each t; ties to the even index."""
+    mid = (grid[1:] + grid[:-1]) / 2  # exact: grid entries have few significant bits
+    lo = np.searchsorted(mid, t, side="left")
+    hi = np.searchsorted(mid, t, side="right")
+    return np.where((lo != hi) & (lo % 2 == 1), hi, lo)
+
+
+def quantize_fp4(x):
+    """Codes [..., 128] (0..15) and scale bytes [..., 8] of rows x [..., 128], in 64 bits."""
+    x = np.asarray(x, dtype=np.float64)
+    xb = x.reshape(x.shape[:-1] + (8, 16))
+    with np.errstate(invalid="ignore"):
+        amax = np.abs(xb).max(-1)
+        bad = ~np.isfinite(xb).all(-1)
+    grid = fp4_scale_values()[:FP4_SCALE_MAX + 1]
+    scales = _nearest_even(np.where(bad, 0.0, amax) / 6.0, grid)
+    s = grid[scales][..., None]
+    with np.errstate(invalid="ignore", divide="ignore"):
+        y = np.where((s > 0) & np.isfinite(xb), np.abs(xb) / s, 0.0)
+    codes = _nearest_even(y, FP4_VALUES) | (((xb < 0) & (s > 0)).astype(np.int64) << 3)
+    scales = np.where(bad, FP4_SCALE_NAN, scales).astype(np.uint8)
+    return codes.reshape(x.shape).astype(np.uint8), scales
+
+
+def dequantize_fp4(codes, scales):
+    """fp64 rows [..., 128] of codes and scale bytes (a NaN scale reads as NaN)."""
+    v = FP4_VALUES[codes & 7] * np.where(codes & 8, -1.0, 1.0)
+    return v * np.repeat(fp4_scale_values()[scales], 16, axis=-1)
+
+
+def _fp4_views(cache, is_v):
+    """(code bytes [NB, KVH, G, 16, 64], scale bytes [NB, KVH, G, 16 tokens, 8]) views."""
+    c = cache[..., :1024].reshape(cache.shape[:3] + (16, 64))
+    s = cache[..., 1024:]
+    s = s.reshape(cache.shape[:3] + ((8, 16) if is_v else (16, 8)))
+    return c, s.swapaxes(-1, -2) if is_v else s
+
+
+def fp4_put(cache, is_v, rows, slots, block_size):
+    """Write rows [N, KVH, 128] at slots [N] (negative: skipped) into a uint8 cache
+    [NB, KVH, block_size/16, 1152], in place."""
+    codes, scales = quantize_fp4(rows)
+    packed = codes[..., 0::2] | (codes[..., 1::2] << 4)
+    for i, slot in enumerate(np.asarray(slots)):
+        if slot < 0:
+            continue
+        b, off = divmod(int(slot), block_size)
+        g, t = divmod(off, 16)
+        cache[b, :, g, t * 64:(t + 1) * 64] = packed[i]
+        for j in range(8):
+            cache[b, :, g, 1024 + (j * 16 + t if is_v else t * 8 + j)] = scales[i, :, j]
+
+
+def fp4_values(cache, is_v):
+    """fp64 values [NB, KVH, block_size, 128] a cache holds."""
+    c, s = _fp4_views(cache, is_v)
+    codes = np.stack([c & 15, c >> 4], -1).reshape(c.shape[:-1] + (128,))
+    v = dequantize_fp4(codes, np.ascontiguousarray(s))
+    return v.reshape(cache.shape[:2] + (-1, 128))
+
+
+def fp4_decode(q, k_cache, v_cache, block_table, context_lens, scale):
+    """Decode attention over a 4-bit cache in 64 bits. Returns out [S, H, 128] and, per
+    sequence, the largest sum_d |q_d k_d| * scale and the largest |v| (what rounding errors of
+    the scores and the weights are measured by)."""
+    S, H, D = q.shape
+    KVH = k_cache.shape[1]
+    out, qk, vmax = np.zeros((S, H, D)), np.zeros(S), np.zeros(S)
+    for b in range(S):
+        n = int(context_lens[b])
+        bs = k_cache.shape[2] * 16
+        pages = block_table[b, :-(-n // bs)]
+        k = fp4_values(k_cache[pages], False).transpose(1, 0, 2, 3).reshape(KVH, -1, D)[:, :n]
+        v = fp4_values(v_cache[pages], True).transpose(1, 0, 2, 3).reshape(KVH, -1, D)[:, :n]
+        qb = q[b].astype(np.float64).reshape(KVH, H // KVH, D)
+        s = np.einsum("kgd,knd->kgn", qb, k) * scale
+        p = np.exp(s - s.max(-1, keepdims=True))
+        p /= p.sum(-1, keepdims=True)
+        out[b] = np.einsum("kgn,knd->kgd", p, v).reshape(H, D)
+        qk[b] = abs(scale) * np.einsum("kgd,knd->kgn", np.abs(qb), np.abs(k)).max()
+        vmax[b] = np.abs(v).max()
+    return out, qk, vmax
+
+
+# ---------------------------------------------------------------------------------------
+# Norm and rotation, block tables (no counterparts in the reference)
+# ---------------------------------------------------------------------------------------
+def norm_rope(x, weight, positions, table, eps, interleaved):
+    """RMS norm (weight None: none) and rotation of rows x [N, heads, 128], in 64 bits."""
+    x = np.asarray(x, dtype=np.float64)
+    if weight is not None:
+        x = x / np.sqrt((x * x).mean(-1, keepdims=True) + eps) * np.asarray(weight, np.float64)
+    rot = table.shape[1]
+    i = np.arange(rot // 2)
+    a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + rot // 2)
+    cs = np.asarray(table, np.float64)[np.asarray(positions)]
+    c, s = cs[:, None, :rot // 2], cs[:, None, rot // 2:]
+    y = x.copy()
+    y[..., a] = x[..., a] * c - x[..., b] * s
+    y[..., b] = x[..., b] * c + x[..., a] * s
+    return y
+
+
+def release_blocks(table, lens, finished, free, bs):
+    """free: list used as a stack. Returns the new lengths; pushes the finished blocks."""
+    lens = list(lens)
+    for b in range(len(lens)):
+        if finished[b]:
+            free.extend(int(x) for x in table[b, :-(-lens[b] // bs)])
+            lens[b] = 0
+    return lens
+
+
+def extend_tables(table, lens, new, free, bs):
+    """Grow every sequence, popping blocks off `free`. Returns slots, positions, starts, lens."""
+    lens, slots, pos, starts = list(lens), [], [], [0]
+    for b in range(len(lens)):
+        for _ in range(int(new[b])):
+            p = lens[b]
+            if p % bs == 0:
+                table[b, p // bs] = free.pop()
+            slots.append(int(table[b, p // bs]) * bs + p % bs)
+            pos.append(p)
+            lens[b] += 1
+        starts.append(len(slots))
+    return slots, pos, starts, lens
