@@ -69,8 +69,8 @@ struct Tile {
   static constexpr bool F4 = KVK == 3;    // fp4 e2m1 values, a scale per 16 (fp4.cuh)
   static constexpr bool BYTE = I8 || F8;  // one-byte elements (the INT8 page layout)
   static constexpr int ELEM = BYTE ? 1 : 2;
-  static constexpr int KT = F4 ? fp4::kGroupBytes : D * kSubTokens * ELEM;  // K tile bytes
-  static constexpr int VT = KT;                                             // V tile bytes
+  static constexpr int KT = D * kSubTokens * ELEM;  // K tile bytes
+  static constexpr int VT = D * kSubTokens * ELEM;  // V tile bytes
   // Scale tiles: 16 K scales at +0 and 16 V scales at +128 (tensor-copy destinations are
   // kept 128-byte aligned); 128 bytes of them are transferred per stage.
   static constexpr int ST = BYTE ? 256 : 0;
@@ -79,12 +79,15 @@ struct Tile {
   static constexpr int MT = D / 16;                 // PV m-tiles (head_dim rows)
   static constexpr int NT = GT / 8;                 // PV n-tiles (heads)
   static constexpr int SLOT = (D + 2) * GT;         // partial slot floats
-  static constexpr size_t SMEM = 1024 + (size_t)WARPS * DEPTH * (KT + VT + ST) +
-                                 (size_t)WARPS * DEPTH * 8;
+  // The page ring: WARPS x DEPTH stages of one 16-token page, or for FP4 of two (K, K, V, V).
+  static constexpr int PT = F4 ? fp4::kGroupBytes : 0;  // FP4 page bytes, K or V
+  static constexpr size_t RING =
+      F4 ? (size_t)WARPS * DEPTH * 4 * PT : (size_t)WARPS * DEPTH * (KT + VT + ST);
+  static constexpr size_t SMEM = 1024 + RING + (size_t)WARPS * DEPTH * 8;
   // Decode step launches: per stage, the new token's K and V rows (16-bit) when the stage's
   // page holds a sequence's new token.
   static constexpr int NR = 2 * D * 2;
-  static constexpr size_t SMEM_STEP = SMEM + 16 + (size_t)WARPS * DEPTH * NR;
+  static constexpr size_t SMEM_STEP = F4 ? SMEM : SMEM + 16 + (size_t)WARPS * DEPTH * NR;
 };
 
 // ---------------------------------------------------------------------------------------
@@ -361,37 +364,8 @@ __device__ __noinline__ void stage_new_token(const uint8_t* rk, uint8_t* kt, uin
                                              const float* vfix, void* kc, void* vc, float* ks,
                                              float* vs, int bs) {
   static_assert(D == 128, "one lane per four head_dim values");
-  constexpr bool BYTE = KVK == 1 || KVK == 2;
+  constexpr bool BYTE = KVK != 0;
   constexpr int KIND = KVK == 1 ? kRowsI8 : (KVK == 2 ? kRowsFP8 : kRowsF16);
-  if constexpr (KVK == 3) {
-    // The staged tile and the cache hold the group in the same layout.
-    uint8_t* kg = static_cast<uint8_t*>(kc) + fp4::group_offset((size_t)row, off, bs);
-    uint8_t* vg = static_cast<uint8_t*>(vc) + fp4::group_offset((size_t)row, off, bs);
-#pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      float x[4];
-      const uint8_t* src = rk + which * D * 2;
-      if (new_dtype == PA_DTYPE_BF16) {
-        load_vals<__nv_bfloat16, 4>(reinterpret_cast<const __nv_bfloat16*>(src) + 4 * lane, x);
-      } else {
-        load_vals<__half, 4>(reinterpret_cast<const __half*>(src) + 4 * lane, x);
-      }
-      uint32_t sb;
-      const uint32_t w = fp4::warp_quantize4<false>(x, sb);
-      uint8_t* tile = which ? vt : kt;
-      uint8_t* grp = which ? vg : kg;
-      const int co = t * fp4::kCodeRow + 2 * lane;
-      const int so = fp4::scale_offset(which != 0, t, lane >> 2);
-      *reinterpret_cast<uint16_t*>(tile + co) = (uint16_t)w;
-      *reinterpret_cast<uint16_t*>(grp + co) = (uint16_t)w;
-      if ((lane & 3) == 0) {
-        tile[so] = (uint8_t)sb;
-        grp[so] = (uint8_t)sb;
-      }
-    }
-    __syncwarp();
-    return;
-  }
   RowQ<KIND, D> qk, qv;
   if (new_dtype == PA_DTYPE_BF16) {
     qk = warp_quantize_row<__nv_bfloat16, KIND, D>(reinterpret_cast<const __nv_bfloat16*>(rk),
@@ -424,6 +398,36 @@ __device__ __noinline__ void stage_new_token(const uint8_t* rk, uint8_t* kt, uin
   }
   store_row(qk, lane, false, kc, ks, (size_t)row, off, bs);
   store_row(qv, lane, true, vc, vs, (size_t)row, off, bs);
+  __syncwarp();
+}
+
+// ---------------------------------------------------------------------------------------
+// Decode step over a 4-bit cache: one warp quantises the new token's K and V rows (16-bit, at
+// src_k / src_v) and stores them into the cache, at token `off` of page row `row`, before it
+// loads the page. Only the calling warp reads the page.
+// ---------------------------------------------------------------------------------------
+template <int D>
+__device__ __noinline__ void store_new_token_fp4(const uint8_t* src_k, const uint8_t* src_v,
+                                                 int new_dtype, uint8_t* kc, uint8_t* vc,
+                                                 size_t row, int off, int bs, int lane) {
+  static_assert(D == 128, "one lane per four head_dim values");
+  const size_t grp = fp4::group_offset(row, off, bs);
+  const int t = off % fp4::kGroupTokens;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const uint8_t* src = which ? src_v : src_k;
+    float x[4];
+    if (new_dtype == PA_DTYPE_BF16) {
+      load_vals<__nv_bfloat16, 4>(reinterpret_cast<const __nv_bfloat16*>(src) + 4 * lane, x);
+    } else {
+      load_vals<__half, 4>(reinterpret_cast<const __half*>(src) + 4 * lane, x);
+    }
+    uint32_t sb;
+    const uint32_t w = fp4::warp_quantize4<false>(x, sb);
+    uint8_t* dst = (which ? vc : kc) + grp;
+    *reinterpret_cast<uint16_t*>(dst + t * fp4::kCodeRow + 2 * lane) = (uint16_t)w;
+    if ((lane & 3) == 0) dst[fp4::scale_offset(which != 0, t, lane >> 2)] = (uint8_t)sb;
+  }
   __syncwarp();
 }
 
@@ -465,7 +469,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   uint8_t* k_tiles = dsm;
   uint8_t* v_tiles = k_tiles + WARPS * DEPTH * C::KT;
   uint8_t* s_tiles = v_tiles + WARPS * DEPTH * C::VT;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_tiles + WARPS * DEPTH * C::ST);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(dsm + C::RING);
   // New-token rows of a decode step (allocated only for step launches).
   uint8_t* r_tiles = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(bars + WARPS * DEPTH) + 15) & ~uintptr_t(15));
@@ -773,6 +777,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       blk = 0;
       wr = -1;
     }
+    if constexpr (F4)  // index of the 16-token group (below 2^31)
+      return (blk * a.KVH + (meta >> 3)) * a.subs + (meta & 7);
     return ((blk * a.KVH + (meta >> 3)) << 3) | (meta & 7);
   };
   // The block ids of the next 32 pages are copied into shared memory in the background
@@ -797,8 +803,72 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   int curw, meta0;
   const int* bref0 = page_ref(0, meta0, curw);
   const int blk0 = bref0 != nullptr ? __ldg(bref0) : 0;
-  prefetch_batch(32);  // requested before the first batch's ids are waited for
+  if constexpr (!F4) prefetch_batch(32);  // requested before the first batch's ids are waited for
   int cur = pack_page(blk0, meta0, curw);
+
+  // FP4, decode step: the new token in the page of group gi, if it holds one (sequence wb >= 0),
+  // is written into the cache before the page is copied.
+  auto write_new = [&](uint32_t gi, int wb) {
+    if (wb < 0) return;
+    const uint32_t row = gi / (uint32_t)a.subs;
+    const size_t so = ((size_t)wb * a.new_stride + (size_t)(row % (uint32_t)a.KVH) * D) * 2;
+    store_new_token_fp4<D>(static_cast<const uint8_t*>(a.new_k) + so,
+                           static_cast<const uint8_t*>(a.new_v) + so, a.new_dtype,
+                           static_cast<uint8_t*>(a.kc_w), static_cast<uint8_t*>(a.vc_w), row,
+                           (s_ctx[wb] - 1) % a.bs, a.bs, lane);
+    __threadfence();  // the copies read what the warp has just written, from L2
+  };
+  // FP4: the warp's ring is filled by 16-byte asynchronous copies of all its lanes, one commit
+  // group per stage of two pages. (Four bulk copies per stage, issued by one lane, cost 87 of the
+  // step's 640 instructions; nine copies a lane and their addresses cost about 25.) A page's K
+  // and V groups are 72 chunks each: two rounds of the warp, and the last eight chunks of all
+  // four groups in one more round.
+  [[maybe_unused]] const uint32_t f4base =
+      smem_u32(k_tiles) + (uint32_t)(warp * DEPTH) * 4u * (uint32_t)C::PT;
+  [[maybe_unused]] const uint8_t* k_lane = a.k_base + 16 * lane;
+  [[maybe_unused]] const uint8_t* v_lane = a.v_base + 16 * lane;
+  [[maybe_unused]] const uint8_t* rest_lane =
+      ((lane & 16) ? a.v_base : a.k_base) + 1024 + 16 * (lane & 7);
+  [[maybe_unused]] const uint32_t rest_off =
+      (uint32_t)(lane >> 3) * (uint32_t)C::PT + 1024u + 16u * (uint32_t)(lane & 7);
+  // Pages jj and jj + 1 (jj even; asked for in order) into stage s; past the range's end the
+  // group is empty, and a missing second page is the first once more. The ids of the next 32
+  // pages come along with a batch's first stage, sixteen groups before they are needed.
+  auto issue_pair = [&](int jj, int s) {
+    if (jj < n) {
+      if ((jj & 31) == 0) {
+        if (jj > 0) {
+          curw = s_nwr[warp][lane];
+          cur = pack_page(s_nblk[warp][lane], s_nmeta[warp][lane], curw);
+        }
+        int meta, wr;
+        const int* p = page_ref(jj + 32, meta, wr);
+        s_nmeta[warp][lane] = meta;
+        s_nwr[warp][lane] = wr;
+        if (p != nullptr) cp_async_4(&s_nblk[warp][lane], p);
+      }
+      const int i1 = (jj & 31) + (jj + 1 < n ? 1 : 0);
+      const uint32_t g0 = __shfl_sync(0xffffffffu, (uint32_t)cur, jj & 31);
+      const uint32_t g1 = __shfl_sync(0xffffffffu, (uint32_t)cur, i1);
+      if (step_write) {
+        write_new(g0, __shfl_sync(0xffffffffu, curw, jj & 31));
+        write_new(g1, __shfl_sync(0xffffffffu, curw, i1));
+      }
+      const uint32_t st = f4base + (uint32_t)s * 4u * (uint32_t)C::PT + 16u * (uint32_t)lane;
+      const size_t o0 = (size_t)g0 * C::PT, o1 = (size_t)g1 * C::PT;
+      cp_async_16_hint(st, k_lane + o0, pol);
+      cp_async_16_hint(st + 512, k_lane + o0 + 512, pol);
+      cp_async_16_hint(st + C::PT, k_lane + o1, pol);
+      cp_async_16_hint(st + C::PT + 512, k_lane + o1 + 512, pol);
+      cp_async_16_hint(st + 2 * C::PT, v_lane + o0, pol);
+      cp_async_16_hint(st + 2 * C::PT + 512, v_lane + o0 + 512, pol);
+      cp_async_16_hint(st + 3 * C::PT, v_lane + o1, pol);
+      cp_async_16_hint(st + 3 * C::PT + 512, v_lane + o1 + 512, pol);
+      cp_async_16_hint(st - 16u * (uint32_t)lane + rest_off,
+                       rest_lane + (size_t)((lane & 8) ? g1 : g0) * C::PT, pol);
+    }
+    cp_async_commit();
+  };
 
   auto issue = [&](int j, int s) {
     if (j > 0 && (j & 31) == 0) {
@@ -827,12 +897,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         }
       }
       // The cache pages stream through L2 marked evict-first.
-      if constexpr (F4) {  // a group of 16 tokens is contiguous, whatever the block size
-        const size_t o = ((size_t)row * a.subs + sub) * C::KT;
-        bulk_g2s_hint(kd, a.k_base + o, C::KT, bar, pol);
-        bulk_g2s_hint(vd, a.v_base + o, C::VT, bar, pol);
-        return;
-      }
       if constexpr (BYTE) {
         tma_load_3d_hint(kd, &tm_k, bar, sub * 128, 0, row, pol);
       } else {
@@ -859,8 +923,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   static_assert(DEPTH < 32, "the prologue copies must come from the first batch of block ids");
   const int npro = n < DEPTH ? n : DEPTH;
   __syncwarp();
-  for (int j = 0; j < npro; ++j) issue(j, j);
   int issued = npro;
+  if constexpr (F4) {
+    issued = 0;
+    for (int j = 0; j < DEPTH; ++j) issue_pair(2 * j, j);
+  } else {
+    for (int j = 0; j < npro; ++j) issue(j, j);
+  }
   convert_q();
 
   // Shared-memory offsets of the K cells this lane reads (chunk of load si, token of n-tile
@@ -871,9 +940,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
     for (int jt = 0; jt < 2; ++jt) {
       const int tau = 4 * (g >> 1) + (g & 1) + 2 * jt;
-      if constexpr (F4) {
-        koff[si][jt] = 0;  // one 16-byte load a token, addressed directly
-      } else if constexpr (BYTE) {
+      if constexpr (BYTE) {
         const int c = chunk_i8(r, si);
         koff[si][jt] = c * 128 + ((((tau >> 1) ^ (c & 7)) << 4) | ((tau & 1) << 3));
       } else {
@@ -903,6 +970,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   // head_dim of O's row g (hi = 0) and g + 8 (hi = 1) of m-tile i.
   auto drow = [&](int i, int hi) { return F4 ? 16 * g + 2 * i + hi : 16 * i + g + 8 * hi; };
 
+  // FP4: running maximum and sum of heads nt * 8 + 2r and the next.
+  [[maybe_unused]] float fm[NT][2], fl[NT][2], fmb[NT][2];  // fmb = kPExp - fm
+  [[maybe_unused]] const int tau = 4 * (g >> 1) + (g & 1);  // token of K row g (row g + 8: + 2)
   int jfail = -1;
   int s = 0;        // ring stage of page j
   uint32_t ph = 0;  // its mbarrier phase parity
@@ -945,6 +1015,204 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) oacc[i][nt][e] = 0.f;
 
+    if constexpr (F4) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          fm[nt][e] = neg_inf();
+          fmb[nt][e] = -neg_inf();
+          fl[nt][e] = 0.f;
+        }
+      // A stage's two pages per step; where a piece begins or ends inside a stage, the page that
+      // is not its own is masked (and met again by the other piece).
+      for (int k = 0; k < len;) {
+        const int first = j & 1;
+        const int cnt = min(2 - first, len - k);
+        if (first == 0) {  // the stage's copies: this lane's, then every lane's
+          cp_async_wait_groups<DEPTH - 1>();
+          __syncwarp();
+        }
+        const int left = cctx - (csp + k) * kSubTokens;  // tokens from the step's first page on
+        const int valid0 = first ? 0 : min(kSubTokens, left);
+        const int valid1 = first ? min(kSubTokens, left)
+                                 : (cnt == 2 ? min(kSubTokens, left - kSubTokens) : 0);
+        const bool full = valid0 == kSubTokens && valid1 == kSubTokens;
+        const uint32_t st = f4base + (uint32_t)s * 4u * (uint32_t)C::PT;
+        const uint32_t ka = st + tau * fp4::kCodeRow + 16 * r;
+        const uint32_t ksa = st + fp4::kCodes + tau * 8 + 2 * r;
+        const uint32_t va = st + 2 * C::PT + 4 * r * fp4::kCodeRow + 8 * g;
+        const uint32_t vsa = st + 2 * C::PT + fp4::kCodes + 16 * g + 4 * r;
+
+        // S^T = K Q^T: rows = tokens (row g: token tau, row g + 8: tau + 2), columns = heads, so
+        // that eight heads fill the MMA. A lane reads the 32 codes 32r .. 32r + 31 of its two
+        // tokens; codes -> fp16, times the block scale, is exact (fp4.cuh).
+        float x[2][NT][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint4 c0 = lds128(ka + u * C::PT), c1 = lds128(ka + u * C::PT + 2 * fp4::kCodeRow);
+          const uint32_t z0 = lds16(ksa + u * C::PT), z1 = lds16(ksa + u * C::PT + 16);
+          const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
+          const uint32_t s0 = fp4::scale_pair(z0), s1 = fp4::scale_pair(z1);
+          float acc[2][NT][4];  // even and odd steps: two shorter chains
+          auto mma = [](bool begin, float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                        uint32_t a3, uint32_t b0, uint32_t b1) {
+            if (begin) mma_16816_zero(d, a0, a1, a2, a3, b0, b1);
+            else mma_16816(d, a0, a1, a2, a3, b0, b1);
+          };
+#pragma unroll
+          for (int si = 0; si < NS; ++si) {
+            uint32_t h[4], i4[4];
+            fp4::codes_to_f16x2(w0[si], h[0], h[1], h[2], h[3]);
+            fp4::codes_to_f16x2(w1[si], i4[0], i4[1], i4[2], i4[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              h[e] = si < NS / 2 ? fp4::hmul2_half<false>(h[e], s0)
+                                 : fp4::hmul2_half<true>(h[e], s0);
+              i4[e] = si < NS / 2 ? fp4::hmul2_half<false>(i4[e], s1)
+                                  : fp4::hmul2_half<true>(i4[e], s1);
+            }
+            mma(si == 0, acc[0][0], h[0], i4[0], h[1], i4[1], qa[si].x, qa[si].y);
+            mma(si == 0, acc[1][0], h[2], i4[2], h[3], i4[3], qa[si].z, qa[si].w);
+            if constexpr (NT == 2) {
+              mma(si == 0, acc[0][1], h[0], i4[0], h[1], i4[1], qb[si].x, qb[si].y);
+              mma(si == 0, acc[1][1], h[2], i4[2], h[3], i4[3], qb[si].z, qb[si].w);
+            }
+          }
+          // Logits in log2 units: heads nt * 8 + 2r + (e & 1) of token tau (e < 2) and tau + 2.
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              const float2 v = mul2(add2(make_float2(acc[0][nt][e], acc[0][nt][e + 1]),
+                                         make_float2(acc[1][nt][e], acc[1][nt][e + 1])),
+                                    make_float2(qs, qs));
+              x[u][nt][e] = v.x;
+              x[u][nt][e + 1] = v.y;
+            }
+        }
+        if (!full) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int vd = u ? valid1 : valid0;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (tau + (e & 2) >= vd) x[u][nt][e] = neg_inf();
+          }
+        }
+        // The reference maximum moves only when a score passes it by 2^kLazy: weights then stay
+        // below 2^(kPExp + kLazy) (far inside fp16), O and l carry the same factor, and most
+        // steps need neither a reduction over the lanes nor a rescale.
+        constexpr float kLazy = 8.f;
+        float tm[NT][2];
+        bool up = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            tm[nt][e] = fmaxf(fmaxf(x[0][nt][e], x[0][nt][2 + e]),
+                              fmaxf(x[1][nt][e], x[1][nt][2 + e]));
+            up = up || tm[nt][e] > fm[nt][e] + kLazy;
+          }
+        if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float c[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float v = tm[nt][e];
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+              c[e] = v > fm[nt][e] ? ex2(fm[nt][e] - v) : 1.f;
+              fm[nt][e] = fmaxf(v, fm[nt][e]);
+              fmb[nt][e] = kPExp - fm[nt][e];
+              fl[nt][e] *= c[e];
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {  // O's columns are the lane's own heads
+              oacc[i][nt][0] *= c[0];
+              oacc[i][nt][1] *= c[1];
+              oacc[i][nt][2] *= c[0];
+              oacc[i][nt][3] *= c[1];
+            }
+          }
+        }
+
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          // Weights, as two fp16 parts each (about 22 significant bits, as for the other
+          // caches); the transposed 8 x 8 tiles are the PV MMA's B fragments.
+          uint32_t ph0[NT], ph1[NT], pl0[NT], pl1[NT];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              const float2 v = add2(make_float2(x[u][nt][e], x[u][nt][e + 1]),
+                                    make_float2(fmb[nt][0], fmb[nt][1]));
+              p[e] = ex2(v.x);
+              p[e + 1] = ex2(v.y);
+              const float2 l = add2(make_float2(fl[nt][0], fl[nt][1]),
+                                    make_float2(p[e], p[e + 1]));
+              fl[nt][0] = l.x;
+              fl[nt][1] = l.y;
+            }
+            split_f16x2_packed(p[0], p[1], ph0[nt], pl0[nt]);
+            split_f16x2_packed(p[2], p[3], ph1[nt], pl1[nt]);
+            ph0[nt] = transpose8x8(ph0[nt]);
+            ph1[nt] = transpose8x8(ph1[nt]);
+            pl0[nt] = transpose8x8(pl0[nt]);
+            pl1[nt] = transpose8x8(pl1[nt]);
+          }
+          // V: tokens 4r .. 4r + 3, values 16g .. 16g + 15 (one block a token). Scales of slots
+          // past the context may be anything: zero there (a finite code times zero is 0).
+          uint2 vq[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vq[e] = lds64(va + u * C::PT + e * fp4::kCodeRow);
+          const uint32_t z = lds32(vsa + u * C::PT);
+          uint32_t s01 = fp4::scale_pair(z), s23 = fp4::scale_pair(z, 0x3424u);
+          if (!full) {
+            const int vd = u ? valid1 : valid0;
+            s01 &= ((4 * r < vd) ? 0x0000ffffu : 0u) | ((4 * r + 1 < vd) ? 0xffff0000u : 0u);
+            s23 &= ((4 * r + 2 < vd) ? 0x0000ffffu : 0u) | ((4 * r + 3 < vd) ? 0xffff0000u : 0u);
+          }
+          // O^T += V^T P^T. The MMA pairs tokens: the even and the odd head_dim codes of two
+          // tokens share a byte before they convert. Rows g and g + 8 of m-tile 4h + jj are
+          // head_dim 16g + 8h + 2jj and the next.
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t w0 = h ? vq[0].y : vq[0].x, w1 = h ? vq[1].y : vq[1].x;
+            const uint32_t w2 = h ? vq[2].y : vq[2].x, w3 = h ? vq[3].y : vq[3].x;
+            constexpr uint32_t kLow = 0x0f0f0f0fu;
+            uint32_t A0[4], A1[4], A2[4], A3[4];
+            fp4::codes_to_f16x2((w0 & kLow) | ((w1 << 4) & ~kLow), A0[0], A0[1], A0[2], A0[3]);
+            fp4::codes_to_f16x2(((w0 >> 4) & kLow) | (w1 & ~kLow), A1[0], A1[1], A1[2], A1[3]);
+            fp4::codes_to_f16x2((w2 & kLow) | ((w3 << 4) & ~kLow), A2[0], A2[1], A2[2], A2[3]);
+            fp4::codes_to_f16x2(((w2 >> 4) & kLow) | (w3 & ~kLow), A3[0], A3[1], A3[2], A3[3]);
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+              const int i = 4 * h + jj;
+              const uint32_t a0 = fp4::hmul2(A0[jj], s01), a1 = fp4::hmul2(A1[jj], s01);
+              const uint32_t a2 = fp4::hmul2(A2[jj], s23), a3 = fp4::hmul2(A3[jj], s23);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma_16816(oacc[i][nt], a0, a1, a2, a3, ph0[nt], ph1[nt]);
+                mma_16816(oacc[i][nt], a0, a1, a2, a3, pl0[nt], pl1[nt]);
+              }
+            }
+          }
+        }
+        k += cnt;
+        j += cnt;
+        if ((j & 1) == 0) {  // both pages of the stage are done with: refill it
+          __syncwarp();
+          issue_pair(j + 2 * DEPTH - 2, s);
+          if (++s == DEPTH) s = 0;
+        }
+      }
+    } else {
     for (int k = 0; k < len; ++k) {
     if (!mbar_wait_bounded(&wbar[s], ph, a.status)) {
       jfail = j;
@@ -967,22 +1235,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     uint32_t v8[MT][2];
     uint2 v16[MT][2];
     float4 ksv = make_float4(0.f, 0.f, 0.f, 0.f), vsv = ksv;
-    // FP4: tokens 4 (g / 2) + g % 2 + 2 jt of K (values 32 r .. 32 r + 31: one block scale a
-    // half), tokens 4r .. 4r + 3 of V (values 16 g .. 16 g + 15: one block scale a token).
-    uint4 k4[2];
-    uint2 v4[4];
-    uint32_t k4s[2], v4s = 0u;
-    if constexpr (F4) {
-#pragma unroll
-      for (int jt = 0; jt < 2; ++jt) {
-        const int tau = 4 * (g >> 1) + (g & 1) + 2 * jt;
-        k4[jt] = lds128(kb + tau * fp4::kCodeRow + 16 * r);
-        k4s[jt] = lds16(kb + fp4::kCodes + tau * 8 + 2 * r);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v4[e] = lds64(vb + (4 * r + e) * fp4::kCodeRow + 8 * g);
-      v4s = lds32(vb + fp4::kCodes + 16 * g + 4 * r);
-    } else {
 #pragma unroll
     for (int si = 0; si < NS; ++si) {
 #pragma unroll
@@ -1000,7 +1252,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         v16[i][0] = lds64(vb + voff + i * 512);
         v16[i][1] = lds64(vb + voff + i * 512 + 256);
       }
-    }
     }
     if constexpr (BYTE) {
       ksv = lds128f(sb + 16 * r);
@@ -1094,24 +1345,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
               e4m3x4_to_f16x2x2(k8[si][jt].x, k16[si][jt].x, k16[si][jt].y);
               e4m3x4_to_f16x2x2(k8[si][jt].y, k16[si][jt].z, k16[si][jt].w);
             }
-        }
-        if constexpr (F4) {
-          // Codes -> fp16, times the block scale: exact (fp4.cuh).
-#pragma unroll
-          for (int jt = 0; jt < 2; ++jt) {
-            const uint32_t w[4] = {k4[jt].x, k4[jt].y, k4[jt].z, k4[jt].w};
-            const uint32_t sc[2] = {(k4s[jt] & 0xffu) * 0x00800080u,
-                                    (k4s[jt] >> 8) * 0x00800080u};
-#pragma unroll
-            for (int si = 0; si < NS; ++si) {
-              uint4& h = k16[si][jt];
-              fp4::codes_to_f16x2(w[si], h.x, h.y, h.z, h.w);
-              h.x = fp4::hmul2(h.x, sc[si >> 1]);
-              h.y = fp4::hmul2(h.y, sc[si >> 1]);
-              h.z = fp4::hmul2(h.z, sc[si >> 1]);
-              h.w = fp4::hmul2(h.w, sc[si >> 1]);
-            }
-          }
         }
         // Two accumulation chains per n-tile (even / odd si) shorten the MMA dependency.
         float sacc[2][2][4];
@@ -1252,51 +1485,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         split_f16x2(py[2], py[3], pc1, pm1);
       }
 
-      // FP4: the lane's V scales of tokens (4r, 4r + 1) and (4r + 2, 4r + 3); zero past the
-      // context, where the bytes may be anything (a finite code times zero is zero).
-      uint32_t vs01 = 0u, vs23 = 0u;
-      uint32_t vlo01[2], vhi01[2], vlo23[2], vhi23[2];
-      if constexpr (F4) {
-        vs01 = prmt(v4s, 0u, 0x4140u) << 7;
-        vs23 = prmt(v4s, 0u, 0x4342u) << 7;
-        if (valid < kSubTokens) {
-          vs01 &= ((4 * r < valid) ? 0x0000ffffu : 0u) | ((4 * r + 1 < valid) ? 0xffff0000u : 0u);
-          vs23 &= ((4 * r + 2 < valid) ? 0x0000ffffu : 0u) |
-                  ((4 * r + 3 < valid) ? 0xffff0000u : 0u);
-        }
-        // The MMA pairs tokens: the even and odd head_dim codes of two tokens, a byte each.
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t w0 = h ? v4[0].y : v4[0].x, w1 = h ? v4[1].y : v4[1].x;
-          const uint32_t w2 = h ? v4[2].y : v4[2].x, w3 = h ? v4[3].y : v4[3].x;
-          vlo01[h] = (w0 & 0x0f0f0f0fu) | ((w1 << 4) & 0xf0f0f0f0u);
-          vhi01[h] = ((w0 >> 4) & 0x0f0f0f0fu) | (w1 & 0xf0f0f0f0u);
-          vlo23[h] = (w2 & 0x0f0f0f0fu) | ((w3 << 4) & 0xf0f0f0f0u);
-          vhi23[h] = ((w2 >> 4) & 0x0f0f0f0fu) | (w3 & 0xf0f0f0f0u);
-        }
-        // O^T rows g and g + 8 of m-tile 4h + j are head_dim 16 g + 8 h + 2 j and the next.
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t A0[4], A1[4], A2[4], A3[4];
-          fp4::codes_to_f16x2(vlo01[h], A0[0], A0[1], A0[2], A0[3]);
-          fp4::codes_to_f16x2(vhi01[h], A1[0], A1[1], A1[2], A1[3]);
-          fp4::codes_to_f16x2(vlo23[h], A2[0], A2[1], A2[2], A2[3]);
-          fp4::codes_to_f16x2(vhi23[h], A3[0], A3[1], A3[2], A3[3]);
-#pragma unroll
-          for (int jj = 0; jj < 4; ++jj) {
-            const int i = 4 * h + jj;
-            const uint32_t a0 = fp4::hmul2(A0[jj], vs01), a1 = fp4::hmul2(A1[jj], vs01);
-            const uint32_t a2 = fp4::hmul2(A2[jj], vs23), a3 = fp4::hmul2(A3[jj], vs23);
-            mma_16816(oacc[i][0], a0, a1, a2, a3, pb0, pb1);
-            mma_16816(oacc[i][0], a0, a1, a2, a3, pl0, pl1);
-            if constexpr (NT == 2) {
-              mma_16816(oacc[i][1], a0, a1, a2, a3, pc0, pc1);
-              mma_16816(oacc[i][1], a0, a1, a2, a3, pm0, pm1);
-            }
-          }
-        }
-      }
-
       // O^T += V^T P^T : rows = head_dim (16 per m-tile), columns = heads.
       uint32_t mlo = 0xffffffffu, mhi = 0xffffffffu;
       if (!I8 && valid < kSubTokens) {
@@ -1304,7 +1492,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         mhi = ((4 * r + 2 < valid) ? 0x0000ffffu : 0u) | ((4 * r + 3 < valid) ? 0xffff0000u : 0u);
       }
 #pragma unroll
-      for (int i = 0; i < (F4 ? 0 : MT); ++i) {
+      for (int i = 0; i < MT; ++i) {
         uint32_t a0, a1, a2, a3;
         if constexpr (I8) {
           i8x4_to_f16x2x2(v8[i][0], a0, a2);
@@ -1338,11 +1526,21 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       ph ^= 1u;
     }
     }  // pages of the piece
+    }
     if (jfail >= 0) break;
     csp += len;
 
     {
       // ---- piece epilogue ---------------------------------------------------------------------
+      if constexpr (F4) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1)
+              fl[nt][e] += __shfl_xor_sync(0xffffffffu, fl[nt][e], o);
+      }
       float lt0 = l0 + __shfl_xor_sync(0xffffffffu, l0, 1);
       lt0 += __shfl_xor_sync(0xffffffffu, lt0, 2);
       float lt1 = 0.f;
@@ -1369,7 +1567,17 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
                 make_float2(oacc[i][nt][2] * kUnscale, oacc[i][nt][3] * kUnscale);
           }
         }
-        if (r == 0) {
+        if constexpr (F4) {
+          if (g == 0) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              *reinterpret_cast<float2*>(slot + D * GT + nt * 8 + 2 * r) =
+                  make_float2(fm[nt][0], fm[nt][1]);
+              *reinterpret_cast<float2*>(slot + D * GT + GT + nt * 8 + 2 * r) =
+                  make_float2(fl[nt][0] * kUnscale, fl[nt][1] * kUnscale);
+            }
+          }
+        } else if (r == 0) {
           slot[D * GT + g] = m0;
           slot[D * GT + GT + g] = lt0 * kUnscale;
           if constexpr (NT == 2) {
@@ -1384,11 +1592,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       } else if (piece_sp0 == 0 && csp == cpg) {
         // The whole segment was this warp's: normalise and store directly.
         if (a.mode == kModeStream) {
-          const float inv0 = 1.f / lt0;
-          const float ia = __shfl_sync(0xffffffffu, inv0, 8 * r);
-          const float ib = __shfl_sync(0xffffffffu, inv0, 8 * r + 4);
-          float ic = 0.f, id = 0.f;
-          if constexpr (NT == 2) {
+          float ia, ib, ic = 0.f, id = 0.f;
+          if constexpr (F4) {
+            ia = 1.f / fl[0][0];
+            ib = 1.f / fl[0][1];
+            ic = 1.f / fl[NT - 1][0];
+            id = 1.f / fl[NT - 1][1];
+          } else {
+            const float inv0 = 1.f / lt0;
+            ia = __shfl_sync(0xffffffffu, inv0, 8 * r);
+            ib = __shfl_sync(0xffffffffu, inv0, 8 * r + 4);
+          }
+          if constexpr (NT == 2 && !F4) {
             const float inv1 = 1.f / lt1;
             ic = __shfl_sync(0xffffffffu, inv1, 8 * r);
             id = __shfl_sync(0xffffffffu, inv1, 8 * r + 4);
@@ -1460,6 +1675,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     }
   }
 
+  if constexpr (F4) cp_async_wait_all();
   if (jfail >= 0) {
     // Let copies still in flight land before the CTA's shared memory is released.
     for (int jj = jfail; jj < issued; ++jj) {
@@ -1490,7 +1706,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     s_npend[warp] = k;
   }
   __syncthreads();  // every warp is past its page loop: the ring memory is free
-  constexpr size_t kRing = (size_t)WARPS * DEPTH * (C::KT + C::VT + C::ST);
+  constexpr size_t kRing = C::RING;
   constexpr int kStageCap = (int)(kRing / (SLOT * sizeof(float)));
   float* scratch = reinterpret_cast<float*>(k_tiles);
   const bool stream = (a.mode == kModeStream);
@@ -1618,10 +1834,10 @@ template <> struct Shape<2, 16> { static constexpr int W = 8, DP = 4; };
 #define PA_F4_WARPS 12
 #endif
 #ifndef PA_F4_DEPTH
-#define PA_F4_DEPTH 4
+#define PA_F4_DEPTH 3
 #endif
 template <> struct Shape<3, 8> { static constexpr int W = PA_F4_WARPS, DP = PA_F4_DEPTH; };
-template <> struct Shape<3, 16> { static constexpr int W = 8, DP = 6; };
+template <> struct Shape<3, 16> { static constexpr int W = 8, DP = 4; };
 
 template <int KVK, int GT>
 cudaError_t launch_one(const DecodeArgs& a, const CUtensorMap* maps, int grid,

@@ -111,6 +111,20 @@ __device__ __forceinline__ void codes_to_f16x2(uint32_t w, uint32_t& h0, uint32_
       : "r"(w));
 }
 
+// Two scale bytes of z as two fp16 scales: bytes 0 and 1, or 2 and 3 with sel 0x3424.
+__device__ __forceinline__ uint32_t scale_pair(uint32_t z, uint32_t sel = 0x1404u) {
+  return prmt(z, 0u, sel) >> 1;  // b << 8 in each half, shifted down to b << 7
+}
+
+// a times the low or the high half of s (the multiply takes the half as an operand modifier).
+template <bool kHigh>
+__device__ __forceinline__ uint32_t hmul2_half(uint32_t a, uint32_t s) {
+  const __half2 s2 = *reinterpret_cast<const __half2*>(&s);
+  const __half2 d = __hmul2(*reinterpret_cast<const __half2*>(&a),
+                            kHigh ? __high2half2(s2) : __low2half2(s2));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
