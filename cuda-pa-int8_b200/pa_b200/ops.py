@@ -30,7 +30,13 @@ def _ptr(t):
     return t.data_ptr() if t is not None else None
 
 
+# The current stream's handle without building a Stream object, which costs 2 us a call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(device):
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
 
 
@@ -144,12 +150,15 @@ def _check_lengths(context_lens, capacity, host_context_lens=None):
 
 def _check_fp4_caches(k_cache, v_cache, block_size):
     """(num_blocks, kv_heads) of 4-bit caches [num_blocks, kv_heads, block_size/16, 1152]."""
-    for name, t in (("k_cache", k_cache), ("v_cache", v_cache)):
-        _require(t.dtype == torch.uint8 and t.dim() == 4 and t.shape[3] == FP4_GROUP_BYTES and
-                 t.shape[2] * FP4_GROUP_TOKENS == block_size and t.shape == k_cache.shape,
-                 f"{name} of a 4-bit cache must be uint8 [num_blocks, kv_heads, block_size/16, "
-                 f"{FP4_GROUP_BYTES}]; got {t.dtype} {tuple(t.shape)}")
-    return k_cache.shape[0], k_cache.shape[1]
+    shape = k_cache.shape
+    if not (k_cache.dtype == torch.uint8 and v_cache.dtype == torch.uint8 and
+            v_cache.shape == shape and len(shape) == 4 and shape[3] == FP4_GROUP_BYTES and
+            shape[2] * FP4_GROUP_TOKENS == block_size):
+        raise RuntimeError(
+            f"a 4-bit cache is uint8 [num_blocks, kv_heads, block_size/16, {FP4_GROUP_BYTES}], K "
+            f"and V alike; got {k_cache.dtype} {tuple(shape)} and {v_cache.dtype} "
+            f"{tuple(v_cache.shape)} for block_size {block_size}")
+    return shape[0], shape[1]
 
 
 def _check_decode_args(out, q, k_cache, v_cache, block_table, context_lens, block_size,
@@ -663,12 +672,19 @@ def fp4_cache(num_blocks, num_kv_heads, block_size=16, device="cuda"):
                  for _ in range(2))
 
 
+# The checks of the calls below are written out as single conditions: they run once per launch of
+# kernels that take a few microseconds.
 def _check_slots(slot_mapping, num_tokens, device):
-    _require(slot_mapping.dtype == torch.int32 and slot_mapping.is_cuda,
-             "slot_mapping must be int32 on CUDA")
-    _require(slot_mapping.numel() == num_tokens and slot_mapping.is_contiguous() and
-             slot_mapping.device == device,
-             "slot_mapping must be contiguous, with one entry per token, on the rows' device")
+    if not (slot_mapping.dtype == torch.int32 and slot_mapping.device == device and
+            slot_mapping.numel() == num_tokens and slot_mapping.is_contiguous()):
+        raise RuntimeError("slot_mapping must be contiguous int32 with one entry per token, on the "
+                           "rows' CUDA device")
+
+
+def _check_on(device, *tensors):
+    for t in tensors:
+        if t is not None and not (t.device == device and t.is_contiguous()):
+            raise RuntimeError("cache tensors must be contiguous and on the rows' device")
 
 
 def quantize_into_cache_fp4(key, value, k_cache, v_cache, slot_mapping, block_size=16):
@@ -679,22 +695,25 @@ def quantize_into_cache_fp4(key, value, k_cache, v_cache, slot_mapping, block_si
     even; a value becomes the nearest of 0, .5, 1, 1.5, 2, 3, 4, 6 times it, ties to the even
     code. A block holding a NaN or an infinity reads back as NaN. Two tokens with the same slot
     in one call leave a mixture of their blocks there."""
-    _check_rows(key, value)
-    N, KVH, D = key.shape
-    _require(D == HEAD_DIM, f"head_dim {D} unsupported (this build: {HEAD_DIM})")
-    _check_slots(slot_mapping, N, key.device)
+    dev, dt = key.device, key.dtype
+    if not (key.is_cuda and dt in _DTYPE_CODE and value.dtype == dt and value.device == dev):
+        raise RuntimeError("key/value must both be fp16, bf16 or fp32, on one CUDA device")
+    shape, stride = key.shape, key.stride()
+    if not (len(shape) == 3 and value.shape == shape and shape[2] == HEAD_DIM):
+        raise RuntimeError("key/value must be [num_tokens, num_kv_heads, 128]")
+    N, KVH, D = shape
+    if not (stride[2] == 1 and stride[1] == D and value.stride() == stride):
+        raise RuntimeError("key/value rows must be contiguous")
+    _check_slots(slot_mapping, N, dev)
     NB, kvh = _check_fp4_caches(k_cache, v_cache, block_size)
-    _require(kvh == KVH, f"the cache has {kvh} kv heads, the rows {KVH}")
-    for t in (value, k_cache, v_cache):
-        _require(t.device == key.device, "all tensors must be on the same CUDA device")
-    for t in (k_cache, v_cache):
-        _require(t.is_contiguous(), "cache tensors must be contiguous")
-    with _Guard(key.device):
-        ws = workspace(key.device, 256)
+    if kvh != KVH:
+        raise RuntimeError(f"the cache has {kvh} kv heads, the rows {KVH}")
+    _check_on(dev, k_cache, v_cache)
+    with _Guard(dev):
         rc = _lib.lib().pa_quantize_into_cache_fp4(
-            key.data_ptr(), value.data_ptr(), _DTYPE_CODE[key.dtype], key.stride(0),
+            key.data_ptr(), value.data_ptr(), _DTYPE_CODE[dt], stride[0],
             slot_mapping.data_ptr(), N, KVH, D, k_cache.data_ptr(), v_cache.data_ptr(), NB,
-            block_size, ws.data_ptr(), _stream(key.device))
+            block_size, workspace(dev, 256).data_ptr(), _stream(dev))
         _lib.check(rc, "quantize_into_cache (fp4)")
 
 
@@ -704,28 +723,30 @@ def read_from_cache_fp4(k_cache, v_cache, slot_mapping, block_size=16, *, dtype=
     at slot_mapping, for instance a cached prefix for the attention of a prompt's next chunk.
     Held values are exact in fp16, bf16 and fp32. Rows of negative slots are not written: they
     keep what `out`, a pair of tensors to write into, held, and are undefined without it."""
-    _require(k_cache.is_cuda and v_cache.is_cuda, "tensors must be on CUDA")
+    dev = k_cache.device
+    if not k_cache.is_cuda:
+        raise RuntimeError("tensors must be on CUDA")
     NB, KVH = _check_fp4_caches(k_cache, v_cache, block_size)
     N = slot_mapping.numel()
-    _check_slots(slot_mapping, N, k_cache.device)
-    _require(v_cache.device == k_cache.device and k_cache.is_contiguous() and
-             v_cache.is_contiguous(), "cache tensors must be contiguous and on one device")
+    _check_slots(slot_mapping, N, dev)
+    _check_on(dev, k_cache, v_cache)
     if out is None:
-        _require(dtype in _DTYPE_CODE, "dtype must be fp16, bf16 or fp32")
-        out = tuple(torch.empty(N, KVH, HEAD_DIM, dtype=dtype, device=k_cache.device)
-                    for _ in range(2))
-    key, value = out
-    for t in (key, value):
-        _require(t.dtype in _DTYPE_CODE and t.dtype == key.dtype and t.device == k_cache.device and
-                 tuple(t.shape) == (N, KVH, HEAD_DIM) and t.is_contiguous(),
-                 f"out must be two contiguous [{N}, {KVH}, {HEAD_DIM}] tensors of one type on the "
-                 "cache's device")
-    with _Guard(k_cache.device):
-        ws = workspace(k_cache.device, 256)
+        if dtype not in _DTYPE_CODE:
+            raise RuntimeError("dtype must be fp16, bf16 or fp32")
+        key = torch.empty((N, KVH, HEAD_DIM), dtype=dtype, device=dev)
+        value = torch.empty_like(key)
+    else:
+        key, value = out
+        for t in (key, value):
+            if not (t.dtype in _DTYPE_CODE and t.dtype == key.dtype and t.device == dev and
+                    tuple(t.shape) == (N, KVH, HEAD_DIM) and t.is_contiguous()):
+                raise RuntimeError(f"out must be two contiguous [{N}, {KVH}, {HEAD_DIM}] tensors "
+                                   "of one type on the cache's device")
+    with _Guard(dev):
         rc = _lib.lib().pa_read_from_cache_fp4(
             key.data_ptr(), value.data_ptr(), _DTYPE_CODE[key.dtype], k_cache.data_ptr(),
             v_cache.data_ptr(), slot_mapping.data_ptr(), N, KVH, HEAD_DIM, NB, block_size,
-            ws.data_ptr(), _stream(k_cache.device))
+            workspace(dev, 256).data_ptr(), _stream(dev))
         _lib.check(rc, "read_from_cache (fp4)")
     return key, value
 
@@ -742,42 +763,46 @@ def rope_table(num_positions, rot_dim=HEAD_DIM, base=10000.0, device="cuda"):
     return torch.cat([ang.cos(), ang.sin()], 1).float()
 
 
-def _check_head_rows(name, t, like, heads=None):
-    """[num_tokens, heads, 128] rows, contiguous per token; like: a tensor whose tokens, type
-    and device they share."""
-    _require(t.is_cuda, "tensors must be on CUDA")
-    _require(t.dim() == 3 and t.shape[2] == HEAD_DIM and t.shape[0] == like.shape[0] and
-             (heads is None or t.shape[1] == heads),
-             f"{name} must be [{like.shape[0]}, {heads or 'heads'}, {HEAD_DIM}]; "
-             f"got {tuple(t.shape)}")
-    _require(t.dtype == like.dtype and t.device == like.device,
-             f"{name} must have q's type and device")
-    _require(t.numel() == 0 or (t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == HEAD_DIM)
-                                and (t.shape[0] == 1 or t.stride(0) >= t.shape[1] * HEAD_DIM)),
-             f"{name} rows must be contiguous per token")
-
-
-def _token_stride(t):
-    return max(t.stride(0), t.shape[1] * HEAD_DIM)
+def _head_rows(name, t, tokens, heads, dtype, device):
+    """Number of heads and token stride of rows [tokens, heads, 128], contiguous per token."""
+    shape, stride = t.shape, t.stride()
+    if not (len(shape) == 3 and shape[0] == tokens and shape[2] == HEAD_DIM and
+            (heads is None or shape[1] == heads) and t.dtype == dtype and t.device == device):
+        raise RuntimeError(f"{name} must be [{tokens}, {heads or 'heads'}, {HEAD_DIM}] of q's type "
+                           f"on q's device; got {t.dtype} {tuple(shape)} on {t.device}")
+    H = shape[1]
+    row = H * HEAD_DIM
+    if row == 0 or tokens == 0:
+        return H, row
+    if not (stride[2] == 1 and (H == 1 or stride[1] == HEAD_DIM) and
+            (tokens == 1 or stride[0] >= row)):
+        raise RuntimeError(f"{name} rows must be contiguous per token")
+    return H, stride[0] if tokens > 1 else row
 
 
 def _check_norm_rope(q, k, q_weight, k_weight, positions, table, eps):
-    _require(q.is_cuda and q.dtype in _DTYPE_CODE, "q must be fp16, bf16 or fp32 on CUDA")
-    _require(q.dim() == 3, "q must be [num_tokens, num_heads, head_dim]")
-    _check_head_rows("q", q, q)
-    _check_head_rows("k", k, q)
+    dev, dt = q.device, q.dtype
+    if not (q.is_cuda and dt in _DTYPE_CODE and q.dim() == 3):
+        raise RuntimeError("q must be fp16, bf16 or fp32 [num_tokens, num_heads, 128] on CUDA")
+    N = q.shape[0]
+    H, qs = _head_rows("q", q, N, None, dt, dev)
+    KVH, ks = _head_rows("k", k, N, None, dt, dev)
     for w in (q_weight, k_weight):
-        _require(w is None or (w.dtype == q.dtype and w.device == q.device and
-                               tuple(w.shape) == (HEAD_DIM,) and w.is_contiguous()),
-                 f"weights must be [{HEAD_DIM}] of q's type, on q's device")
-    _require(positions.dtype == torch.int32 and positions.device == q.device and
-             positions.is_contiguous() and positions.numel() == q.shape[0],
-             "positions must be int32, one per token, on q's device")
-    _require(table.dtype == torch.float32 and table.device == q.device and table.dim() == 2 and
-             table.is_contiguous() and table.shape[0] > 0, "table must be fp32 [positions, rot_dim]")
-    _require(0 < table.shape[1] <= HEAD_DIM and table.shape[1] % 16 == 0,
-             "rot_dim must be a multiple of 16 up to 128")
-    _require(eps >= 0, "eps must be >= 0")
+        if w is not None and not (w.dtype == dt and w.device == dev and w.dim() == 1 and
+                                  w.numel() == HEAD_DIM and w.is_contiguous()):
+            raise RuntimeError(f"weights must be [{HEAD_DIM}] of q's type, on q's device")
+    if not (positions.dtype == torch.int32 and positions.device == dev and
+            positions.numel() == N and positions.is_contiguous()):
+        raise RuntimeError("positions must be int32, one per token, on q's device")
+    size = table.shape
+    if not (table.dtype == torch.float32 and table.device == dev and len(size) == 2 and
+            size[0] > 0 and table.is_contiguous()):
+        raise RuntimeError("table must be fp32 [positions, rot_dim] on q's device")
+    if not (0 < size[1] <= HEAD_DIM and size[1] % 16 == 0):
+        raise RuntimeError("rot_dim must be a multiple of 16 up to 128")
+    if not eps >= 0:
+        raise RuntimeError("eps must be >= 0")
+    return N, H, qs, KVH, ks
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, positions, table, *, eps=1e-6, interleaved=False,
@@ -792,21 +817,24 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, table, *, eps=1e-6, interl
     position (extend_block_tables' padding) are not written: they keep what q_out and k_out held,
     and are undefined where those are not given. q_out may be q and k_out k. Returns
     (q_out, k_out)."""
-    _check_norm_rope(q, k, q_weight, k_weight, positions, table, eps)
-    N, H, D = q.shape
-    KVH = k.shape[1]
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device) if k_out is None else k_out
-    _check_head_rows("q_out", q_out, q, H)
-    _check_head_rows("k_out", k_out, q, KVH)
-    with _Guard(q.device):
-        ws = workspace(q.device, 256)
+    N, H, qs, KVH, ks = _check_norm_rope(q, k, q_weight, k_weight, positions, table, eps)
+    dev, dt = q.device, q.dtype
+    if q_out is None:
+        q_out = torch.empty((N, H, HEAD_DIM), dtype=dt, device=dev)
+        qos = H * HEAD_DIM
+    else:
+        _, qos = _head_rows("q_out", q_out, N, H, dt, dev)
+    if k_out is None:
+        k_out = torch.empty((N, KVH, HEAD_DIM), dtype=dt, device=dev)
+        kos = KVH * HEAD_DIM
+    else:
+        _, kos = _head_rows("k_out", k_out, N, KVH, dt, dev)
+    with _Guard(dev):
         rc = _lib.lib().pa_qk_norm_rope(
-            q_out.data_ptr(), _token_stride(q_out), k_out.data_ptr(), _token_stride(k_out),
-            q.data_ptr(), _token_stride(q), k.data_ptr(), _token_stride(k),
-            _DTYPE_CODE[q.dtype], _ptr(q_weight), _ptr(k_weight), float(eps),
-            positions.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1],
-            1 if interleaved else 0, N, H, KVH, D, ws.data_ptr(), _stream(q.device))
+            q_out.data_ptr(), qos, k_out.data_ptr(), kos, q.data_ptr(), qs, k.data_ptr(), ks,
+            _DTYPE_CODE[dt], _ptr(q_weight), _ptr(k_weight), eps, positions.data_ptr(),
+            table.data_ptr(), table.shape[0], table.shape[1], 1 if interleaved else 0, N, H, KVH,
+            HEAD_DIM, workspace(dev, 256).data_ptr(), _stream(dev))
         _lib.check(rc, "qk_norm_rope")
     return q_out, k_out
 
@@ -820,16 +848,17 @@ def norm_rope_into_cache(q, k, v, q_weight, k_weight, positions, table, k_cache,
     gives. The cache is fp16, int8 or float8_e4m3fn (with k_scales and v_scales), or 4-bit. A
     negative slot writes nothing to the cache, a negative position skips the token. Returns
     q_out [num_tokens, heads, 128]; it may be q."""
-    _check_norm_rope(q, k, q_weight, k_weight, positions, table, eps)
-    N, H, D = q.shape
-    KVH = k.shape[1]
-    _check_head_rows("v", v, q, KVH)
-    _check_slots(slot_mapping, N, q.device)
+    N, H, qs, KVH, ks = _check_norm_rope(q, k, q_weight, k_weight, positions, table, eps)
+    dev, dt = q.device, q.dtype
+    _, vs = _head_rows("v", v, N, KVH, dt, dev)
+    _check_slots(slot_mapping, N, dev)
     kind = _kv_kind(k_cache, k_scales)
     if kind == "f4":
         NB, kvh = _check_fp4_caches(k_cache, v_cache, block_size)
-        _require(kvh == KVH, f"the cache has {kvh} kv heads, the rows {KVH}")
-        _require(k_scales is None and v_scales is None, "a 4-bit cache holds its own scales")
+        if kvh != KVH:
+            raise RuntimeError(f"the cache has {kvh} kv heads, the rows {KVH}")
+        if not (k_scales is None and v_scales is None):
+            raise RuntimeError("a 4-bit cache holds its own scales")
     else:
         want = {"f16": torch.float16, "i8": torch.int8, "f8": _FP8}[kind]
         _require(k_cache.dtype == want and v_cache.dtype == want,
@@ -838,22 +867,21 @@ def norm_rope_into_cache(q, k, v, q_weight, k_weight, positions, table, k_cache,
             _require(k_scales is not None and v_scales is not None and
                      k_scales.dtype == torch.float32 and v_scales.dtype == torch.float32,
                      "scales must be fp32")
-        NB = _check_cache_layout(k_cache, v_cache, KVH, D, block_size, k_scales, v_scales)
-    for t in (k_cache, v_cache, k_scales, v_scales):
-        _require(t is None or (t.is_contiguous() and t.device == q.device),
-                 "cache tensors must be contiguous and on q's device")
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device) if q_out is None else q_out
-    _check_head_rows("q_out", q_out, q, H)
-    with _Guard(q.device):
-        ws = workspace(q.device, 256)
+        NB = _check_cache_layout(k_cache, v_cache, KVH, HEAD_DIM, block_size, k_scales, v_scales)
+    _check_on(dev, k_cache, v_cache, k_scales, v_scales)
+    if q_out is None:
+        q_out = torch.empty((N, H, HEAD_DIM), dtype=dt, device=dev)
+        qos = H * HEAD_DIM
+    else:
+        _, qos = _head_rows("q_out", q_out, N, H, dt, dev)
+    with _Guard(dev):
         rc = _lib.lib().pa_norm_rope_into_cache(
-            q_out.data_ptr(), _token_stride(q_out), q.data_ptr(), _token_stride(q),
-            k.data_ptr(), _token_stride(k), v.data_ptr(), _token_stride(v),
-            _DTYPE_CODE[q.dtype], _ptr(q_weight), _ptr(k_weight), float(eps),
-            positions.data_ptr(), table.data_ptr(), table.shape[0], table.shape[1],
-            1 if interleaved else 0, slot_mapping.data_ptr(), N, H, KVH, D, _KV_CODE[kind],
-            k_cache.data_ptr(), v_cache.data_ptr(), _ptr(k_scales), _ptr(v_scales), NB,
-            block_size, ws.data_ptr(), _stream(q.device))
+            q_out.data_ptr(), qos, q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs,
+            _DTYPE_CODE[dt], _ptr(q_weight), _ptr(k_weight), eps, positions.data_ptr(),
+            table.data_ptr(), table.shape[0], table.shape[1], 1 if interleaved else 0,
+            slot_mapping.data_ptr(), N, H, KVH, HEAD_DIM, _KV_CODE[kind], k_cache.data_ptr(),
+            v_cache.data_ptr(), _ptr(k_scales), _ptr(v_scales), NB, block_size,
+            workspace(dev, 256).data_ptr(), _stream(dev))
         _lib.check(rc, "norm_rope_into_cache")
     return q_out
 
@@ -861,26 +889,27 @@ def norm_rope_into_cache(q, k, v, q_weight, k_weight, positions, table, k_cache,
 # ---------------------------------------------------------------------------------------
 # Block tables of a step
 # ---------------------------------------------------------------------------------------
+def _int_row(name, t, n, device):
+    """t is a contiguous int32 vector of n entries (None: any number) on the device."""
+    if not (t.dtype == torch.int32 and t.device == device and t.dim() == 1 and
+            (n is None or t.numel() == n) and t.is_contiguous()):
+        raise RuntimeError(f"{name} must be a contiguous int32 vector"
+                           + (f" of {n}" if n is not None else "") + " on block_table's device")
+
+
 def _check_tables(block_table, context_lens, per_seq, free_blocks, free_count, block_size):
-    _require(block_table.is_cuda and block_table.dim() == 2,
-             "block_table must be [num_seqs, max_blocks_per_seq] on CUDA")
-    S, max_blocks = block_table.shape
-    _require(max_blocks > 0 and block_size > 0, "max_blocks_per_seq and block_size must be > 0")
-    for name, t, n in (("context_lens", context_lens, S), ("per-sequence values", per_seq, S),
-                       ("free_blocks", free_blocks, None), ("free_count", free_count, 1),
-                       ("block_table", block_table, None)):
-        _require(t.dtype == torch.int32 and t.device == block_table.device and
-                 t.is_contiguous() and (n is None or t.numel() == n),
-                 f"{name} must be contiguous int32 on block_table's device"
-                 + (f", {n} entries" if n is not None else ""))
-    return S, max_blocks
-
-
-def _out_like(t, out, name):
-    out = torch.empty_like(t) if out is None else out
-    _require(out.dtype == torch.int32 and out.shape == t.shape and out.device == t.device and
-             out.is_contiguous(), f"{name} must match its input")
-    return out
+    dev, shape = block_table.device, block_table.shape
+    if not (block_table.is_cuda and len(shape) == 2 and block_table.dtype == torch.int32 and
+            block_table.is_contiguous()):
+        raise RuntimeError("block_table must be contiguous int32 [num_seqs, max_blocks_per_seq] on "
+                           "CUDA")
+    if not (shape[1] > 0 and block_size > 0):
+        raise RuntimeError("max_blocks_per_seq and block_size must be > 0")
+    _int_row("context_lens", context_lens, shape[0], dev)
+    _int_row("the per-sequence values", per_seq, shape[0], dev)
+    _int_row("free_blocks", free_blocks, None, dev)
+    _int_row("free_count", free_count, 1, dev)
+    return shape[0], shape[1], dev
 
 
 def release_blocks(block_table, context_lens, finished, free_blocks, free_count, block_size=16,
@@ -892,11 +921,12 @@ def release_blocks(block_table, context_lens, finished, free_blocks, free_count,
     ones, which may be the inputs. Finished sequences get length 0. A call that does not fit
     (a length past the table, no room in the buffer) changes nothing and sets a status bit
     (check_status)."""
-    S, max_blocks = _check_tables(block_table, context_lens, finished, free_blocks, free_count,
-                                  block_size)
-    dev = block_table.device
-    lens = _out_like(context_lens, context_lens_out, "context_lens_out")
-    count = _out_like(free_count, free_count_out, "free_count_out")
+    S, max_blocks, dev = _check_tables(block_table, context_lens, finished, free_blocks,
+                                       free_count, block_size)
+    lens = torch.empty_like(context_lens) if context_lens_out is None else context_lens_out
+    count = torch.empty_like(free_count) if free_count_out is None else free_count_out
+    _int_row("context_lens_out", lens, S, dev)
+    _int_row("free_count_out", count, 1, dev)
     with _Guard(dev):
         ws = workspace(dev, 256)
         rc = _lib.lib().pa_release_blocks(
@@ -921,23 +951,22 @@ def extend_block_tables(block_table, context_lens, new_lens, free_blocks, free_c
     does not fit (lengths past the table, more than max_tokens tokens, too few free blocks)
     changes nothing, gives slots and positions of -1 and query_start of 0, and sets a status bit
     (check_status)."""
-    S, max_blocks = _check_tables(block_table, context_lens, new_lens, free_blocks, free_count,
-                                  block_size)
-    dev = block_table.device
+    S, max_blocks, dev = _check_tables(block_table, context_lens, new_lens, free_blocks,
+                                       free_count, block_size)
     max_tokens = int(max_tokens)
-    _require(max_tokens >= 0, "max_tokens must be >= 0")
-
-    def int_out(t, n, name):
-        t = torch.empty(n, dtype=torch.int32, device=dev) if t is None else t
-        _require(t.dtype == torch.int32 and t.device == dev and t.is_contiguous() and
-                 t.numel() == n, f"{name} must be contiguous int32 [{n}] on block_table's device")
-        return t
-
-    slot_mapping = int_out(slot_mapping, max_tokens, "slot_mapping")
-    positions = int_out(positions, max_tokens, "positions")
-    query_start = int_out(query_start, S + 1, "query_start")
-    lens = _out_like(context_lens, context_lens_out, "context_lens_out")
-    count = _out_like(free_count, free_count_out, "free_count_out")
+    if max_tokens < 0:
+        raise RuntimeError("max_tokens must be >= 0")
+    outs = [slot_mapping, positions, query_start, context_lens_out, free_count_out]
+    sizes = [max_tokens, max_tokens, S + 1, S, 1]
+    if not any(t is not None for t in outs):  # one allocation, split
+        outs = torch.empty(sum(sizes), dtype=torch.int32, device=dev).split(sizes)
+    else:
+        names = ("slot_mapping", "positions", "query_start", "context_lens_out", "free_count_out")
+        for i, n in enumerate(sizes):
+            if outs[i] is None:
+                outs[i] = torch.empty(n, dtype=torch.int32, device=dev)
+            _int_row(names[i], outs[i], n, dev)
+    slot_mapping, positions, query_start, lens, count = outs
     with _Guard(dev):
         ws = workspace(dev, 256)
         rc = _lib.lib().pa_extend_block_tables(
