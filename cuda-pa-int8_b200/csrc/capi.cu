@@ -273,7 +273,7 @@ int decode_impl(int mode, int kv_i8, void* out, float* part_out, const void* q,
                 const float* v_scales, const int32_t* block_table, const int32_t* context_lens,
                 int B, int H, int KVH, int D, int NB, int bs, int max_blocks, float scale,
                 void* workspace, size_t workspace_bytes, void* stream,
-                const StepWrite* sw = nullptr) {
+                const StepWrite* sw = nullptr, bool act_bf16 = false) {
   int rc = check_common(B, H, KVH, D, NB, bs, max_blocks);
   if (rc != PA_OK) return rc;
   if (B == 0) return PA_OK;
@@ -352,6 +352,7 @@ int decode_impl(int mode, int kv_i8, void* out, float* part_out, const void* q,
     a.block_table = block_table + (size_t)c0 * max_blocks;
     a.context_lens = context_lens + c0;
     a.k_base = static_cast<const uint8_t*>(k_cache);
+    a.act_bf16 = act_bf16 ? 1 : 0;
     a.v_base = static_cast<const uint8_t*>(v_cache);
     a.ks_base = k_scales;
     a.vs_base = v_scales;
@@ -410,6 +411,7 @@ int decode_impl(int mode, int kv_i8, void* out, float* part_out, const void* q,
       ra.num_parts = 0;
       ra.piece_stride = s.SLOT;
       ra.seg_stride = (long long)s.s_max * s.SLOT;
+      ra.bf16 = act_bf16 ? 1 : 0;
       e = pa::launch_reduce(s.GT, ra, s.s_max, st);
       if (e != cudaSuccess) return cuda_fail(e, "reduce launch");
     }
@@ -461,8 +463,8 @@ int check_fp4_rows(int dt, const void* k, const void* v, int64_t token_stride,
   if (num_tokens < 0 || num_kv_heads <= 0 || num_blocks <= 0)
     return fail(PA_ERR_INVALID_ARG, "invalid sizes");
   if (head_dim != 128) return fail(PA_ERR_UNSUPPORTED, "head_dim %d unsupported", head_dim);
-  if (block_size <= 0 || block_size % 16 != 0)
-    return fail(PA_ERR_INVALID_ARG, "block_size must be a multiple of 16");
+  if (block_size <= 0 || block_size % 16 != 0 || 128 % block_size != 0)
+    return fail(PA_ERR_INVALID_ARG, "block_size must be 16, 32, 64 or 128");
   if (k == nullptr || v == nullptr || slot_mapping == nullptr || k_cache == nullptr ||
       v_cache == nullptr)
     return fail(PA_ERR_INVALID_ARG, "null pointer argument");
@@ -471,8 +473,7 @@ int check_fp4_rows(int dt, const void* k, const void* v, int64_t token_stride,
   if (!aligned(k, 16) || !aligned(v, 16) || (token_stride * elem_size(dt)) % 16 != 0 ||
       !aligned(k_cache, 16) || !aligned(v_cache, 16))
     return fail(PA_ERR_INVALID_ARG, "rows and caches must be 16-byte aligned");
-  if ((long long)num_tokens * num_kv_heads > (1LL << 34))
-    return fail(PA_ERR_UNSUPPORTED, "too many rows for one call");
+  if (num_kv_heads > 32767) return fail(PA_ERR_UNSUPPORTED, "num_kv_heads must be <= 32767");
   return PA_OK;
 }
 
@@ -602,7 +603,7 @@ int pa_splitk_i8(void* out, const void* q, const void* k_cache, const void* v_ca
 
 // BF16 activations: q (bf16) -> fp16 copy in the workspace, the fp16-q decode into an fp16
 // output in the workspace, then -> bf16 out. Layout: [decode workspace | q fp16 | out fp16],
-// each part 256-byte aligned.
+// each part 256-byte aligned. Over an fp4 cache the decode kernel reads and writes bf16 itself.
 static size_t round256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 size_t pa_decode_bf16q_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads,
@@ -611,6 +612,7 @@ size_t pa_decode_bf16q_workspace_bytes(int num_seqs, int num_heads, int num_kv_h
   const size_t base = pa_decode_workspace_bytes(num_seqs, num_heads, num_kv_heads, head_dim,
                                                 max_blocks_per_seq, block_size, kv_dtype, splitk);
   if (base == 0 || num_seqs < 0) return 0;
+  if (kv_kind(kv_dtype) == 3) return base;  // converts in the decode kernel
   const size_t act = round256((size_t)num_seqs * num_heads * head_dim * 2);
   return round256(base) + 2 * act;
 }
@@ -640,6 +642,11 @@ int pa_decode_bf16q(void* out, const void* q, const void* k_cache, const void* v
   if (need == 0) return fail(PA_ERR_UNSUPPORTED, "unsupported decode shape");
   if (workspace_bytes < need)
     return fail(PA_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
+  if (kv_kind(kv_dtype) == 3)
+    return decode_impl(splitk ? pa::kModeSplit : pa::kModeStream, 3, out, nullptr, q, k_cache,
+                       v_cache, nullptr, nullptr, block_table, context_lens, num_seqs, num_heads,
+                       num_kv_heads, head_dim, num_blocks, block_size, max_blocks_per_seq, scale,
+                       workspace, workspace_bytes, stream, nullptr, true);
   const size_t base = round256(pa_decode_workspace_bytes(num_seqs, num_heads, num_kv_heads,
                                                          head_dim, max_blocks_per_seq,
                                                          block_size, kv_dtype, splitk));
@@ -926,8 +933,11 @@ static int norm_rope(const char* what, int dtype, int kind, const pa::RopeArgs& 
                   "k_out rows must be non-null, 16-byte aligned and contiguous per token");
   } else {
     if (a.KVH == 0 || a.NB <= 0 || a.bs <= 0) return fail(PA_ERR_INVALID_ARG, "invalid sizes");
-    if (kind == pa::kRowsFP4 && a.bs % 16 != 0)
-      return fail(PA_ERR_INVALID_ARG, "block_size must be a multiple of 16");
+    if (kind == pa::kRowsFP4 && (a.bs % 16 != 0 || 128 % a.bs != 0))
+      return fail(PA_ERR_INVALID_ARG, "block_size must be 16, 32, 64 or 128");
+    // A lane's chunks must not split a block of 16 values.
+    if (kind == pa::kRowsFP4 && !a.interleaved && a.rot % 32 != 0)
+      return fail(PA_ERR_UNSUPPORTED, "rot_dim %d: a multiple of 32 for an fp4 cache", a.rot);
     if (!rows(a.v, a.v_stride, a.KVH))
       return fail(PA_ERR_INVALID_ARG,
                   "v rows must be non-null, 16-byte aligned and contiguous per token");

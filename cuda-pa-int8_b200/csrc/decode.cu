@@ -90,6 +90,15 @@ struct Tile {
   static constexpr size_t SMEM_STEP = F4 ? SMEM : SMEM + 16 + (size_t)WARPS * DEPTH * NR;
 };
 
+// One output value, as fp16 or bf16.
+__device__ __forceinline__ void store_out(__half* p, float v, bool bf) {
+  if (bf) {
+    *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(v);
+  } else {
+    *p = __float2half_rn(v);
+  }
+}
+
 // ---------------------------------------------------------------------------------------
 // Log-sum-exp merge of `np` partial slots by one warp, from copies of the slots in shared
 // memory: the lanes bulk-copy the slots into `stage` (np * SLOT floats) on the warp's
@@ -99,9 +108,9 @@ struct Tile {
 // 2 (wf + k) + 1 for the first piece (it starts the segment), 2 (wf + k) for the others.
 // Returns false (status flagged) if the copies did not arrive within the wait limit; the
 // caller then stops using the staging memory. Out of line: it runs a few times per CTA at
-// the end of the launch and should not add to the page loop's registers.
+// the end of the launch and should not add to the page loop's registers. BF: out rows are bf16.
 // ---------------------------------------------------------------------------------------
-template <int D, int GT>
+template <int D, int GT, bool BF = false>
 __device__ __noinline__ bool staged_combine(const float* part, int wf, int np, int lane,
                                             int hcnt, __half* out_rows, float* out_slot,
                                             int* status, float* stage, uint64_t* bar,
@@ -166,7 +175,7 @@ __device__ __noinline__ bool staged_combine(const float* part, int wf, int np, i
       const float a4[4] = {acc[i].x, acc[i].y, acc[i].z, acc[i].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (h0 + e < hcnt) out_rows[(size_t)(h0 + e) * D + d] = __float2half_rn(a4[e] * inv[e]);
+        if (h0 + e < hcnt) store_out(out_rows + (size_t)(h0 + e) * D + d, a4[e] * inv[e], BF);
     }
   } else {
 #pragma unroll
@@ -198,7 +207,7 @@ struct Coop {
   }
 };
 
-template <int D, int GT, int NTHR, int U, typename PieceFn>
+template <int D, int GT, int NTHR, int U, bool BF = false, typename PieceFn>
 __device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __half* out_rows,
                                              float* out_slot, int* status, float* sm) {
   using CC = Coop<D, GT, NTHR, U>;
@@ -330,7 +339,7 @@ __device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __
           const int h = h0 + e;
           if (h < hcnt) {
             const float L = sL[h];
-            out_rows[(size_t)h * D + d] = __float2half_rn(L > 0.f ? a4[e] / L : 0.f);
+            store_out(out_rows + (size_t)h * D + d, L > 0.f ? a4[e] / L : 0.f, BF);
           }
         }
       } else {
@@ -650,6 +659,28 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   float qks0 = qs, qks1 = qs;
   int q_b = -1, q_seg = -1;
 
+  // FP4 with bf16 activations: eight bf16 values as fp16 (exact inside the fp16 normal range;
+  // larger magnitudes saturate and are flagged, as by pa_decode_bf16q's conversion kernel).
+  [[maybe_unused]] auto bf16_to_f16 = [&](uint4 v) {
+    const uint32_t src[4] = {v.x, v.y, v.z, v.w};
+    uint32_t dst[4];
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float lo = __uint_as_float(src[e] << 16), hi = __uint_as_float(src[e] & 0xffff0000u);
+      if (fabsf(lo) > 65504.f) {
+        bad = true;
+        lo = copysignf(65504.f, lo);
+      }
+      if (fabsf(hi) > 65504.f) {
+        bad = true;
+        hi = copysignf(65504.f, hi);
+      }
+      dst[e] = pack_f16x2(lo, hi);
+    }
+    if (bad) flag_error(a.status, PA_ERR_Q_RANGE);
+    return make_uint4(dst[0], dst[1], dst[2], dst[3]);
+  };
   auto fetch_q = [&](int b, int seg) {
     const int kvh = seg / a.HT;
     const int ht = seg - kvh * a.HT;
@@ -740,6 +771,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       for (int si = 0; si < NS; ++si) {
         qa[si] = ra[si];
         qb[si] = rb[si];
+        if constexpr (F4) {
+          if (a.act_bf16) {
+            qa[si] = bf16_to_f16(ra[si]);
+            if constexpr (NT == 2) qb[si] = bf16_to_f16(rb[si]);
+          }
+        }
       }
     }
   };
@@ -1609,8 +1646,34 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
             id = __shfl_sync(0xffffffffu, inv1, 8 * r + 4);
           }
           __half* ob = a.out + ((size_t)cb * a.H + hbase) * D;
+          if constexpr (F4) {
+            // A lane holds values 16g .. 16g + 15 of its heads: 32 contiguous bytes each.
 #pragma unroll
-          for (int i = 0; i < MT; ++i) {
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int h = nt * 8 + 2 * r + e;
+                const float f = nt ? (e ? id : ic) : (e ? ib : ia);
+                uint32_t w[MT];
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                  const float lo = oacc[i][nt][e] * f, hi = oacc[i][nt][2 + e] * f;
+                  if (a.act_bf16) {
+                    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+                    w[i] = *reinterpret_cast<const uint32_t*>(&v);
+                  } else {
+                    w[i] = pack_f16x2(lo, hi);
+                  }
+                }
+                if (h < hcnt) {
+                  uint4* o = reinterpret_cast<uint4*>(ob + (size_t)h * D + 16 * g);
+                  o[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                  o[1] = make_uint4(w[4], w[5], w[6], w[7]);
+                }
+              }
+          }
+#pragma unroll
+          for (int i = 0; i < (F4 ? 0 : MT); ++i) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               const int h = nt * 8 + 2 * r;
@@ -1728,10 +1791,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       }
       if (inwave == warp) {
         const int segid = pe[0], wf = pe[1], b = pe[3], hbase = pe[4], hcnt = pe[5];
-        if (!staged_combine<D, GT>(a.part, wf, np, lane, hcnt,
-                                   stream ? a.out + ((size_t)b * a.H + hbase) * D : nullptr,
-                                   stream ? nullptr : a.part_out + (size_t)segid * SLOT,
-                                   a.status, scratch + (size_t)used * SLOT, &s_mmb[warp], mph)) {
+        __half* orow = stream ? a.out + ((size_t)b * a.H + hbase) * D : nullptr;
+        float* oslot = stream ? nullptr : a.part_out + (size_t)segid * SLOT;
+        float* stg = scratch + (size_t)used * SLOT;
+        const bool done =
+            F4 && a.act_bf16
+                ? staged_combine<D, GT, F4>(a.part, wf, np, lane, hcnt, orow, oslot, a.status, stg,
+                                            &s_mmb[warp], mph)
+                : staged_combine<D, GT>(a.part, wf, np, lane, hcnt, orow, oslot, a.status, stg,
+                                        &s_mmb[warp], mph);
+        if (!done) {
           // Timed out: let the copies land before the memory is used again.
           (void)mbar_wait_bounded(&s_mmb[warp], mph, nullptr);
         }
@@ -1759,7 +1828,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       auto piece = [&](int k) -> const float* {
         return a.part + ((size_t)(wf + k) * 2 + (k == 0 ? 1 : 0)) * SLOT;
       };
-      if (stream) {
+      if (F4 && stream && a.act_bf16) {
+        coop_combine<D, GT, NTHR, 8, F4>(piece, np, hcnt,
+                                         a.out + ((size_t)b * a.H + hbase) * D, nullptr,
+                                         a.status, scratch);
+      } else if (stream) {
         coop_combine<D, GT, NTHR, 8>(piece, np, hcnt, a.out + ((size_t)b * a.H + hbase) * D,
                                      nullptr, a.status, scratch);
       } else {
@@ -1777,7 +1850,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 // ---------------------------------------------------------------------------------------
 constexpr int kReduceThreads = 512;
 
-template <int D, int GT>
+template <int D, int GT, bool BF>
 __global__ void __launch_bounds__(kReduceThreads, 1) reduce_kernel(const ReduceArgs a) {
   extern __shared__ __align__(16) float rsm[];
   const int SEGS = a.KVH * a.HT;
@@ -1803,7 +1876,7 @@ __global__ void __launch_bounds__(kReduceThreads, 1) reduce_kernel(const ReduceA
     return;
   }
   const float* base = a.part + (size_t)segid * a.seg_stride;
-  coop_combine<D, GT, kReduceThreads, 16>(
+  coop_combine<D, GT, kReduceThreads, 16, BF>(
       [&](int k) { return base + (size_t)k * a.piece_stride; }, np, hcnt, orow, nullptr,
       a.status, rsm);
 }
@@ -1917,19 +1990,21 @@ cudaError_t launch_reduce(int gt, const ReduceArgs& a, int max_pieces, cudaStrea
   cudaError_t e;
   if (Coop<128, 16, kReduceThreads, 16>::floats(max_pieces) * sizeof(float) > 200 * 1024)
     return cudaErrorInvalidValue;  // more splits than one CTA can merge (contexts > ~3M tokens)
+  auto launch = [&](auto kern, size_t floats) {
+    smem = floats * sizeof(float);
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) kern<<<segs, kReduceThreads, smem, stream>>>(a);
+  };
+  const size_t f8 = Coop<128, 8, kReduceThreads, 16>::floats(max_pieces);
+  const size_t f16 = Coop<128, 16, kReduceThreads, 16>::floats(max_pieces);
   if (gt == 8) {
-    smem = Coop<128, 8, kReduceThreads, 16>::floats(max_pieces) * sizeof(float);
-    e = cudaFuncSetAttribute(reduce_kernel<128, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)smem);
-    if (e != cudaSuccess) return e;
-    reduce_kernel<128, 8><<<segs, kReduceThreads, smem, stream>>>(a);
+    if (a.bf16) launch(reduce_kernel<128, 8, true>, f8);
+    else launch(reduce_kernel<128, 8, false>, f8);
   } else {
-    smem = Coop<128, 16, kReduceThreads, 16>::floats(max_pieces) * sizeof(float);
-    e = cudaFuncSetAttribute(reduce_kernel<128, 16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             (int)smem);
-    if (e != cudaSuccess) return e;
-    reduce_kernel<128, 16><<<segs, kReduceThreads, smem, stream>>>(a);
+    if (a.bf16) launch(reduce_kernel<128, 16, true>, f16);
+    else launch(reduce_kernel<128, 16, false>, f16);
   }
+  if (e != cudaSuccess) return e;
   return cudaGetLastError();
 }
 

@@ -1,10 +1,12 @@
 // Rows into and out of the 4-bit K/V cache (format and layout: fp4.cuh).
 //
-// Both directions are streams: a thread takes one 16-value block of one row (token, kv head, K
-// or V), so a block's maximum needs no other lane, eight neighbouring threads cover a row, and a
-// warp's loads and stores of values are contiguous. Every byte of the cache belongs to one
-// token, so rows are written independently: a decode step's appends, a prompt through slots
-// and rows in any order all take the same path.
+// Both directions are streams of rows (token, kv head, K or V), bound by memory once their
+// instructions per row are few: the kv head and K or V come from the block index (no division),
+// the write gives a thread a whole 16-value block (its maximum needs no other lane), the read
+// eight values (one 16-byte store a thread, contiguous over the warp), and each thread takes
+// several tokens at once so that their loads overlap. Every byte of the cache belongs to one token,
+// so rows are written independently: a decode step's appends, a prompt through slots and rows in
+// any order all take the same path.
 
 #include "fp4.cuh"
 #include "pa_common.cuh"
@@ -15,91 +17,137 @@ namespace pa {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kBlocksPerRow = 8;  // 128 head_dim values in blocks of 16
+constexpr int kWriteRow = 8;   // threads of a row in the write: 128 values in blocks of 16
+constexpr int kReadRow = 16;   // in the read: eight values each
+// Tokens a thread takes. 1.05 M rows of K and of V: write 125 us with one, 111 with two or four;
+// read 157 with two, 143 with four, 164 with eight.
+constexpr int kWriteTokens = 2;
+constexpr int kReadTokens = 4;
 
-// Sixteen consecutive values as fp32 (p aligned to 16 bytes).
-__device__ __forceinline__ void load16(const __half* p, float (&x)[16]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-      x[8 * i + 2 * e] = f.x;
-      x[8 * i + 2 * e + 1] = f.y;
-    }
-  }
-}
-__device__ __forceinline__ void load16(const __nv_bfloat16* p, float (&x)[16]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[8 * i + 2 * e] = __uint_as_float(w[e] << 16);
-      x[8 * i + 2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-    }
-  }
-}
-__device__ __forceinline__ void load16(const float* p, float (&x)[16]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float4 f = __ldg(reinterpret_cast<const float4*>(p) + i);
-    x[4 * i] = f.x;
-    x[4 * i + 1] = f.y;
-    x[4 * i + 2] = f.z;
-    x[4 * i + 3] = f.w;
-  }
+// Where the groups of a cache are. Group indices fit 32 bits: 2^32 groups would be 4.9 TB.
+struct Cache {
+  int NB, KVH;
+  int shift;  // log2 of the block size (16 .. 128)
+};
+// Group index of `slot` and kv head kvh; the token of the group in t.
+__device__ __forceinline__ uint32_t group_of(const Cache& c, int blk, int slot, int kvh, int& t) {
+  t = slot & (fp4::kGroupTokens - 1);
+  const uint32_t page = (uint32_t)blk * (uint32_t)c.KVH + (uint32_t)kvh;
+  return (page << (c.shift - 4)) | (((uint32_t)slot & ((1u << c.shift) - 1u)) >> 4);
 }
 
-// Block b (16 values x) of token `off` of page row `page`: eight code bytes and the scale byte.
+// Sixteen consecutive values (p aligned to 16 bytes) as loaded: 16-bit values packed in pairs.
+template <typename T> struct Block { uint32_t w[8]; };
+template <> struct Block<float> { uint32_t w[16]; };
+
 template <typename T>
-__device__ __forceinline__ void put_block(const float (&x)[16], uint8_t* cache, bool is_v,
-                                          size_t page, int off, int bs, int b) {
+__device__ __forceinline__ void load_block(const T* p, Block<T>& r) {
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T); ++i) {  // 32 or 64 bytes
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    r.w[4 * i] = u.x;
+    r.w[4 * i + 1] = u.y;
+    r.w[4 * i + 2] = u.z;
+    r.w[4 * i + 3] = u.w;
+  }
+}
+// Bit pattern of the largest magnitude as fp32. Bit patterns without the sign order as the
+// magnitudes do, NaN above infinity, so the 16-bit types compare two at a time as integers.
+__device__ __forceinline__ uint32_t max_bits(const Block<float>& r) {
   uint32_t m = 0u;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
-  const uint32_t sb = fp4::scale_byte(m);
-  const float s = fp4::scale_value(sb), inv = fp4::scale_inverse(sb);
-  constexpr bool kWide = sizeof(T) == 4;
-  uint32_t w[2] = {0u, 0u};
+  for (int e = 0; e < 16; ++e) m = max(m, r.w[e] & 0x7fffffffu);
+  return m;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t max_pair(const Block<T>& r) {
+  uint32_t m = 0u;
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    w[e >> 2] |= fp4::code_pair(fp4::code_y<kWide>(x[2 * e], s, inv),
-                                fp4::code_y<kWide>(x[2 * e + 1], s, inv))
-                 << (8 * (e & 3));
-  uint8_t* grp = cache + fp4::group_offset(page, off, bs);
-  const int t = off % fp4::kGroupTokens;
+  for (int e = 0; e < 8; ++e) m = __vmaxu2(m, r.w[e] & 0x7fff7fffu);
+  return max(m & 0xffffu, m >> 16);
+}
+__device__ __forceinline__ uint32_t max_bits(const Block<__half>& r) {
+  return __float_as_uint(__half2float(__ushort_as_half((unsigned short)max_pair(r))));
+}
+__device__ __forceinline__ uint32_t max_bits(const Block<__nv_bfloat16>& r) {
+  return max_pair(r) << 16;
+}
+// Values 2e and 2e + 1.
+__device__ __forceinline__ float2 pair_of(const Block<float>& r, int e) {
+  return make_float2(__uint_as_float(r.w[2 * e]), __uint_as_float(r.w[2 * e + 1]));
+}
+__device__ __forceinline__ float2 pair_of(const Block<__half>& r, int e) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&r.w[e]));
+}
+__device__ __forceinline__ float2 pair_of(const Block<__nv_bfloat16>& r, int e) {
+  return make_float2(__uint_as_float(r.w[e] << 16), __uint_as_float(r.w[e] & 0xffff0000u));
+}
+
+// Block b of token t of a group: eight code bytes and the scale byte.
+template <typename T>
+__device__ __forceinline__ void put_block(const Block<T>& r, uint8_t* grp, bool is_v, int t,
+                                          int b) {
+  constexpr bool kWide = sizeof(T) == 4;
+  const uint32_t sb = fp4::scale_byte<kWide>(max_bits(r));
+  const float s = fp4::scale_value(sb), inv = fp4::scale_inverse<kWide>(sb);
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float y[8];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float2 v = pair_of(r, 4 * h + e);
+      if constexpr (kWide) {
+        v = make_float2(fp4::code_y<true>(v.x, s, inv), fp4::code_y<true>(v.y, s, inv));
+      } else {  // fp4::code_y<false>, two values at a time
+        v = add2(fma2(v, make_float2(inv, inv), make_float2(96.f, 96.f)),
+                 make_float2(-96.f, -96.f));
+      }
+      y[2 * e] = v.x;
+      y[2 * e + 1] = v.y;
+    }
+    w[h] = fp4::code_word(y);
+  }
   *reinterpret_cast<uint2*>(grp + t * fp4::kCodeRow + 8 * b) = make_uint2(w[0], w[1]);
   grp[fp4::scale_offset(is_v, t, b)] = (uint8_t)sb;
 }
 
-// Rows of a slot-mapped write; rows of one token are contiguous (kv_heads x 128 values).
+// Rows of a slot-mapped write; rows of one token are contiguous (kv_heads x 128 values). Block
+// row y of the grid: kv head y / 2, K (even) or V.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) write_fp4_kernel(
     const T* __restrict__ k, const T* __restrict__ v, long long token_stride,
-    const int* __restrict__ slot_mapping, int N, int KVH, uint8_t* __restrict__ k_cache,
-    uint8_t* __restrict__ v_cache, int NB, int bs, int* status) {
-  const bool is_v = blockIdx.y != 0;
-  const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-  const long long row = i >> 3;
-  const int b = (int)(i & 7);
-  if (row >= (long long)N * KVH) return;
-  const int n = (int)(row / KVH);
-  const int kvh = (int)(row - (long long)n * KVH);
-  const int slot = __ldg(slot_mapping + n);
-  if (slot < 0) return;  // padding token
-  const int blk = slot / bs;
-  if (blk >= NB) {
-    flag_error(status, PA_ERR_SLOT);
-    return;
+    const int* __restrict__ slot_mapping, int N, uint8_t* __restrict__ k_cache,
+    uint8_t* __restrict__ v_cache, const Cache c, int* status) {
+  constexpr int kTokens = kThreads / kWriteRow;  // tokens of a CTA's round
+  const bool is_v = (blockIdx.y & 1) != 0;
+  const int kvh = blockIdx.y >> 1;
+  const int b = threadIdx.x % kWriteRow;
+  const unsigned n0 = blockIdx.x * (unsigned)(kTokens * kWriteTokens) + threadIdx.x / kWriteRow;
+  const T* src = (is_v ? v : k) + kvh * 128 + 16 * b;
+  uint8_t* cache = is_v ? v_cache : k_cache;
+  int slot[kWriteTokens];
+#pragma unroll
+  for (int i = 0; i < kWriteTokens; ++i) {
+    const unsigned n = n0 + i * kTokens;
+    slot[i] = n < (unsigned)N ? __ldg(slot_mapping + n) : -1;  // negative: padding token
   }
-  float x[16];
-  load16((is_v ? v : k) + (size_t)n * token_stride + (size_t)kvh * 128 + 16 * b, x);
-  put_block<T>(x, is_v ? v_cache : k_cache, is_v, (size_t)blk * KVH + kvh, slot - blk * bs, bs,
-               b);
+  Block<T> r[kWriteTokens];
+#pragma unroll
+  for (int i = 0; i < kWriteTokens; ++i)
+    if (slot[i] >= 0) load_block(src + (n0 + i * kTokens) * token_stride, r[i]);
+#pragma unroll
+  for (int i = 0; i < kWriteTokens; ++i) {
+    if (slot[i] < 0) continue;
+    const int blk = slot[i] >> c.shift;
+    if (blk >= c.NB) {
+      flag_error(status, PA_ERR_SLOT);
+      continue;
+    }
+    int t;
+    const uint32_t g = group_of(c, blk, slot[i], kvh, t);
+    put_block<T>(r[i], cache + (size_t)g * fp4::kGroupBytes, is_v, t, b);
+  }
 }
 
 // The decode step's new token: position context_lens[b] - 1 of sequence b, through its table.
@@ -107,51 +155,51 @@ template <typename T>
 __global__ void __launch_bounds__(kThreads) step_fp4_kernel(
     const T* __restrict__ k, const T* __restrict__ v, long long token_stride,
     const int* __restrict__ block_table, const int* __restrict__ context_lens, int max_blocks,
-    int B, int KVH, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache, int NB, int bs,
+    int B, uint8_t* __restrict__ k_cache, uint8_t* __restrict__ v_cache, const Cache c,
     int* status) {
-  const bool is_v = blockIdx.y != 0;
-  const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-  const long long row = i >> 3;
-  const int b = (int)(i & 7);
-  if (row >= (long long)B * KVH) return;
-  const int n = (int)(row / KVH);
-  const int kvh = (int)(row - (long long)n * KVH);
+  const bool is_v = (blockIdx.y & 1) != 0;
+  const int kvh = blockIdx.y >> 1;
+  const int b = threadIdx.x % kWriteRow;
+  const int n = blockIdx.x * (kThreads / kWriteRow) + threadIdx.x / kWriteRow;
+  if (n >= B) return;
   const int ctx = __ldg(context_lens + n);
-  if (ctx < 1 || ctx > max_blocks * bs) return;  // the decode flags the length
+  if (ctx < 1 || ctx > max_blocks << c.shift) return;  // the decode flags the length
   const int pos = ctx - 1;
-  const int blk = __ldg(block_table + (size_t)n * max_blocks + pos / bs);
-  if (blk < 0 || blk >= NB) {
+  const int blk = __ldg(block_table + (size_t)n * max_blocks + (pos >> c.shift));
+  if (blk < 0 || blk >= c.NB) {
     flag_error(status, PA_ERR_BLOCK_ID);
     return;
   }
-  float x[16];
-  load16((is_v ? v : k) + (size_t)n * token_stride + (size_t)kvh * 128 + 16 * b, x);
-  put_block<T>(x, is_v ? v_cache : k_cache, is_v, (size_t)blk * KVH + kvh, pos % bs, bs, b);
+  Block<T> r;
+  load_block((is_v ? v : k) + n * token_stride + kvh * 128 + 16 * b, r);
+  int t;
+  const uint32_t g = group_of(c, blk, pos, kvh, t);
+  put_block<T>(r, (is_v ? v_cache : k_cache) + (size_t)g * fp4::kGroupBytes, is_v, t, b);
 }
 
-// Sixteen held values as fp16 pairs, stored as T (exact: every held value is an fp16 and a bf16
-// number; a NaN scale gives NaN).
-__device__ __forceinline__ void store16(const uint32_t (&h)[8], __half* p) {
-  reinterpret_cast<uint4*>(p)[0] = make_uint4(h[0], h[1], h[2], h[3]);
-  reinterpret_cast<uint4*>(p)[1] = make_uint4(h[4], h[5], h[6], h[7]);
+// Eight held values as fp16 pairs, stored as T (exact: every held value is an fp16 and a bf16
+// number; a NaN scale gives NaN). Streaming stores: the read is bound by its writes (1.05 M rows
+// of 128 fp16 values, K and V: 139.6 us with them, 143.5 without, 143.5 for filling the same
+// memory with a constant).
+__device__ __forceinline__ void store8(const uint32_t (&h)[4], __half* p) {
+  __stcs(reinterpret_cast<uint4*>(p), make_uint4(h[0], h[1], h[2], h[3]));
 }
-__device__ __forceinline__ void store16(const uint32_t (&h)[8], __nv_bfloat16* p) {
-  uint32_t w[8];
+__device__ __forceinline__ void store8(const uint32_t (&h)[4], __nv_bfloat16* p) {
+  uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int i = 0; i < 4; ++i) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
     const __nv_bfloat162 o = __floats2bfloat162_rn(f.x, f.y);
     w[i] = *reinterpret_cast<const uint32_t*>(&o);
   }
-  reinterpret_cast<uint4*>(p)[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  reinterpret_cast<uint4*>(p)[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  __stcs(reinterpret_cast<uint4*>(p), make_uint4(w[0], w[1], w[2], w[3]));
 }
-__device__ __forceinline__ void store16(const uint32_t (&h)[8], float* p) {
+__device__ __forceinline__ void store8(const uint32_t (&h)[4], float* p) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2; ++i) {
     const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&h[2 * i]));
     const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&h[2 * i + 1]));
-    reinterpret_cast<float4*>(p)[i] = make_float4(a.x, a.y, b.x, b.y);
+    __stcs(reinterpret_cast<float4*>(p) + i, make_float4(a.x, a.y, b.x, b.y));
   }
 }
 
@@ -159,50 +207,72 @@ __device__ __forceinline__ void store16(const uint32_t (&h)[8], float* p) {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) read_fp4_kernel(
     T* __restrict__ k_out, T* __restrict__ v_out, const uint8_t* __restrict__ k_cache,
-    const uint8_t* __restrict__ v_cache, const int* __restrict__ slot_mapping, int N, int KVH,
-    int NB, int bs, int* status) {
-  const bool is_v = blockIdx.y != 0;
-  const long long i = (long long)blockIdx.x * kThreads + threadIdx.x;
-  const long long row = i >> 3;
-  const int b = (int)(i & 7);
-  if (row >= (long long)N * KVH) return;
-  const int n = (int)(row / KVH);
-  const int kvh = (int)(row - (long long)n * KVH);
-  const int slot = __ldg(slot_mapping + n);
-  if (slot < 0) return;
-  const int blk = slot / bs;
-  if (blk >= NB) {
-    flag_error(status, PA_ERR_SLOT);
-    return;
-  }
-  const int off = slot - blk * bs, t = off % fp4::kGroupTokens;
-  const uint8_t* grp = (is_v ? v_cache : k_cache) +
-                       fp4::group_offset((size_t)blk * KVH + kvh, off, bs);
-  const uint2 c = *reinterpret_cast<const uint2*>(grp + t * fp4::kCodeRow + 8 * b);
-  const uint32_t s = (uint32_t)grp[fp4::scale_offset(is_v, t, b)] * 0x00800080u;  // twice << 7
-  uint32_t h[8];
-  fp4::codes_to_f16x2(c.x, h[0], h[1], h[2], h[3]);
-  fp4::codes_to_f16x2(c.y, h[4], h[5], h[6], h[7]);
+    const uint8_t* __restrict__ v_cache, const int* __restrict__ slot_mapping, int N,
+    const Cache c, int* status) {
+  constexpr int kTokens = kThreads / kReadRow;
+  const bool is_v = (blockIdx.y & 1) != 0;
+  const int kvh = blockIdx.y >> 1;
+  const int c8 = threadIdx.x % kReadRow;
+  const unsigned n0 = blockIdx.x * (unsigned)(kTokens * kReadTokens) + threadIdx.x / kReadRow;
+  const uint8_t* cache = is_v ? v_cache : k_cache;
+  T* out = (is_v ? v_out : k_out) + kvh * 128 + 8 * c8;
+  const long long row = (long long)c.KVH * 128;
+  int slot[kReadTokens];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) h[e] = fp4::hmul2(h[e], s);
-  store16(h, (is_v ? v_out : k_out) + (size_t)row * 128 + 16 * b);
+  for (int i = 0; i < kReadTokens; ++i) {
+    const unsigned n = n0 + i * kTokens;
+    slot[i] = n < (unsigned)N ? __ldg(slot_mapping + n) : -1;
+  }
+  uint32_t w[kReadTokens], s[kReadTokens];
+#pragma unroll
+  for (int i = 0; i < kReadTokens; ++i) {
+    const int blk = slot[i] >> c.shift;
+    if (blk >= c.NB) {
+      flag_error(status, PA_ERR_SLOT);
+      slot[i] = -1;
+    }
+    if (slot[i] >= 0) {
+      int t;
+      const uint32_t g = group_of(c, blk, slot[i], kvh, t);
+      const uint8_t* grp = cache + (size_t)g * fp4::kGroupBytes;
+      w[i] = __ldg(reinterpret_cast<const uint32_t*>(grp + t * fp4::kCodeRow + 4 * c8));
+      s[i] = __ldg(grp + fp4::scale_offset(is_v, t, c8 >> 1));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kReadTokens; ++i) {
+    if (slot[i] < 0) continue;
+    uint32_t h[4];
+    fp4::codes_to_f16x2(w[i], h[0], h[1], h[2], h[3]);
+    const uint32_t s2 = s[i] * 0x00800080u;  // twice byte << 7
+#pragma unroll
+    for (int e = 0; e < 4; ++e) h[e] = fp4::hmul2(h[e], s2);
+    store8(h, out + (n0 + i * kTokens) * row);
+  }
 }
 
-// Threads of N x KVH rows, eight each; 0 when there are none, -1 when a grid cannot hold them.
-long long grid_of(long long rows) {
-  const long long g = (rows * kBlocksPerRow + kThreads - 1) / kThreads;
-  return g > 0x7fffffffLL ? -1 : g;
+Cache cache_of(int NB, int KVH, int bs) {
+  int shift = 4;
+  while ((1 << shift) < bs) ++shift;
+  return Cache{NB, KVH, shift};
+}
+
+// Grid of `tokens` tokens, per_cta of them to a CTA, for K and V of every kv head (the grid's
+// second dimension holds 65535).
+bool grid_of(long long tokens, int per_cta, int KVH, dim3* g) {
+  if (KVH > 32767) return false;
+  *g = dim3((unsigned)((tokens + per_cta - 1) / per_cta), 2u * (unsigned)KVH);
+  return true;
 }
 
 template <typename T>
 cudaError_t write_t(const void* k, const void* v, long long ts, const int* slots, int N, int KVH,
                     void* kc, void* vc, int NB, int bs, int* status, cudaStream_t st) {
-  const long long g = grid_of((long long)N * KVH);
-  if (g < 0) return cudaErrorInvalidValue;
-  if (g == 0) return cudaSuccess;
-  write_fp4_kernel<T><<<dim3((unsigned)g, 2), kThreads, 0, st>>>(
-      static_cast<const T*>(k), static_cast<const T*>(v), ts, slots, N, KVH,
-      static_cast<uint8_t*>(kc), static_cast<uint8_t*>(vc), NB, bs, status);
+  dim3 g;
+  if (!grid_of(N, kThreads / kWriteRow * kWriteTokens, KVH, &g)) return cudaErrorInvalidValue;
+  write_fp4_kernel<T><<<g, kThreads, 0, st>>>(
+      static_cast<const T*>(k), static_cast<const T*>(v), ts, slots, N,
+      static_cast<uint8_t*>(kc), static_cast<uint8_t*>(vc), cache_of(NB, KVH, bs), status);
   return cudaGetLastError();
 }
 
@@ -210,24 +280,22 @@ template <typename T>
 cudaError_t step_t(const void* k, const void* v, long long ts, const int* bt, const int* cl,
                    int max_blocks, int B, int KVH, void* kc, void* vc, int NB, int bs,
                    int* status, cudaStream_t st) {
-  const long long g = grid_of((long long)B * KVH);
-  if (g < 0) return cudaErrorInvalidValue;
-  if (g == 0) return cudaSuccess;
-  step_fp4_kernel<T><<<dim3((unsigned)g, 2), kThreads, 0, st>>>(
-      static_cast<const T*>(k), static_cast<const T*>(v), ts, bt, cl, max_blocks, B, KVH,
-      static_cast<uint8_t*>(kc), static_cast<uint8_t*>(vc), NB, bs, status);
+  dim3 g;
+  if (!grid_of(B, kThreads / kWriteRow, KVH, &g)) return cudaErrorInvalidValue;
+  step_fp4_kernel<T><<<g, kThreads, 0, st>>>(
+      static_cast<const T*>(k), static_cast<const T*>(v), ts, bt, cl, max_blocks, B,
+      static_cast<uint8_t*>(kc), static_cast<uint8_t*>(vc), cache_of(NB, KVH, bs), status);
   return cudaGetLastError();
 }
 
 template <typename T>
 cudaError_t read_t(void* k, void* v, const void* kc, const void* vc, const int* slots, int N,
                    int KVH, int NB, int bs, int* status, cudaStream_t st) {
-  const long long g = grid_of((long long)N * KVH);
-  if (g < 0) return cudaErrorInvalidValue;
-  if (g == 0) return cudaSuccess;
-  read_fp4_kernel<T><<<dim3((unsigned)g, 2), kThreads, 0, st>>>(
+  dim3 g;
+  if (!grid_of(N, kThreads / kReadRow * kReadTokens, KVH, &g)) return cudaErrorInvalidValue;
+  read_fp4_kernel<T><<<g, kThreads, 0, st>>>(
       static_cast<T*>(k), static_cast<T*>(v), static_cast<const uint8_t*>(kc),
-      static_cast<const uint8_t*>(vc), slots, N, KVH, NB, bs, status);
+      static_cast<const uint8_t*>(vc), slots, N, cache_of(NB, KVH, bs), status);
   return cudaGetLastError();
 }
 

@@ -48,12 +48,23 @@ __device__ __forceinline__ int scale_offset(bool is_v, int t, int b) {
 
 // Scale byte of a block from the bit pattern of its largest magnitude (as an unsigned integer:
 // NaN and infinities compare above every finite value): the nearest representable to amax / 6,
-// ties to even. The fp32 quotient rounds to the same byte as the exact one: it reaches a
-// midpoint between two scales (five significant bits) only where the exact quotient does.
+// ties to even.
+// fp32 inputs (kWide): the IEEE quotient, which reaches a midpoint between two scales (five
+// significant bits) only where the exact one does.
+// 16-bit inputs: amax times 1/6, two roundings off by at most 2^-23 of it, then rounded to 17
+// significant bits. A quotient on a midpoint comes out as the midpoint; any other quotient of an
+// 11-bit amax by 6 is at least 2^-13 of its value away from it.
+template <bool kWide>
 __device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
   if (amax_bits >= 0x7f800000u) return kScaleNan;
-  const float t = __fdiv_rn(__uint_as_float(amax_bits), 6.f);
-  const uint32_t u = __float_as_uint(t);
+  const float amax = __uint_as_float(amax_bits);
+  uint32_t u;
+  if constexpr (kWide) {
+    u = __float_as_uint(__fdiv_rn(amax, 6.f));
+  } else {
+    u = (__float_as_uint(__fmul_rn(amax, 1.f / 6.f)) + 0x40u) & ~0x7fu;
+  }
+  const float t = __uint_as_float(u);
   // From 2^-14 up: round to four significant bits; the exponent field moves from bias 127 to 15.
   const uint32_t normal = ((u + 0x7ffffu + ((u >> 20) & 1u)) >> 20) - (112u << 3);
   // Below: steps of 2^-17 (adding 96 rounds to that grid, ties to even).
@@ -66,15 +77,20 @@ __device__ __forceinline__ float scale_value(uint32_t byte) {
 }
 
 // Factor for code_y below: 1 / scale; 0 for the zero scale (zero codes) and for NaN, where the
-// codes mean nothing.
+// codes mean nothing. 16-bit inputs take the hardware's approximate reciprocal (2^-23 off at most).
+template <bool kWide>
 __device__ __forceinline__ float scale_inverse(uint32_t byte) {
-  return (byte == 0u || byte == kScaleNan) ? 0.f : __frcp_rn(scale_value(byte));
+  if (byte == 0u || byte == kScaleNan) return 0.f;
+  if constexpr (kWide) return __frcp_rn(scale_value(byte));
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(scale_value(byte)));
+  return r;
 }
 
 // x / scale, close enough to round to the same code as the exact quotient.
 // 16-bit inputs (kWide false): fma(x, 1/scale, 96) - 96 puts the quotient on a grid of 2^-17.
 // The borders between codes (.25 .75 1.25 1.75 2.5 3.5 5) lie on that grid, the product is within
-// 2^-21 of the quotient there, so a quotient on a border comes out as the border; any other
+// 2^-20 of the quotient there, so a quotient on a border comes out as the border; any other
 // quotient of an 11-bit x and a 4-bit scale is at least 2^-13 away from it.
 // fp32 inputs: the IEEE quotient, which reaches a border only where the exact one does.
 template <bool kWide>
@@ -95,6 +111,19 @@ __device__ __forceinline__ uint32_t code_pair(float a, float b) {
       "cvt.u32.u8 %0, c;\n\t}"
       : "=r"(r)
       : "f"(a), "f"(b));
+  return r;
+}
+// Eight codes, y[0] in the lowest four bits.
+__device__ __forceinline__ uint32_t code_word(const float (&y)[8]) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 c0, c1, c2, c3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c0, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c1, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c2, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c3, %8, %7;\n\t"
+      "mov.b32 %0, {c0, c1, c2, c3};\n\t}"
+      : "=r"(r)
+      : "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7]));
   return r;
 }
 
@@ -140,8 +169,8 @@ __device__ __forceinline__ uint32_t warp_quantize4(const float (&x)[4], uint32_t
   for (int e = 0; e < 4; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
   m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  scale = scale_byte(m);
-  const float s = scale_value(scale), inv = scale_inverse(scale);
+  scale = scale_byte<kWide>(m);
+  const float s = scale_value(scale), inv = scale_inverse<kWide>(scale);
   float y[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = code_y<kWide>(x[e], s, inv);

@@ -59,7 +59,8 @@ struct DecodeArgs {
   void* vc_w;
   float* ks_w;
   float* vs_w;
-  const uint8_t* k_base;       // K cache base (fp4: its groups are untiled bulk copies)
+  const uint8_t* k_base;       // K cache base (fp4)
+  int act_bf16;                // fp4: q and out are bf16
 };
 
 struct ReduceArgs {
@@ -71,6 +72,7 @@ struct ReduceArgs {
   int num_parts;               // > 0: fixed number of pieces per segment (cross-GPU merge)
   long long piece_stride;      // floats between consecutive pieces of one segment
   long long seg_stride;        // floats between consecutive segments
+  int bf16;                    // out is bf16
 };
 
 // Launch helpers implemented in decode.cu. They return a cudaError_t.

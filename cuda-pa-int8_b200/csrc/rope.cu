@@ -8,16 +8,18 @@
 // with c, s = the cosine and sine of the token's position, read from the caller's table. All of
 // it in fp32, rounded once to the rows' type.
 //
-// Sixteen lanes hold a row, eight neighbouring values each (one 16-byte access for 16-bit rows), so a
-// warp works on two heads at a time: four shuffles sum the squares, and a pair's other half is
-// a neighbour value (interleaved) or eight lanes' exchange (rot / 16 lanes away). A warp stays
-// with one token and takes kHeads heads per half-warp, all loaded before the first is used: the
-// token's cosines and sines are read once for them and the loads overlap.
+// Bound by memory for many tokens (each row read and written once), by latency for few. What kept
+// a first version from that bound was its instruction count (104 a row), so:
+//  * sixteen lanes hold a row, two chunks of four neighbouring values each, and a pair's two
+//    halves sit in the same lane: chunk a holds values 4l .., chunk b the values rot/2 further on
+//    (interleaved, and past rot: eight neighbouring values), so the rotation needs no exchange;
+//  * a warp stays with one token and one kind of row (q, k or v) and takes kHeads heads per
+//    half-warp, all loaded before the first is used. It folds the weights into the token's
+//    cosines and sines once: a' = r (a (c w_a) - b (s w_b)), r = 1/rms, three operations a value.
 //
 // The cache forms (kCache) round K to the rows' type first, so caches are bit for bit those of
-// the separate calls, then quantise as the cache writes do: the 4-bit format's blocks are two
-// lanes, the one-byte formats' row maximum is a half-warp's. One launch less for a step, and
-// K's rows never go to memory and back.
+// the separate calls, then quantise as the cache writes do. One launch less for a step, and K's
+// rows never go to memory and back.
 
 #include "fp4.cuh"
 #include "pa_common.cuh"
@@ -28,132 +30,128 @@ namespace pa {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kVals = 8;  // values of a lane
 
-template <typename T> struct Row8 { uint4 u; };
-template <> struct Row8<float> { float4 a, b; };
+// Four neighbouring values as loaded (8 bytes for 16-bit rows, 16 for fp32).
+template <typename T> struct Raw { using type = uint2; };
+template <> struct Raw<float> { using type = float4; };
 
 template <typename T>
-__device__ __forceinline__ Row8<T> load8(const T* p) {
-  return Row8<T>{__ldg(reinterpret_cast<const uint4*>(p))};
+__device__ __forceinline__ typename Raw<T>::type load4(const T* p) {
+  return __ldg(reinterpret_cast<const typename Raw<T>::type*>(p));
 }
-template <>
-__device__ __forceinline__ Row8<float> load8<float>(const float* p) {
-  return Row8<float>{__ldg(reinterpret_cast<const float4*>(p)),
-                     __ldg(reinterpret_cast<const float4*>(p) + 1)};
+__device__ __forceinline__ void widen(uint2 u, const __half*, float2 (&x)[2]) {
+  x[0] = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+  x[1] = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
 }
-__device__ __forceinline__ void widen(const Row8<__half>& r, float (&x)[kVals]) {
-  const uint32_t w[4] = {r.u.x, r.u.y, r.u.z, r.u.w};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-    x[2 * e] = f.x;
-    x[2 * e + 1] = f.y;
-  }
+__device__ __forceinline__ void widen(uint2 u, const __nv_bfloat16*, float2 (&x)[2]) {
+  x[0] = make_float2(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u));
+  x[1] = make_float2(__uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
 }
-__device__ __forceinline__ void widen(const Row8<__nv_bfloat16>& r, float (&x)[kVals]) {
-  const uint32_t w[4] = {r.u.x, r.u.y, r.u.z, r.u.w};
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    x[2 * e] = __uint_as_float(w[e] << 16);
-    x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-  }
+__device__ __forceinline__ void widen(float4 u, const float*, float2 (&x)[2]) {
+  x[0] = make_float2(u.x, u.y);
+  x[1] = make_float2(u.z, u.w);
 }
-__device__ __forceinline__ void widen(const Row8<float>& r, float (&x)[kVals]) {
-  x[0] = r.a.x; x[1] = r.a.y; x[2] = r.a.z; x[3] = r.a.w;
-  x[4] = r.b.x; x[5] = r.b.y; x[6] = r.b.z; x[7] = r.b.w;
-}
-__device__ __forceinline__ uint32_t pair_bits(float a, float b, const __half*) {
-  const __half2 h = __floats2half2_rn(a, b);
+__device__ __forceinline__ uint32_t pair_bits(float2 v, const __half*) {
+  const __half2 h = __floats2half2_rn(v.x, v.y);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint32_t pair_bits(float a, float b, const __nv_bfloat16*) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+__device__ __forceinline__ uint32_t pair_bits(float2 v, const __nv_bfloat16*) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&x)[kVals]) {
+__device__ __forceinline__ void store4(T* p, const float2 (&x)[2]) {
   const T* tag = nullptr;
-  *reinterpret_cast<uint4*>(p) =
-      make_uint4(pair_bits(x[0], x[1], tag), pair_bits(x[2], x[3], tag),
-                 pair_bits(x[4], x[5], tag), pair_bits(x[6], x[7], tag));
+  *reinterpret_cast<uint2*>(p) = make_uint2(pair_bits(x[0], tag), pair_bits(x[1], tag));
 }
 template <>
-__device__ __forceinline__ void store8<float>(float* p, const float (&x)[kVals]) {
-  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
-  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+__device__ __forceinline__ void store4<float>(float* p, const float2 (&x)[2]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
 }
 
-// Eight values of a row into the cache: lane l of the row's sixteen holds values 8l .. 8l + 7.
-// All sixteen lanes call this together (`mask`: the lanes of the warp that do).
+// A row into the cache. The lane's chunks: values oa .. oa + 3 (x[0], x[1]) and ob .. ob + 3
+// (x[2], x[3]); `apart`: the chunks lie in different 16-value blocks, each shared by four
+// neighbouring lanes (else both in one block of two lanes; for the 4-bit cache rot is a multiple
+// of 32, so four neighbouring lanes agree). All sixteen lanes of the row call this together
+// (mask: the lanes of the warp that do).
 template <typename T, int KIND>
-__device__ __forceinline__ void cache_row(const float (&x)[kVals], int l, unsigned mask,
-                                          bool is_v, void* cache, float* scales, size_t page,
-                                          int off, int bs) {
+__device__ __forceinline__ void cache_row(const float2 (&x)[4], int l, int oa, int ob, bool apart,
+                                          unsigned mask, bool is_v, void* cache, float* scales,
+                                          size_t page, int off, int bs) {
+  const float v[8] = {x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
   if constexpr (KIND == kRowsFP4) {
-    uint32_t m = 0u;
+    uint32_t m[2] = {0u, 0u};
 #pragma unroll
-    for (int e = 0; e < kVals; ++e) m = max(m, __float_as_uint(x[e]) & 0x7fffffffu);
-    m = max(m, __shfl_xor_sync(mask, m, 1));
-    const uint32_t sb = fp4::scale_byte(m);
-    const float s = fp4::scale_value(sb), inv = fp4::scale_inverse(sb);
-    constexpr bool kWide = sizeof(T) == 4;
-    uint32_t w = 0u;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      w |= fp4::code_pair(fp4::code_y<kWide>(x[2 * e], s, inv),
-                          fp4::code_y<kWide>(x[2 * e + 1], s, inv))
-           << (8 * e);
+    for (int e = 0; e < 8; ++e) m[e >> 2] = max(m[e >> 2], __float_as_uint(v[e]) & 0x7fffffffu);
+    if (!apart) m[0] = m[1] = max(m[0], m[1]);
     uint8_t* grp = static_cast<uint8_t*>(cache) + fp4::group_offset(page, off, bs);
     const int t = off % fp4::kGroupTokens;
-    *reinterpret_cast<uint32_t*>(grp + t * fp4::kCodeRow + 4 * l) = w;
-    if ((l & 1) == 0) grp[fp4::scale_offset(is_v, t, l >> 1)] = (uint8_t)sb;
-  } else {
-    uint32_t w[4];  // fp16: eight halves; one byte: eight bytes in w[0], w[1]
-    float s = 0.f;
-    if constexpr (KIND == kRowsF16) {
+    constexpr bool kWide = sizeof(T) == 4;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        w[e] = pair_bits(x[2 * e], x[2 * e + 1], static_cast<const __half*>(nullptr));
-    } else {
+    for (int c = 0; c < 2; ++c) {
+      uint32_t mc = max(m[c], __shfl_xor_sync(mask, m[c], 1));
+      const uint32_t far = __shfl_xor_sync(mask, mc, 2);
+      if (apart) mc = max(mc, far);
+      const uint32_t sb = fp4::scale_byte<kWide>(mc);
+      const float s = fp4::scale_value(sb), inv = fp4::scale_inverse<kWide>(sb);
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = fp4::code_y<kWide>(v[4 * c + e], s, inv);
+      const int o = c ? ob : oa;
+      *reinterpret_cast<uint16_t*>(grp + t * fp4::kCodeRow + o / 2) =
+          (uint16_t)(fp4::code_pair(y[0], y[1]) | (fp4::code_pair(y[2], y[3]) << 8));
+      if ((o & 15) == 0) grp[fp4::scale_offset(is_v, t, o / 16)] = (uint8_t)sb;
+    }
+  } else {
+    float s = 0.f, inv = 0.f;
+    if constexpr (KIND != kRowsF16) {
       float am = 0.f;
 #pragma unroll
-      for (int e = 0; e < kVals; ++e) am = fmaxf(am, fabsf(x[e]));
+      for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(v[e]));
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) am = fmaxf(am, __shfl_xor_sync(mask, am, o));
       s = KIND == kRowsI8 ? token_scale<T>(am) : __fdiv_rn(am, 448.f);
-      const float inv = KIND == kRowsI8 ? __frcp_rn(s) : 0.f;
-      w[0] = w[1] = 0u;
-#pragma unroll
-      for (int e = 0; e < kVals; ++e) {
-        uint32_t q;
-        if constexpr (KIND == kRowsI8) {
-          q = (uint8_t)quant_fast(x[e], s, inv);
-        } else {
-          q = s > 0.f ? (uint32_t)(uint8_t)__nv_cvt_float_to_fp8(__fdiv_rn(x[e], s),
-                                                                 __NV_SATFINITE, __NV_E4M3)
-                      : 0u;
-        }
-        w[e >> 2] |= q << (8 * (e & 3));
-      }
+      inv = KIND == kRowsI8 ? __frcp_rn(s) : 0.f;
     }
     constexpr int ES = KIND == kRowsF16 ? 2 : 1;
-    uint8_t* c = static_cast<uint8_t*>(cache);
-    if (!is_v) {  // K page [D/8][bs][8]: a lane's values are one chunk
-      uint8_t* dst = c + ((page * 16 + l) * (size_t)bs + off) * 8 * ES;
-      if constexpr (KIND == kRowsF16) {
-        *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-      } else {
-        *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
-      }
-    } else {  // V page [D][bs]
+    uint8_t* c8 = static_cast<uint8_t*>(cache);
 #pragma unroll
-      for (int e = 0; e < kVals; ++e) {
-        const size_t i = (page * 128 + 8 * l + e) * bs + off;
+    for (int c = 0; c < 2; ++c) {
+      const int o = c ? ob : oa;
+      uint32_t w[2] = {0u, 0u};  // fp16: four halves; one byte: four bytes in w[0]
+      if constexpr (KIND == kRowsF16) {
+        w[0] = pair_bits(x[2 * c], static_cast<const __half*>(nullptr));
+        w[1] = pair_bits(x[2 * c + 1], static_cast<const __half*>(nullptr));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t q;
+          if constexpr (KIND == kRowsI8) {
+            q = (uint8_t)quant_fast(v[4 * c + e], s, inv);
+          } else {
+            q = s > 0.f ? (uint32_t)(uint8_t)__nv_cvt_float_to_fp8(__fdiv_rn(v[4 * c + e], s),
+                                                                   __NV_SATFINITE, __NV_E4M3)
+                        : 0u;
+          }
+          w[0] |= q << (8 * e);
+        }
+      }
+      if (!is_v) {  // K page [D/8][bs][8]
+        uint8_t* dst = c8 + ((page * 16 + o / 8) * (size_t)bs + off) * 8 * ES + (o & 7) * ES;
         if constexpr (KIND == kRowsF16) {
-          reinterpret_cast<uint16_t*>(c)[i] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+          *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
         } else {
-          c[i] = (uint8_t)(w[e >> 2] >> (8 * (e & 3)));
+          *reinterpret_cast<uint32_t*>(dst) = w[0];
+        }
+      } else {  // V page [D][bs]
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const size_t i = (page * 128 + o + e) * bs + off;
+          if constexpr (KIND == kRowsF16) {
+            reinterpret_cast<uint16_t*>(c8)[i] = (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+          } else {
+            c8[i] = (uint8_t)(w[0] >> (8 * e));
+          }
         }
       }
     }
@@ -161,162 +159,198 @@ __device__ __forceinline__ void cache_row(const float (&x)[kVals], int l, unsign
   }
 }
 
-// kCache: the cache's RowKind, or -1 for k rows written to k_out (and no V).
-template <typename T, int kCache, int kHeads>
+// kCache: the cache's RowKind, or -1 for k rows written to k_out (and no V). kInter: pairs
+// (2i, 2i + 1).
+template <typename T, int kCache, int kHeads, bool kInter>
 __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeArgs a) {
+  using R = typename Raw<T>::type;
   const int lane = threadIdx.x & 31;
   const int l = lane & 15;  // lane of the row
   const int half = lane >> 4;
   const unsigned mask = 0xffffu << (16 * half);
-  const int heads = a.H + a.KVH + (kCache >= 0 ? a.KVH : 0);
-  const int per_token = (heads + 2 * kHeads - 1) / (2 * kHeads);  // warps of a token
-  const long long gw = ((long long)blockIdx.x * kThreads + threadIdx.x) >> 5;
-  const long long n = gw / per_token;
-  if (n >= a.N) return;
-  const int h0 = (int)(gw - n * per_token) * 2 * kHeads + half;
+  // Warps of a token: those of its q rows, then k, then v.
+  const int qw = (a.H + 2 * kHeads - 1) / (2 * kHeads);
+  const int kw = (a.KVH + 2 * kHeads - 1) / (2 * kHeads);
+  const unsigned per_token = qw + (kCache >= 0 ? 2 : 1) * kw;
+  const unsigned gw = blockIdx.x * (unsigned)(kThreads / 32) + (threadIdx.x >> 5);
+  const unsigned n = gw / per_token;
+  if (n >= (unsigned)a.N) return;
+  int w = (int)(gw - n * per_token);
+  const bool is_q = w < qw;
+  const bool is_v = w >= qw + kw;
+  if (!is_q) w -= is_v ? qw + kw : qw;
+  const int heads = is_q ? a.H : a.KVH;
+  const int h0 = w * 2 * kHeads + half;  // this half-warp's heads: h0, h0 + 2, ...
 
-  // This half-warp's heads: h0, h0 + 2, ... (q heads, then k, then v).
-  Row8<T> raw[kHeads];
+  // The lane's chunks.
+  const int turning = is_v ? 0 : a.rot >> 3;  // lanes whose values turn
+  const bool apart = !kInter && l < turning;
+  const int oa = apart ? 4 * l : 8 * l;
+  const int ob = apart ? (a.rot >> 1) + 4 * l : 8 * l + 4;
+
+  const int pos = __ldg(a.positions + n);  // first: the table's row waits for it
+  const T* src = static_cast<const T*>(is_q ? a.q : (is_v ? a.v : a.k)) +
+                 (size_t)n * (is_q ? a.q_stride : (is_v ? a.v_stride : a.k_stride));
+  R ra[kHeads], rb[kHeads];
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
     const int h = h0 + 2 * i;
-    const T* src;
-    if (h < a.H) {
-      src = static_cast<const T*>(a.q) + n * a.q_stride + (size_t)h * 128;
-    } else if (h < a.H + a.KVH) {
-      src = static_cast<const T*>(a.k) + n * a.k_stride + (size_t)(h - a.H) * 128;
-    } else if (h < heads) {
-      src = static_cast<const T*>(a.v) + n * a.v_stride + (size_t)(h - a.H - a.KVH) * 128;
-    } else {
-      break;
+    if (h < heads) {
+      ra[i] = load4(src + h * 128 + oa);
+      rb[i] = load4(src + h * 128 + ob);
     }
-    raw[i] = load8(src + kVals * l);
   }
 
-  const int pos = __ldg(a.positions + n);
   if (pos < 0) return;  // padding token
   if (pos >= a.table_len) {
-    if (lane == 0 && h0 == 0) flag_error(a.status, PA_ERR_POSITION);
+    if (lane == 0 && w == 0 && is_q == (a.H > 0)) flag_error(a.status, PA_ERR_POSITION);
     return;
   }
   // This token's place in the cache: page row of kv head 0, or none.
   long long page0 = -1;
   int off = 0;
   if constexpr (kCache >= 0) {
-    const int slot = __ldg(a.slots + n);
-    if (slot >= 0) {
-      const int blk = slot / a.bs;
-      if (blk < a.NB) {
-        page0 = (long long)blk * a.KVH;
-        off = slot - blk * a.bs;
-      } else if (lane == 0 && h0 == 0) {
-        flag_error(a.status, PA_ERR_SLOT);
+    if (!is_q) {
+      const int slot = __ldg(a.slots + n);
+      if (slot >= 0) {
+        const int blk = slot / a.bs;
+        if (blk < a.NB) {
+          page0 = (long long)blk * a.KVH;
+          off = slot - blk * a.bs;
+        } else if (lane == 0 && w == 0 && !is_v) {
+          flag_error(a.status, PA_ERR_SLOT);
+        }
       }
+      if (page0 < 0) return;
     }
   }
 
-  // Cosines and sines of the lane's values: pairs share an angle, so the values 8l .. 8l + 7
-  // need angles (8l .. 8l + 7) mod rot/2, or 4l .. 4l + 3 interleaved. Lanes past rot turn by
-  // angle zero.
-  const int rl = a.rot >> 3;      // lanes that turn
-  const int hl = a.rot >> 4;      // lanes between a pair's halves (not interleaved)
-  float c[kVals], s[kVals];
+  // Rotation coefficients with the weights folded in. Not interleaved: (a, b) = (chunk a, chunk b)
+  // value by value; interleaved: (even, odd) values of the two chunks.
+  //   u = a (c w_a) - b (s w_b),  v = b (c w_b) + a (s w_a)
+  float2 cu[2], su[2], cv[2], sv[2];
+  const T* wt = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
+  const bool norm = !is_v && wt != nullptr;
+  if (!is_v) {
+    float2 wa[2], wb[2];
+    if (norm) {
+      widen(load4(wt + oa), static_cast<const T*>(nullptr), wa);
+      widen(load4(wt + ob), static_cast<const T*>(nullptr), wb);
+    } else {
+      wa[0] = wa[1] = wb[0] = wb[1] = make_float2(1.f, 1.f);
+    }
+    float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (l < turning) {
+      const float* row = a.table + (size_t)pos * a.rot + 4 * l;
+      c = __ldg(reinterpret_cast<const float4*>(row));
+      s = __ldg(reinterpret_cast<const float4*>(row + (a.rot >> 1)));
+    }
+    const float2 c2[2] = {make_float2(c.x, c.y), make_float2(c.z, c.w)};
+    const float2 s2[2] = {make_float2(s.x, s.y), make_float2(s.z, s.w)};
+    if constexpr (kInter) {
+      // The pair's a-values: even values of the lane's eight; w likewise.
+      const float2 we[2] = {make_float2(wa[0].x, wa[1].x), make_float2(wb[0].x, wb[1].x)};
+      const float2 wo[2] = {make_float2(wa[0].y, wa[1].y), make_float2(wb[0].y, wb[1].y)};
 #pragma unroll
-  for (int e = 0; e < kVals; ++e) {
-    c[e] = 1.f;
-    s[e] = 0.f;
-  }
-  if (l < rl) {
-    const float* row = a.table + (size_t)pos * a.rot;
-    if (a.interleaved) {
-      const float4 c4 = __ldg(reinterpret_cast<const float4*>(row + 4 * l));
-      const float4 s4 = __ldg(reinterpret_cast<const float4*>(row + a.rot / 2 + 4 * l));
-      const float cc[4] = {c4.x, c4.y, c4.z, c4.w}, ss[4] = {s4.x, s4.y, s4.z, s4.w};
-#pragma unroll
-      for (int e = 0; e < kVals; ++e) {
-        c[e] = cc[e >> 1];
-        s[e] = (e & 1) ? ss[e >> 1] : -ss[e >> 1];
+      for (int i = 0; i < 2; ++i) {
+        cu[i] = mul2(c2[i], we[i]);
+        su[i] = mul2(make_float2(-s2[i].x, -s2[i].y), wo[i]);
+        cv[i] = mul2(c2[i], wo[i]);
+        sv[i] = mul2(s2[i], we[i]);
       }
     } else {
-      const bool up = l >= hl;  // second halves of the pairs: b c + a s, else a c - b s
-      const float4* p = reinterpret_cast<const float4*>(row + 8 * (up ? l - hl : l));
-      const float4* q = reinterpret_cast<const float4*>(row + a.rot / 2 + 8 * (up ? l - hl : l));
-      const float4 c0 = __ldg(p), c1 = __ldg(p + 1), s0 = __ldg(q), s1 = __ldg(q + 1);
-      const float cc[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-      const float ss[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
-      for (int e = 0; e < kVals; ++e) {
-        c[e] = cc[e];
-        s[e] = up ? ss[e] : -ss[e];
+      for (int i = 0; i < 2; ++i) {
+        cu[i] = mul2(c2[i], wa[i]);
+        su[i] = mul2(make_float2(-s2[i].x, -s2[i].y), wb[i]);
+        cv[i] = mul2(c2[i], wb[i]);
+        sv[i] = mul2(s2[i], wa[i]);
       }
     }
   }
-  // The lane holding the other halves (itself where nothing turns).
-  const int other = (lane & 16) | (l < hl ? l + hl : (l < rl ? l - hl : l));
 
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
     const int h = h0 + 2 * i;
     if (h >= heads) break;
-    float x[kVals];
-    widen(raw[i], x);
-    const bool is_q = h < a.H;
-    const bool is_v = kCache >= 0 && h >= a.H + a.KVH;
+    float2 x[4];  // chunk a, chunk b
+    {
+      float2 xa[2], xb[2];
+      widen(ra[i], static_cast<const T*>(nullptr), xa);
+      widen(rb[i], static_cast<const T*>(nullptr), xb);
+      x[0] = xa[0]; x[1] = xa[1]; x[2] = xb[0]; x[3] = xb[1];
+    }
     if (!is_v) {
-      const T* w = static_cast<const T*>(is_q ? a.q_weight : a.k_weight);
-      if (w != nullptr) {
-        float sum = 0.f;
+      if (norm) {
+        float2 q2 = mul2(x[0], x[0]);
 #pragma unroll
-        for (int e = 0; e < kVals; ++e) sum = fmaf(x[e], x[e], sum);
+        for (int e = 1; e < 4; ++e) q2 = fma2(x[e], x[e], q2);
+        float sum = q2.x + q2.y;
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
-        const float inv = __frcp_rn(__fsqrt_rn(fmaf(sum, 1.f / 128.f, a.eps)));
-        float wv[kVals];
-        widen(load8(w + kVals * l), wv);
+        const float r = rsqrtf(fmaf(sum, 1.f / 128.f, a.eps));
 #pragma unroll
-        for (int e = 0; e < kVals; ++e) x[e] = x[e] * inv * wv[e];
+        for (int e = 0; e < 4; ++e) x[e] = mul2(x[e], make_float2(r, r));
       }
-      float y[kVals];
+      if constexpr (kInter) {
 #pragma unroll
-      for (int e = 0; e < kVals; ++e) {
-        const float o = a.interleaved ? x[e ^ 1] : __shfl_sync(mask, x[e], other);
-        y[e] = fmaf(x[e], c[e], o * s[e]);
+        for (int e = 0; e < 2; ++e) {
+          const float2 p = make_float2(x[2 * e].x, x[2 * e + 1].x);
+          const float2 q = make_float2(x[2 * e].y, x[2 * e + 1].y);
+          const float2 u = fma2(q, su[e], mul2(p, cu[e]));
+          const float2 v = fma2(p, sv[e], mul2(q, cv[e]));
+          x[2 * e] = make_float2(u.x, v.x);
+          x[2 * e + 1] = make_float2(u.y, v.y);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 u = fma2(x[2 + e], su[e], mul2(x[e], cu[e]));
+          const float2 v = fma2(x[e], sv[e], mul2(x[2 + e], cv[e]));
+          x[e] = u;
+          x[2 + e] = v;
+        }
       }
-#pragma unroll
-      for (int e = 0; e < kVals; ++e) x[e] = y[e];
     }
-    if (is_q) {
-      store8(static_cast<T*>(a.q_out) + n * a.qo_stride + (size_t)h * 128 + kVals * l, x);
-    } else if constexpr (kCache < 0) {
-      store8(static_cast<T*>(a.k_out) + n * a.ko_stride + (size_t)(h - a.H) * 128 + kVals * l,
-             x);
-    } else if (page0 >= 0) {
-      const int kvh = h - a.H - (is_v ? a.KVH : 0);
+    if (kCache < 0 || is_q) {
+      T* dst = is_q ? static_cast<T*>(a.q_out) + (size_t)n * a.qo_stride + h * 128
+                    : static_cast<T*>(a.k_out) + (size_t)n * a.ko_stride + h * 128;
+      const float2 lo[2] = {x[0], x[1]}, hi[2] = {x[2], x[3]};
+      store4(dst + oa, lo);
+      store4(dst + ob, hi);
+    } else if constexpr (kCache >= 0) {
       if (!is_v) {
 #pragma unroll
-        for (int e = 0; e < kVals; ++e) x[e] = In<T>::round_t(x[e]);
+        for (int e = 0; e < 4; ++e)
+          x[e] = make_float2(In<T>::round_t(x[e].x), In<T>::round_t(x[e].y));
       }
-      cache_row<T, kCache>(x, l, mask, is_v, is_v ? a.v_cache : a.k_cache,
-                           is_v ? a.v_scales : a.k_scales, (size_t)page0 + kvh, off, a.bs);
+      cache_row<T, kCache>(x, l, oa, ob, apart, mask, is_v, is_v ? a.v_cache : a.k_cache,
+                           is_v ? a.v_scales : a.k_scales, (size_t)page0 + h, off, a.bs);
     }
   }
 }
 
-template <typename T, int kCache>
-cudaError_t launch_t(const RopeArgs& a, int sms, cudaStream_t st) {
-  const long long heads = a.H + a.KVH + (kCache >= 0 ? a.KVH : 0);
-  // Four heads per half-warp where that still gives every SM sixteen warps, else one.
-  const long long w4 = (long long)a.N * ((heads + 7) / 8);
-  const bool few = w4 < 16LL * sms;
-  const long long warps = few ? (long long)a.N * ((heads + 1) / 2) : w4;
+template <typename T, int kCache, int kHeads>
+cudaError_t launch_heads(const RopeArgs& a, long long warps, cudaStream_t st) {
   const long long grid = (warps + kThreads / 32 - 1) / (kThreads / 32);
-  if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
-  if (few) {
-    norm_rope_kernel<T, kCache, 1><<<(int)grid, kThreads, 0, st>>>(a);
+  if (warps > 0x7fffffffLL) return cudaErrorInvalidValue;
+  if (a.interleaved) {
+    norm_rope_kernel<T, kCache, kHeads, true><<<(int)grid, kThreads, 0, st>>>(a);
   } else {
-    norm_rope_kernel<T, kCache, 4><<<(int)grid, kThreads, 0, st>>>(a);
+    norm_rope_kernel<T, kCache, kHeads, false><<<(int)grid, kThreads, 0, st>>>(a);
   }
   return cudaGetLastError();
+}
+
+template <typename T, int kCache>
+cudaError_t launch_t(const RopeArgs& a, int sms, cudaStream_t st) {
+  auto warps = [&](int heads) {  // of the launch with `heads` heads a half-warp
+    auto of = [&](int h) { return (h + 2LL * heads - 1) / (2 * heads); };
+    return a.N * (of(a.H) + (kCache >= 0 ? 2 : 1) * of(a.KVH));
+  };
+  // Four heads per half-warp where that still gives every SM sixteen warps, else one.
+  if (warps(4) >= 16LL * sms) return launch_heads<T, kCache, 4>(a, warps(4), st);
+  return launch_heads<T, kCache, 1>(a, warps(1), st);
 }
 
 template <typename T>

@@ -6,15 +6,18 @@
 // block a sequence grows by, in sequence order, so the result does not depend on timing.
 //
 // A sequence's place (its first token in the packed batch, its first popped or pushed block) is
-// an exclusive prefix sum over the sequences before it. Every CTA takes a range of tokens (or
-// of pushed blocks) and runs the same scan over the lengths, 1024 sequences at a time in shared
-// memory, searching each chunk for its own items; the lengths are a few KB and stay in L2, so
-// the repeated scan costs less than a second launch would. Nothing is changed unless the whole
-// call fits: a first scan of the totals decides that, in every CTA alike. The lengths and the
-// count may be updated in place: the CTAs are one cluster, and its first one writes them after a
-// cluster barrier, when all have read. (A counter in the workspace would allow more CTAs, but
-// two captured graphs that share a workspace would share the counter; eight SMs write the maps
-// of 64 K tokens as fast as the launch itself.)
+// an exclusive prefix sum over the sequences before it. Every CTA runs the same scan over the
+// lengths, a chunk of sequences (one a thread) at a time in shared memory, and searches it for
+// its own items; the lengths are a few KB and stay in L2, so the repeated scan costs less than a
+// second launch would. Nothing is changed unless the whole call fits: the totals of a first scan
+// decide that, in every CTA alike (with one chunk, its scan is kept). The lengths and the count
+// may be updated in place: the CTAs are one cluster, and its first one writes them after a
+// cluster barrier, when all have read. (A counter in the workspace would allow more CTAs, but two
+// captured graphs that share a workspace would share the counter.)
+//
+// Both are bound by latency (256 requests: 5 us for the pair of them, against 8 bytes a token to
+// write): a chain of dependent loads and barriers, so small calls run in small CTAs, and a thread
+// takes four neighbouring tokens, which nearly always share their sequence and block.
 
 #include "pa_common.cuh"
 #include "pa_internal.h"
@@ -22,56 +25,51 @@
 namespace pa {
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kWarps = kThreads / 32;
+constexpr int kMaxThreads = 1024;
+constexpr int kTokens = 4;  // neighbouring tokens of a thread
 
-// Inclusive sums over the block of two counts per thread; returns the block's totals in tot.
+// Two counts per sequence, saturating at 2^31 - 1 (which every caller's limit refuses).
 struct Pair {
-  long long a, b;
+  unsigned a, b;
 };
-
-__device__ __forceinline__ Pair shfl_up(Pair v, int o) {
-  return Pair{__shfl_up_sync(0xffffffffu, v.a, o), __shfl_up_sync(0xffffffffu, v.b, o)};
+constexpr unsigned kSaturated = 0x7fffffffu;
+__device__ __forceinline__ unsigned sat_add(unsigned x, unsigned y) {
+  return min(x + y, kSaturated);  // both at most 2^31 - 1: no wrap
+}
+__device__ __forceinline__ Pair sat_add(Pair x, Pair y) {
+  return Pair{sat_add(x.a, y.a), sat_add(x.b, y.b)};
 }
 
+// Inclusive sums over the block; the block's totals in tot. s_warp: 32 entries.
 __device__ __forceinline__ Pair block_scan(Pair v, Pair* s_warp, Pair& tot) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const Pair u = shfl_up(v, o);
-    if (lane >= o) {
-      v.a += u.a;
-      v.b += u.b;
-    }
-  }
-  if (lane == 31) s_warp[warp] = v;
-  __syncthreads();
-  if (warp == 0) {
-    Pair w = s_warp[lane];  // kWarps == 32
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  auto warp_scan = [&](Pair x) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const Pair u = shfl_up(w, o);
-      if (lane >= o) {
-        w.a += u.a;
-        w.b += u.b;
-      }
+      const Pair u{__shfl_up_sync(0xffffffffu, x.a, o), __shfl_up_sync(0xffffffffu, x.b, o)};
+      if (lane >= o) x = sat_add(x, u);
     }
-    s_warp[lane] = w;
-  }
+    return x;
+  };
+  v = warp_scan(v);
+  if (lane == 31) s_warp[warp] = v;
   __syncthreads();
-  if (warp > 0) {
-    v.a += s_warp[warp - 1].a;
-    v.b += s_warp[warp - 1].b;
-  }
-  tot = s_warp[kWarps - 1];
-  __syncthreads();
+  // Every warp scans the warps' totals for itself: one barrier less.
+  const Pair w = warp_scan(lane < warps ? s_warp[lane] : Pair{0u, 0u});
+  tot = Pair{__shfl_sync(0xffffffffu, w.a, 31), __shfl_sync(0xffffffffu, w.b, 31)};
+  const Pair before{__shfl_sync(0xffffffffu, w.a, max(warp - 1, 0)),
+                    __shfl_sync(0xffffffffu, w.b, max(warp - 1, 0))};
+  if (warp > 0) v = sat_add(v, before);
+  __syncthreads();  // s_warp may be used again
   return v;
 }
 
-__device__ __forceinline__ int ceil_div(int a, int b) { return (int)(((unsigned)a + b - 1) / (unsigned)b); }
+__device__ __forceinline__ int ceil_div(int a, int b) {
+  return (int)(((unsigned)a + (unsigned)b - 1u) / (unsigned)b);
+}
 
 // Largest i in [0, n) with s[i] <= x (s ascending, s[0] <= x).
-__device__ __forceinline__ int find(const long long* s, int n, long long x) {
+__device__ __forceinline__ int find(const unsigned* s, int n, unsigned x) {
   int lo = 0, hi = n - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -89,87 +87,103 @@ __device__ __forceinline__ void cluster_barrier() {
           : "memory");
 }
 
-__global__ void __launch_bounds__(kThreads) release_kernel(const TableArgs a) {
-  __shared__ long long s_off[kThreads];
-  __shared__ Pair s_warp[kWarps];
-  const int tid = threadIdx.x;
+__global__ void __launch_bounds__(kMaxThreads) release_kernel(const TableArgs a) {
+  __shared__ unsigned s_off[kMaxThreads];
+  __shared__ Pair s_warp[32];
+  const int tid = threadIdx.x, nthr = blockDim.x;
   const int cap = a.max_blocks * a.bs;
   const int top = __ldg(a.free_count);
+  const bool single = a.S <= nthr;
 
   int err = 0;
-  long long total = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    if (pass == 1) {
-      if (top < 0 || top + total > a.pool) err |= PA_ERR_FREE_BLOCKS;
-      if (__syncthreads_or(err) != 0) break;
-    }
-    long long carry = 0;
-    for (int base = 0; base < a.S; base += kThreads) {
+  unsigned total = 0;
+  int kept = 0, was = 0;  // one chunk: this thread's sequence's new and old length
+  bool ok = false;
+  for (int pass = single ? 1 : 0; pass < 2; ++pass) {
+    unsigned carry = 0;
+    for (int base = 0; base < a.S || base == 0; base += nthr) {
       const int i = base + tid;
       int n = 0;
-      if (i < a.S && __ldg(a.flags + i) != 0) {
-        const int c = __ldg(a.lens + i);
-        if (c < 0 || c > cap) {
-          err |= PA_ERR_CONTEXT_RANGE;
-        } else {
-          n = ceil_div(c, a.bs);
+      if (i < a.S) {
+        const int f = __ldg(a.flags + i), c = __ldg(a.lens + i);
+        kept = f != 0 ? 0 : c;
+        was = c;
+        if (f != 0) {
+          if (c < 0 || c > cap) {
+            err |= PA_ERR_CONTEXT_RANGE;
+          } else {
+            n = ceil_div(c, a.bs);
+          }
         }
       }
       Pair tot;
-      const Pair v = block_scan(Pair{n, 0}, s_warp, tot);
-      if (pass == 1 && tot.a > 0) {
-        s_off[tid] = carry + v.a - n;
-        __syncthreads();
-        const int cnt = min(kThreads, a.S - base);
-        // Pushed block r of the chunk: CTAs take them in turn, a thread each.
-        for (long long r = carry + (long long)blockIdx.x * kThreads + tid; r < carry + tot.a;
-             r += (long long)gridDim.x * kThreads) {
-          const int q = find(s_off, cnt, r);
-          const int j = (int)(r - s_off[q]);
-          a.free_blocks[top + r] = __ldg(a.table + (size_t)(base + q) * a.max_blocks + j);
+      const Pair v = block_scan(Pair{(unsigned)n, 0u}, s_warp, tot);
+      if (single) total = tot.a;
+      if (pass == 1) {
+        if (base == 0) {  // the totals are known: does the call fit?
+          if (top < 0 || (long long)top + total > a.pool || total == kSaturated)
+            err |= PA_ERR_FREE_BLOCKS;
+          ok = __syncthreads_or(err) == 0;
+          if (!ok) break;
         }
-        __syncthreads();
+        if (tot.a > 0) {
+          s_off[tid] = carry + v.a - n;
+          __syncthreads();
+          const int cnt = min(nthr, a.S - base);
+          // Pushed block r of the chunk: CTAs take them in turn, a thread each.
+          for (unsigned r = carry + blockIdx.x * nthr + tid; r < carry + tot.a;
+               r += gridDim.x * nthr) {
+            const int q = find(s_off, cnt, r);
+            const int j = (int)(r - s_off[q]);
+            a.free_blocks[top + (int)r] =
+                __ldg(a.table + (size_t)(base + q) * a.max_blocks + j);
+          }
+          __syncthreads();
+        }
       }
-      carry += tot.a;
+      carry = sat_add(carry, tot.a);
     }
-    total = carry;
+    if (pass == 0) total = carry;
   }
-  const bool ok = __syncthreads_or(err) == 0;
   if (!ok && blockIdx.x == 0 && err != 0) flag_error(a.status, err);
   cluster_barrier();
   if (blockIdx.x != 0) return;
-  for (int i = tid; i < a.S; i += kThreads) {
-    const int c = a.lens[i];
-    a.lens_out[i] = ok && a.flags[i] != 0 ? 0 : c;
+  if (single) {
+    if (tid < a.S) a.lens_out[tid] = ok ? kept : was;
+  } else {
+    for (int i = tid; i < a.S; i += nthr) {
+      const int c = a.lens[i];
+      a.lens_out[i] = ok && a.flags[i] != 0 ? 0 : c;
+    }
   }
-  if (tid == 0) *a.count_out = ok ? (int)(top + total) : top;
+  if (tid == 0) *a.count_out = ok ? top + (int)total : top;
 }
 
-__global__ void __launch_bounds__(kThreads) extend_kernel(const TableArgs a) {
-  __shared__ long long s_tok[kThreads], s_blk[kThreads];
-  __shared__ int s_len[kThreads];
-  __shared__ Pair s_warp[kWarps];
-  const int tid = threadIdx.x;
+__global__ void __launch_bounds__(kMaxThreads) extend_kernel(const TableArgs a) {
+  __shared__ unsigned s_tok[kMaxThreads], s_blk[kMaxThreads];
+  __shared__ int s_len[kMaxThreads];
+  __shared__ Pair s_warp[32];
+  const int tid = threadIdx.x, nthr = blockDim.x;
   const long long cap = (long long)a.max_blocks * a.bs;
   const int top = __ldg(a.free_count);
-  const long long stride = (long long)gridDim.x * kThreads;
-  const long long me = (long long)blockIdx.x * kThreads + tid;
+  const unsigned stride = gridDim.x * nthr * kTokens;
+  const unsigned me = (blockIdx.x * nthr + tid) * kTokens;
+  const bool single = a.S <= nthr;
 
   int err = 0;
-  long long tokens = 0, blocks = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    if (pass == 1) {
-      if (tokens > a.max_tokens) err |= PA_ERR_TOKENS;
-      if (top < 0 || top > a.pool || blocks > top) err |= PA_ERR_FREE_BLOCKS;
-      if (__syncthreads_or(err) != 0) break;
-    }
-    Pair carry{0, 0};
-    for (int base = 0; base < a.S; base += kThreads) {
+  Pair total{0u, 0u};
+  int kept = 0, was = 0;  // one chunk: this thread's sequence's new and old length
+  bool ok = false;
+  for (int pass = single ? 1 : 0; pass < 2; ++pass) {
+    Pair carry{0u, 0u};
+    for (int base = 0; base < a.S || base == 0; base += nthr) {
       const int i = base + tid;
       int c = 0, add = 0, need = 0;
       if (i < a.S) {
         c = __ldg(a.lens + i);
         add = __ldg(a.flags + i);
+        was = c;
+        kept = (int)((unsigned)c + (unsigned)add);
         if (c < 0 || add < 0 || (long long)c + add > cap) {
           err |= PA_ERR_CONTEXT_RANGE;
           c = add = 0;
@@ -177,77 +191,103 @@ __global__ void __launch_bounds__(kThreads) extend_kernel(const TableArgs a) {
         need = ceil_div(c + add, a.bs) - ceil_div(c, a.bs);
       }
       Pair tot;
-      const Pair v = block_scan(Pair{add, need}, s_warp, tot);
+      const Pair v = block_scan(Pair{(unsigned)add, (unsigned)need}, s_warp, tot);
+      if (single) total = tot;
       if (pass == 1) {
+        if (base == 0) {
+          if (total.a == kSaturated || total.a > (unsigned)a.max_tokens) err |= PA_ERR_TOKENS;
+          if (top < 0 || top > a.pool || total.b > (unsigned)max(top, 0))
+            err |= PA_ERR_FREE_BLOCKS;
+          ok = __syncthreads_or(err) == 0;
+          if (!ok) break;
+        }
         s_tok[tid] = carry.a + v.a - add;
         s_blk[tid] = carry.b + v.b - need;
         s_len[tid] = c;
         if (blockIdx.x == 0 && i < a.S) a.starts[i] = (int)(carry.a + v.a - add);
         __syncthreads();
-        const int cnt = min(kThreads, a.S - base);
-        // The CTA's tokens (every gridDim-th run of kThreads) that lie in this chunk.
-        long long t = me;
-        if (t < carry.a) t += (carry.a - t + stride - 1) / stride * stride;
-        for (; t < carry.a + tot.a; t += stride) {
-          const int q = find(s_tok, cnt, t);
-          const int len = s_len[q];
-          const int pos = len + (int)(t - s_tok[q]);
-          const int col = (int)((unsigned)pos / (unsigned)a.bs);
-          const int off = pos - col * a.bs;
-          const int had = ceil_div(len, a.bs);
-          int* cell = a.table + (size_t)(base + q) * a.max_blocks + col;
-          int blk;
-          if (col >= had) {
-            blk = __ldg(a.free_blocks + (top - 1 - (s_blk[q] + col - had)));
-            if (off == 0) *cell = blk;  // each new block's first token is new
-          } else {
-            blk = *cell;
+        const int cnt = min(nthr, a.S - base);
+        const unsigned end = carry.a + tot.a;
+        // This thread's runs of four tokens that reach into the chunk.
+        unsigned t0 = me;
+        if (t0 + kTokens <= carry.a)
+          t0 += (carry.a - t0 - kTokens) / stride * stride + stride;
+        for (; t0 < end; t0 += stride) {
+          int q = -1, last_col = -1, blk = 0;
+#pragma unroll
+          for (int e = 0; e < kTokens; ++e) {
+            const unsigned t = t0 + e;
+            if (t < carry.a || t >= end) continue;
+            if (q < 0 || (q + 1 < cnt && s_tok[q + 1] <= t)) {
+              q = find(s_tok, cnt, t);
+              last_col = -1;
+            }
+            const int len = s_len[q];
+            const int pos = len + (int)(t - s_tok[q]);
+            const int col = (int)((unsigned)pos / (unsigned)a.bs);
+            const int off = pos - col * a.bs;
+            if (col != last_col) {
+              last_col = col;
+              const int had = ceil_div(len, a.bs);
+              int* cell = a.table + (size_t)(base + q) * a.max_blocks + col;
+              if (col >= had) {
+                blk = __ldg(a.free_blocks + (top - 1 - ((int)s_blk[q] + col - had)));
+                if (off == 0) *cell = blk;  // each new block's first token is new
+              } else {
+                blk = *cell;
+              }
+            }
+            const bool good = blk >= 0 && blk < a.NB;
+            if (!good) flag_error(a.status, PA_ERR_BLOCK_ID);
+            a.slots[t] = good ? blk * a.bs + off : -1;
+            a.positions[t] = pos;
           }
-          const bool good = blk >= 0 && blk < a.NB;
-          if (!good) flag_error(a.status, PA_ERR_BLOCK_ID);
-          a.slots[t] = good ? blk * a.bs + off : -1;
-          a.positions[t] = pos;
         }
         __syncthreads();
       }
-      carry.a += tot.a;
-      carry.b += tot.b;
+      carry = sat_add(carry, tot);
     }
-    tokens = carry.a;
-    blocks = carry.b;
+    if (pass == 0) total = carry;
   }
-  const bool ok = __syncthreads_or(err) == 0;
   if (!ok && blockIdx.x == 0 && err != 0) flag_error(a.status, err);
-  for (long long t = me; t < a.max_tokens; t += stride) {
-    if (ok && t < tokens) continue;
+  // Padding: everything past the last token, or all of a refused call.
+  const unsigned tokens = ok ? total.a : 0u;
+  for (unsigned t = tokens + blockIdx.x * nthr + tid; t < (unsigned)a.max_tokens;
+       t += gridDim.x * nthr) {
     a.slots[t] = -1;
     a.positions[t] = -1;
   }
   if (blockIdx.x == 0) {
     if (!ok)
-      for (int i = tid; i < a.S; i += kThreads) a.starts[i] = 0;
-    if (tid == 0) a.starts[a.S] = ok ? (int)tokens : 0;
+      for (int i = tid; i < a.S; i += nthr) a.starts[i] = 0;
+    if (tid == 0) a.starts[a.S] = (int)tokens;
   }
   cluster_barrier();
   if (blockIdx.x != 0) return;
-  for (int i = tid; i < a.S; i += kThreads) {
-    const int c = a.lens[i];
-    a.lens_out[i] = ok ? c + a.flags[i] : c;
+  if (single) {
+    if (tid < a.S) a.lens_out[tid] = ok ? kept : was;
+  } else {
+    for (int i = tid; i < a.S; i += nthr) {
+      const int c = a.lens[i];
+      a.lens_out[i] = ok ? c + a.flags[i] : c;
+    }
   }
-  if (tid == 0) *a.count_out = ok ? (int)(top - blocks) : top;
+  if (tid == 0) *a.count_out = ok ? top - (int)total.b : top;
 }
 
-}  // namespace
-
-namespace {
-// One cluster of up to eight CTAs (the portable limit), for at most `items` items.
+// One cluster of up to eight CTAs (the portable limit) for at most `items` items of `per` to a
+// thread; a CTA has as many threads as the sequences or its items can use.
 template <typename K>
-cudaError_t launch_cluster(K kern, const TableArgs& a, long long items, cudaStream_t st) {
+cudaError_t launch_cluster(K kern, const TableArgs& a, long long items, int per,
+                           cudaStream_t st) {
+  const long long want = (items + per - 1) / per > a.S ? (items + per - 1) / per : a.S;
+  int threads = 128;
+  while (threads < kMaxThreads && threads < want) threads *= 2;
   unsigned n = 1;
-  while (n < 8 && (long long)n * kThreads < items) n *= 2;
+  while (n < 8 && (long long)n * threads * per < items) n *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(n);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -258,15 +298,17 @@ cudaError_t launch_cluster(K kern, const TableArgs& a, long long items, cudaStre
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, a);
 }
+
 }  // namespace
 
 cudaError_t launch_release(const TableArgs& a, cudaStream_t st) {
-  // The pushed blocks are not known on the host: at most max_blocks a sequence.
-  return launch_cluster(release_kernel, a, (long long)a.S * a.max_blocks, st);
+  // The pushed blocks are not known on the host: at most max_blocks a sequence, rarely
+  // more than an eighth of that.
+  return launch_cluster(release_kernel, a, (long long)a.S * a.max_blocks, 8, st);
 }
 
 cudaError_t launch_extend(const TableArgs& a, cudaStream_t st) {
-  return launch_cluster(extend_kernel, a, a.max_tokens, st);
+  return launch_cluster(extend_kernel, a, a.max_tokens, kTokens, st);
 }
 
 }  // namespace pa

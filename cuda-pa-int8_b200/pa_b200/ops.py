@@ -161,10 +161,43 @@ def _check_fp4_caches(k_cache, v_cache, block_size):
     return shape[0], shape[1]
 
 
+def _check_decode_args_fp4(out, q, k_cache, v_cache, block_table, context_lens, block_size,
+                           k_scales, v_scales, act_dtype):
+    """_check_decode_args over a 4-bit cache."""
+    dev, shape = q.device, q.shape
+    if not (q.is_cuda and q.dtype == act_dtype and len(shape) == 3 and shape[2] == HEAD_DIM and
+            q.is_contiguous()):
+        raise RuntimeError(f"q must be contiguous {act_dtype} [num_seqs, num_heads, {HEAD_DIM}] on "
+                           "CUDA")
+    if out is not None and not (out.dtype == act_dtype and out.device == dev and
+                                out.shape == shape and out.is_contiguous()):
+        raise RuntimeError("out must have the type and shape of q and be contiguous")
+    if block_size <= 0 or 128 % block_size != 0:
+        raise RuntimeError("block_size must divide TILE (multiple of 16)")
+    NB, KVH = _check_fp4_caches(k_cache, v_cache, block_size)
+    _check_on(dev, k_cache, v_cache)
+    if k_scales is not None or v_scales is not None:
+        raise RuntimeError("a 4-bit cache holds its own scales")
+    B, H, D = shape
+    if KVH == 0 or H % KVH != 0:
+        raise RuntimeError("num_heads must be a multiple of num_kv_heads")
+    if not (block_table.dtype == torch.int32 and block_table.device == dev and
+            block_table.dim() == 2 and block_table.shape[0] == B and block_table.is_contiguous()):
+        raise RuntimeError("block_table must be contiguous int32 [num_seqs, max_blocks_per_seq] on "
+                           "q's device")
+    if not (context_lens.dtype == torch.int32 and context_lens.device == dev and
+            context_lens.dim() == 1 and context_lens.shape[0] == B and
+            context_lens.is_contiguous()):
+        raise RuntimeError("context_lens must be contiguous int32 [num_seqs] on q's device")
+    return B, H, KVH, D, NB
+
+
 def _check_decode_args(out, q, k_cache, v_cache, block_table, context_lens, block_size,
                        kind, k_scales, v_scales, act_dtype=torch.float16):
-    scaled = kind in ("i8", "f8")  # one-byte cache with per-token scales
-    fp4 = kind == "f4"
+    if kind == "f4":
+        return _check_decode_args_fp4(out, q, k_cache, v_cache, block_table, context_lens,
+                                      block_size, k_scales, v_scales, act_dtype)
+    scaled = kind != "f16"  # one-byte cache with per-token scales (int8 or fp8)
     _require(q.is_cuda and (out is None or out.is_cuda), "tensors must be on CUDA")
     act_name = "fp16" if act_dtype == torch.float16 else "bf16"
     _require(q.dtype == act_dtype, f"q must be {act_name}")
@@ -179,10 +212,6 @@ def _check_decode_args(out, q, k_cache, v_cache, block_table, context_lens, bloc
                  "k_scales must be fp32")
         _require(v_scales is not None and v_scales.dtype == torch.float32,
                  "v_scales must be fp32")
-    elif fp4:
-        _require(k_cache.dtype == torch.uint8 and v_cache.dtype == torch.uint8,
-                 "a 4-bit cache is uint8, K and V")
-        _require(k_scales is None and v_scales is None, "a 4-bit cache holds its own scales")
     else:
         _require(k_cache.dtype == torch.float16, "k_cache must be fp16")
         _require(v_cache.dtype == torch.float16, "v_cache must be fp16")
@@ -202,25 +231,19 @@ def _check_decode_args(out, q, k_cache, v_cache, block_table, context_lens, bloc
     if out is not None:
         _require(tuple(out.shape) == (B, H, D) and out.dtype == act_dtype,
                  f"out must be {act_name} with the shape of q")
-    if fp4:
-        _require(D == HEAD_DIM, f"head_dim {D} unsupported (this build: {HEAD_DIM})")
-        _require(block_size > 0 and block_size % 16 == 0 and 128 % block_size == 0,
-                 "block_size must divide TILE (multiple of 16)")
-        NB, KVH = _check_fp4_caches(k_cache, v_cache, block_size)
-    else:
-        _require(k_cache.dim() == 5,
-                 "k_cache must be [num_blocks, kv_heads, head_dim/x, block_size, x]")
-        NB, KVH, DX, BS, x = k_cache.shape
-        if scaled:
-            _require(x == 8, "int8 K cache requires x == 8")
-        _require(x == X, "K cache requires x == 8")
-        _require(D == HEAD_DIM, f"head_dim {D} unsupported (this build: {HEAD_DIM})")
-        _require(DX * x == D, "k_cache head_dim/x does not match q")
-        _require(block_size % 16 == 0 and 128 % block_size == 0,
-                 "block_size must divide TILE (multiple of 16)")
-        _require(BS == block_size, f"k_cache block dimension {BS} != block_size {block_size}")
-        _require(tuple(v_cache.shape) == (NB, KVH, D, block_size),
-                 "v_cache must be [num_blocks, kv_heads, head_dim, block_size]")
+    _require(k_cache.dim() == 5,
+             "k_cache must be [num_blocks, kv_heads, head_dim/x, block_size, x]")
+    NB, KVH, DX, BS, x = k_cache.shape
+    if scaled:
+        _require(x == 8, "int8 K cache requires x == 8")
+    _require(x == X, "K cache requires x == 8")
+    _require(D == HEAD_DIM, f"head_dim {D} unsupported (this build: {HEAD_DIM})")
+    _require(DX * x == D, "k_cache head_dim/x does not match q")
+    _require(block_size % 16 == 0 and 128 % block_size == 0,
+             "block_size must divide TILE (multiple of 16)")
+    _require(BS == block_size, f"k_cache block dimension {BS} != block_size {block_size}")
+    _require(tuple(v_cache.shape) == (NB, KVH, D, block_size),
+             "v_cache must be [num_blocks, kv_heads, head_dim, block_size]")
     if scaled:
         _require(tuple(k_scales.shape) == (NB, KVH, block_size) and
                  tuple(v_scales.shape) == (NB, KVH, block_size),
@@ -820,12 +843,12 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, table, *, eps=1e-6, interl
     N, H, qs, KVH, ks = _check_norm_rope(q, k, q_weight, k_weight, positions, table, eps)
     dev, dt = q.device, q.dtype
     if q_out is None:
-        q_out = torch.empty((N, H, HEAD_DIM), dtype=dt, device=dev)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         qos = H * HEAD_DIM
     else:
         _, qos = _head_rows("q_out", q_out, N, H, dt, dev)
     if k_out is None:
-        k_out = torch.empty((N, KVH, HEAD_DIM), dtype=dt, device=dev)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         kos = KVH * HEAD_DIM
     else:
         _, kos = _head_rows("k_out", k_out, N, KVH, dt, dev)
@@ -845,8 +868,8 @@ def norm_rope_into_cache(q, k, v, q_weight, k_weight, positions, table, k_cache,
     """qk_norm_rope with the new K and the V rows going straight into the paged cache at
     slot_mapping, in one launch: bit for bit what qk_norm_rope followed by the cache's write
     (write_into_cache, quantize_into_cache with per-token scales, or quantize_into_cache_fp4)
-    gives. The cache is fp16, int8 or float8_e4m3fn (with k_scales and v_scales), or 4-bit. A
-    negative slot writes nothing to the cache, a negative position skips the token. Returns
+    gives. The cache is fp16, int8 or float8_e4m3fn (with k_scales and v_scales), or 4-bit (with
+    rot_dim a multiple of 32 unless interleaved). A negative slot writes nothing to the cache, a negative position skips the token. Returns
     q_out [num_tokens, heads, 128]; it may be q."""
     N, H, qs, KVH, ks = _check_norm_rope(q, k, q_weight, k_weight, positions, table, eps)
     dev, dt = q.device, q.dtype
@@ -870,7 +893,7 @@ def norm_rope_into_cache(q, k, v, q_weight, k_weight, positions, table, k_cache,
         NB = _check_cache_layout(k_cache, v_cache, KVH, HEAD_DIM, block_size, k_scales, v_scales)
     _check_on(dev, k_cache, v_cache, k_scales, v_scales)
     if q_out is None:
-        q_out = torch.empty((N, H, HEAD_DIM), dtype=dt, device=dev)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         qos = H * HEAD_DIM
     else:
         _, qos = _head_rows("q_out", q_out, N, H, dt, dev)
@@ -889,12 +912,14 @@ def norm_rope_into_cache(q, k, v, q_weight, k_weight, positions, table, k_cache,
 # ---------------------------------------------------------------------------------------
 # Block tables of a step
 # ---------------------------------------------------------------------------------------
-def _int_row(name, t, n, device):
-    """t is a contiguous int32 vector of n entries (None: any number) on the device."""
-    if not (t.dtype == torch.int32 and t.device == device and t.dim() == 1 and
-            (n is None or t.numel() == n) and t.is_contiguous()):
-        raise RuntimeError(f"{name} must be a contiguous int32 vector"
-                           + (f" of {n}" if n is not None else "") + " on block_table's device")
+def _check_int(device, *rows):
+    """rows: (name, tensor, entries or None): contiguous int32 vectors on the device."""
+    for name, t, n in rows:
+        if not (t.dtype == torch.int32 and t.device == device and t.dim() == 1 and
+                (n is None or t.numel() == n) and t.is_contiguous()):
+            raise RuntimeError(f"{name} must be a contiguous int32 vector"
+                               + (f" of {n}" if n is not None else "")
+                               + " on block_table's device")
 
 
 def _check_tables(block_table, context_lens, per_seq, free_blocks, free_count, block_size):
@@ -905,11 +930,10 @@ def _check_tables(block_table, context_lens, per_seq, free_blocks, free_count, b
                            "CUDA")
     if not (shape[1] > 0 and block_size > 0):
         raise RuntimeError("max_blocks_per_seq and block_size must be > 0")
-    _int_row("context_lens", context_lens, shape[0], dev)
-    _int_row("the per-sequence values", per_seq, shape[0], dev)
-    _int_row("free_blocks", free_blocks, None, dev)
-    _int_row("free_count", free_count, 1, dev)
-    return shape[0], shape[1], dev
+    S = shape[0]
+    _check_int(dev, ("context_lens", context_lens, S), ("the per-sequence values", per_seq, S),
+               ("free_blocks", free_blocks, None), ("free_count", free_count, 1))
+    return S, shape[1], dev
 
 
 def release_blocks(block_table, context_lens, finished, free_blocks, free_count, block_size=16,
@@ -923,10 +947,15 @@ def release_blocks(block_table, context_lens, finished, free_blocks, free_count,
     (check_status)."""
     S, max_blocks, dev = _check_tables(block_table, context_lens, finished, free_blocks,
                                        free_count, block_size)
-    lens = torch.empty_like(context_lens) if context_lens_out is None else context_lens_out
-    count = torch.empty_like(free_count) if free_count_out is None else free_count_out
-    _int_row("context_lens_out", lens, S, dev)
-    _int_row("free_count_out", count, 1, dev)
+    lens, count = context_lens_out, free_count_out
+    if lens is None:
+        lens = torch.empty_like(context_lens)
+    else:
+        _check_int(dev, ("context_lens_out", lens, S))
+    if count is None:
+        count = torch.empty_like(free_count)
+    else:
+        _check_int(dev, ("free_count_out", count, 1))
     with _Guard(dev):
         ws = workspace(dev, 256)
         rc = _lib.lib().pa_release_blocks(
@@ -958,14 +987,15 @@ def extend_block_tables(block_table, context_lens, new_lens, free_blocks, free_c
         raise RuntimeError("max_tokens must be >= 0")
     outs = [slot_mapping, positions, query_start, context_lens_out, free_count_out]
     sizes = [max_tokens, max_tokens, S + 1, S, 1]
-    if not any(t is not None for t in outs):  # one allocation, split
-        outs = torch.empty(sum(sizes), dtype=torch.int32, device=dev).split(sizes)
+    if all(t is None for t in outs):  # one allocation, split
+        outs = torch.split_with_sizes(
+            torch.empty(2 * max_tokens + 2 * S + 2, dtype=torch.int32, device=dev), sizes)
     else:
         names = ("slot_mapping", "positions", "query_start", "context_lens_out", "free_count_out")
         for i, n in enumerate(sizes):
             if outs[i] is None:
                 outs[i] = torch.empty(n, dtype=torch.int32, device=dev)
-            _int_row(names[i], outs[i], n, dev)
+            _check_int(dev, (names[i], outs[i], n))
     slot_mapping, positions, query_start, lens, count = outs
     with _Guard(dev):
         ws = workspace(dev, 256)

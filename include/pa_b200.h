@@ -211,10 +211,12 @@ int pa_decode_f16_noalloc_read_status(int* status_out, void* stream);
 
 /* Decode with bf16 activations: q and out are bf16 [num_seqs, num_heads, head_dim]; the cache
  * is fp16 (kv_dtype PA_DTYPE_F16), per-token int8 (PA_DTYPE_I8) or per-token fp8 e4m3
- * (PA_DTYPE_FP8E4M3), the last two with k_scales/v_scales; splitk selects the split-K pair.
+ * (PA_DTYPE_FP8E4M3), the last two with k_scales/v_scales, or fp4 (PA_DTYPE_FP4E2M1); splitk
+ * selects the split-K pair.
  * q is converted to fp16 on the device (exact for magnitudes in the fp16 normal range; larger
  * values saturate and set PA_ERR_Q_RANGE in the status word), the fp16 decode runs, and its
- * output is rounded once to bf16. The workspace holds the decode workspace followed by the
+ * output is rounded once to bf16 (over an fp4 cache both happen in the decode kernel, and the
+ * fp32 result is rounded to bf16). The workspace holds the decode workspace followed by the
  * fp16 copies: size it with pa_decode_bf16q_workspace_bytes. This is the BF16-q support the
  * reference lists as future work (report/benchmark_report.md:196-197); the reference's own
  * ops take fp16 q only. */
@@ -290,7 +292,7 @@ int pa_quantize_into_cache_fp8(const void* k, const void* v, int in_dtype, int64
                                float* v_scales, int num_blocks, int block_size, int* status,
                                void* stream);
 
-/* FP4 write, same rows and slots; rows and caches 16-byte aligned, block_size a multiple of 16.
+/* FP4 write, same rows and slots; rows and caches 16-byte aligned, block_size 16, 32, 64 or 128.
  * Per 16 head_dim values:
  *   scale = the nearest scale byte's value to amax / 6, ties to even, at most 10240
  *   code  = the nearest e2m1 to x / scale, ties to the even code, magnitudes above 6 as 6
@@ -333,7 +335,8 @@ int pa_qk_norm_rope(void* q_out, int64_t q_out_stride, void* k_out, int64_t k_ou
 /* The same, with the new K rows and the V rows written into the paged cache at slot_mapping instead of
  * k_out: cache_dtype F16, I8 (per-token scales), FP8E4M3 or FP4E2M1, bit for bit what
  * pa_qk_norm_rope followed by that cache's write gives, in one launch. A negative slot writes
- * nothing to the cache (q_out is still written). */
+ * nothing to the cache (q_out is still written). For an fp4 cache rot_dim is a multiple of 32
+ * unless interleaved. */
 int pa_norm_rope_into_cache(void* q_out, int64_t q_out_stride, const void* q, int64_t q_stride,
                             const void* k, int64_t k_stride, const void* v, int64_t v_stride,
                             int dtype, const void* q_weight, const void* k_weight, float eps,
