@@ -345,14 +345,12 @@ int decode_impl(int mode, int kv_i8, void* out, float* part_out, const void* q,
 
   for (int c0 = 0; c0 < B; c0 += s.chunk_b) {
     const int nb = (B - c0) < s.chunk_b ? (B - c0) : s.chunk_b;
-    pa::DecodeArgs a;
+    pa::DecodeFp4Args a;
     memset(&a, 0, sizeof(a));
     a.out = out ? static_cast<__half*>(out) + (size_t)c0 * H * D : nullptr;
     a.q = static_cast<const __half*>(q) + (size_t)c0 * H * D;
     a.block_table = block_table + (size_t)c0 * max_blocks;
     a.context_lens = context_lens + c0;
-    a.k_base = static_cast<const uint8_t*>(k_cache);
-    a.act_bf16 = act_bf16 ? 1 : 0;
     a.v_base = static_cast<const uint8_t*>(v_cache);
     a.ks_base = k_scales;
     a.vs_base = v_scales;
@@ -372,6 +370,11 @@ int decode_impl(int mode, int kv_i8, void* out, float* part_out, const void* q,
     a.mode = mode;
     a.s_max = s.s_max;
     a.bulk = bulk ? 1 : 0;
+    a.k_cache = static_cast<const uint8_t*>(k_cache);
+    a.v_cache = static_cast<const uint8_t*>(v_cache);
+    a.k_write = static_cast<uint8_t*>(const_cast<void*>(k_cache));
+    a.v_write = static_cast<uint8_t*>(const_cast<void*>(v_cache));
+    a.act_bf16 = act_bf16 ? 1 : 0;
     a.qk_scale_log2 = scale * 1.4426950408889634f;
     if (fuse) {
       a.new_k = static_cast<const uint8_t*>(sw->k) + (size_t)c0 * sw->stride * new_es;
@@ -392,7 +395,8 @@ int decode_impl(int mode, int kv_i8, void* out, float* part_out, const void* q,
     if (want < 1) want = 1;
     const int grid = (int)(want < s.sms ? want : s.sms);
     a.total_warps = grid * s.warps_per_cta;
-    cudaError_t e = pa::launch_decode(kv_i8, s.GT, a, maps, grid, st);
+    cudaError_t e = fp4 ? pa::launch_decode_fp4(s.GT, a, grid, st)
+                        : pa::launch_decode(kv_i8, s.GT, a, maps, grid, st);
     if (e != cudaSuccess) return cuda_fail(e, "decode launch");
     if (mode == pa::kModeSplit) {
       pa::ReduceArgs ra;

@@ -34,7 +34,6 @@
 // split merge  m = max m_s,  l = sum l_s e^{m_s - m},  o = sum o_s e^{m_s - m} / l.
 // Scores are kept in log2 units (scale * log2 e) so the exponentials are exp2.
 
-#include "fp4.cuh"
 #include "pa_common.cuh"
 #include "pa_internal.h"
 #include "pa_rows.cuh"
@@ -66,8 +65,7 @@ template <int KVK, int D, int GT, int DEPTH, int WARPS>
 struct Tile {
   static constexpr bool I8 = KVK == 1;    // int8 values, per-token scales
   static constexpr bool F8 = KVK == 2;    // fp8 e4m3 values, per-token scales
-  static constexpr bool F4 = KVK == 3;    // fp4 e2m1 values, a scale per 16 (fp4.cuh)
-  static constexpr bool BYTE = I8 || F8;  // one-byte elements (the INT8 page layout)
+  static constexpr bool BYTE = KVK != 0;  // one-byte elements (the INT8 page layout)
   static constexpr int ELEM = BYTE ? 1 : 2;
   static constexpr int KT = D * kSubTokens * ELEM;  // K tile bytes
   static constexpr int VT = D * kSubTokens * ELEM;  // V tile bytes
@@ -79,25 +77,13 @@ struct Tile {
   static constexpr int MT = D / 16;                 // PV m-tiles (head_dim rows)
   static constexpr int NT = GT / 8;                 // PV n-tiles (heads)
   static constexpr int SLOT = (D + 2) * GT;         // partial slot floats
-  // The page ring: WARPS x DEPTH stages of one 16-token page, or for FP4 of two (K, K, V, V).
-  static constexpr int PT = F4 ? fp4::kGroupBytes : 0;  // FP4 page bytes, K or V
-  static constexpr size_t RING =
-      F4 ? (size_t)WARPS * DEPTH * 4 * PT : (size_t)WARPS * DEPTH * (KT + VT + ST);
-  static constexpr size_t SMEM = 1024 + RING + (size_t)WARPS * DEPTH * 8;
+  static constexpr size_t SMEM = 1024 + (size_t)WARPS * DEPTH * (KT + VT + ST) +
+                                 (size_t)WARPS * DEPTH * 8;
   // Decode step launches: per stage, the new token's K and V rows (16-bit) when the stage's
   // page holds a sequence's new token.
   static constexpr int NR = 2 * D * 2;
-  static constexpr size_t SMEM_STEP = F4 ? SMEM : SMEM + 16 + (size_t)WARPS * DEPTH * NR;
+  static constexpr size_t SMEM_STEP = SMEM + 16 + (size_t)WARPS * DEPTH * NR;
 };
-
-// One output value, as fp16 or bf16.
-__device__ __forceinline__ void store_out(__half* p, float v, bool bf) {
-  if (bf) {
-    *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(v);
-  } else {
-    *p = __float2half_rn(v);
-  }
-}
 
 // ---------------------------------------------------------------------------------------
 // Log-sum-exp merge of `np` partial slots by one warp, from copies of the slots in shared
@@ -108,9 +94,9 @@ __device__ __forceinline__ void store_out(__half* p, float v, bool bf) {
 // 2 (wf + k) + 1 for the first piece (it starts the segment), 2 (wf + k) for the others.
 // Returns false (status flagged) if the copies did not arrive within the wait limit; the
 // caller then stops using the staging memory. Out of line: it runs a few times per CTA at
-// the end of the launch and should not add to the page loop's registers. BF: out rows are bf16.
+// the end of the launch and should not add to the page loop's registers.
 // ---------------------------------------------------------------------------------------
-template <int D, int GT, bool BF = false>
+template <int D, int GT>
 __device__ __noinline__ bool staged_combine(const float* part, int wf, int np, int lane,
                                             int hcnt, __half* out_rows, float* out_slot,
                                             int* status, float* stage, uint64_t* bar,
@@ -175,7 +161,7 @@ __device__ __noinline__ bool staged_combine(const float* part, int wf, int np, i
       const float a4[4] = {acc[i].x, acc[i].y, acc[i].z, acc[i].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (h0 + e < hcnt) store_out(out_rows + (size_t)(h0 + e) * D + d, a4[e] * inv[e], BF);
+        if (h0 + e < hcnt) out_rows[(size_t)(h0 + e) * D + d] = __float2half_rn(a4[e] * inv[e]);
     }
   } else {
 #pragma unroll
@@ -207,7 +193,7 @@ struct Coop {
   }
 };
 
-template <int D, int GT, int NTHR, int U, bool BF = false, typename PieceFn>
+template <int D, int GT, int NTHR, int U, typename PieceFn>
 __device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __half* out_rows,
                                              float* out_slot, int* status, float* sm) {
   using CC = Coop<D, GT, NTHR, U>;
@@ -339,7 +325,7 @@ __device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __
           const int h = h0 + e;
           if (h < hcnt) {
             const float L = sL[h];
-            store_out(out_rows + (size_t)h * D + d, L > 0.f ? a4[e] / L : 0.f, BF);
+            out_rows[(size_t)h * D + d] = __float2half_rn(L > 0.f ? a4[e] / L : 0.f);
           }
         }
       } else {
@@ -411,36 +397,6 @@ __device__ __noinline__ void stage_new_token(const uint8_t* rk, uint8_t* kt, uin
 }
 
 // ---------------------------------------------------------------------------------------
-// Decode step over a 4-bit cache: one warp quantises the new token's K and V rows (16-bit, at
-// src_k / src_v) and stores them into the cache, at token `off` of page row `row`, before it
-// loads the page. Only the calling warp reads the page.
-// ---------------------------------------------------------------------------------------
-template <int D>
-__device__ __noinline__ void store_new_token_fp4(const uint8_t* src_k, const uint8_t* src_v,
-                                                 int new_dtype, uint8_t* kc, uint8_t* vc,
-                                                 size_t row, int off, int bs, int lane) {
-  static_assert(D == 128, "one lane per four head_dim values");
-  const size_t grp = fp4::group_offset(row, off, bs);
-  const int t = off % fp4::kGroupTokens;
-#pragma unroll
-  for (int which = 0; which < 2; ++which) {
-    const uint8_t* src = which ? src_v : src_k;
-    float x[4];
-    if (new_dtype == PA_DTYPE_BF16) {
-      load_vals<__nv_bfloat16, 4>(reinterpret_cast<const __nv_bfloat16*>(src) + 4 * lane, x);
-    } else {
-      load_vals<__half, 4>(reinterpret_cast<const __half*>(src) + 4 * lane, x);
-    }
-    uint32_t sb;
-    const uint32_t w = fp4::warp_quantize4<false>(x, sb);
-    uint8_t* dst = (which ? vc : kc) + grp;
-    *reinterpret_cast<uint16_t*>(dst + t * fp4::kCodeRow + 2 * lane) = (uint16_t)w;
-    if ((lane & 3) == 0) dst[fp4::scale_offset(which != 0, t, lane >> 2)] = (uint8_t)sb;
-  }
-  __syncwarp();
-}
-
-// ---------------------------------------------------------------------------------------
 // The decode kernel.
 // ---------------------------------------------------------------------------------------
 template <int KVK, int D, int GT, int DEPTH, int WARPS>
@@ -452,7 +408,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   using C = Tile<KVK, D, GT, DEPTH, WARPS>;
   constexpr bool I8 = C::I8;
   constexpr bool F8 = C::F8;
-  constexpr bool F4 = C::F4;
   constexpr bool BYTE = C::BYTE;
   constexpr int NS = C::NS;
   constexpr int MT = C::MT;
@@ -478,7 +433,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   uint8_t* k_tiles = dsm;
   uint8_t* v_tiles = k_tiles + WARPS * DEPTH * C::KT;
   uint8_t* s_tiles = v_tiles + WARPS * DEPTH * C::VT;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(dsm + C::RING);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_tiles + WARPS * DEPTH * C::ST);
   // New-token rows of a decode step (allocated only for step launches).
   uint8_t* r_tiles = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(bars + WARPS * DEPTH) + 15) & ~uintptr_t(15));
@@ -507,8 +462,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       prefetch_l2_share(a.new_k, nb, blockIdx.x, gridDim.x);
       prefetch_l2_share(a.new_v, nb, blockIdx.x, gridDim.x);
     }
-    if constexpr (!F4) prefetch_tensormap(&tm_k);
-    if (!F4 && !a.bulk) {
+    prefetch_tensormap(&tm_k);
+    if (!a.bulk) {
       prefetch_tensormap(&tm_v);
       if constexpr (BYTE) {
         prefetch_tensormap(&tm_ks);
@@ -659,28 +614,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   float qks0 = qs, qks1 = qs;
   int q_b = -1, q_seg = -1;
 
-  // FP4 with bf16 activations: eight bf16 values as fp16 (exact inside the fp16 normal range;
-  // larger magnitudes saturate and are flagged, as by pa_decode_bf16q's conversion kernel).
-  [[maybe_unused]] auto bf16_to_f16 = [&](uint4 v) {
-    const uint32_t src[4] = {v.x, v.y, v.z, v.w};
-    uint32_t dst[4];
-    bool bad = false;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float lo = __uint_as_float(src[e] << 16), hi = __uint_as_float(src[e] & 0xffff0000u);
-      if (fabsf(lo) > 65504.f) {
-        bad = true;
-        lo = copysignf(65504.f, lo);
-      }
-      if (fabsf(hi) > 65504.f) {
-        bad = true;
-        hi = copysignf(65504.f, hi);
-      }
-      dst[e] = pack_f16x2(lo, hi);
-    }
-    if (bad) flag_error(a.status, PA_ERR_Q_RANGE);
-    return make_uint4(dst[0], dst[1], dst[2], dst[3]);
-  };
   auto fetch_q = [&](int b, int seg) {
     const int kvh = seg / a.HT;
     const int ht = seg - kvh * a.HT;
@@ -688,7 +621,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     const __half* qrow = a.q + ((size_t)b * a.H + (size_t)kvh * a.G + hl) * D;
 #pragma unroll
     for (int si = 0; si < NS; ++si) {
-      const int c = F4 ? 4 * r + si : (BYTE ? chunk_i8(r, si) : chunk_f16(r, si));
+      const int c = BYTE ? chunk_i8(r, si) : chunk_f16(r, si);
       ra[si] = (hl < a.G) ? __ldg(reinterpret_cast<const uint4*>(qrow + 8 * c))
                           : make_uint4(0u, 0u, 0u, 0u);
       if constexpr (GT == 16) {
@@ -771,12 +704,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       for (int si = 0; si < NS; ++si) {
         qa[si] = ra[si];
         qb[si] = rb[si];
-        if constexpr (F4) {
-          if (a.act_bf16) {
-            qa[si] = bf16_to_f16(ra[si]);
-            if constexpr (NT == 2) qb[si] = bf16_to_f16(rb[si]);
-          }
-        }
       }
     }
   };
@@ -814,8 +741,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       blk = 0;
       wr = -1;
     }
-    if constexpr (F4)  // index of the 16-token group (below 2^31)
-      return (blk * a.KVH + (meta >> 3)) * a.subs + (meta & 7);
     return ((blk * a.KVH + (meta >> 3)) << 3) | (meta & 7);
   };
   // The block ids of the next 32 pages are copied into shared memory in the background
@@ -840,72 +765,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   int curw, meta0;
   const int* bref0 = page_ref(0, meta0, curw);
   const int blk0 = bref0 != nullptr ? __ldg(bref0) : 0;
-  if constexpr (!F4) prefetch_batch(32);  // requested before the first batch's ids are waited for
+  prefetch_batch(32);  // requested before the first batch's ids are waited for
   int cur = pack_page(blk0, meta0, curw);
-
-  // FP4, decode step: the new token in the page of group gi, if it holds one (sequence wb >= 0),
-  // is written into the cache before the page is copied.
-  auto write_new = [&](uint32_t gi, int wb) {
-    if (wb < 0) return;
-    const uint32_t row = gi / (uint32_t)a.subs;
-    const size_t so = ((size_t)wb * a.new_stride + (size_t)(row % (uint32_t)a.KVH) * D) * 2;
-    store_new_token_fp4<D>(static_cast<const uint8_t*>(a.new_k) + so,
-                           static_cast<const uint8_t*>(a.new_v) + so, a.new_dtype,
-                           static_cast<uint8_t*>(a.kc_w), static_cast<uint8_t*>(a.vc_w), row,
-                           (s_ctx[wb] - 1) % a.bs, a.bs, lane);
-    __threadfence();  // the copies read what the warp has just written, from L2
-  };
-  // FP4: the warp's ring is filled by 16-byte asynchronous copies of all its lanes, one commit
-  // group per stage of two pages. (Four bulk copies per stage, issued by one lane, cost 87 of the
-  // step's 640 instructions; nine copies a lane and their addresses cost about 25.) A page's K
-  // and V groups are 72 chunks each: two rounds of the warp, and the last eight chunks of all
-  // four groups in one more round.
-  [[maybe_unused]] const uint32_t f4base =
-      smem_u32(k_tiles) + (uint32_t)(warp * DEPTH) * 4u * (uint32_t)C::PT;
-  [[maybe_unused]] const uint8_t* k_lane = a.k_base + 16 * lane;
-  [[maybe_unused]] const uint8_t* v_lane = a.v_base + 16 * lane;
-  [[maybe_unused]] const uint8_t* rest_lane =
-      ((lane & 16) ? a.v_base : a.k_base) + 1024 + 16 * (lane & 7);
-  [[maybe_unused]] const uint32_t rest_off =
-      (uint32_t)(lane >> 3) * (uint32_t)C::PT + 1024u + 16u * (uint32_t)(lane & 7);
-  // Pages jj and jj + 1 (jj even; asked for in order) into stage s; past the range's end the
-  // group is empty, and a missing second page is the first once more. The ids of the next 32
-  // pages come along with a batch's first stage, sixteen groups before they are needed.
-  auto issue_pair = [&](int jj, int s) {
-    if (jj < n) {
-      if ((jj & 31) == 0) {
-        if (jj > 0) {
-          curw = s_nwr[warp][lane];
-          cur = pack_page(s_nblk[warp][lane], s_nmeta[warp][lane], curw);
-        }
-        int meta, wr;
-        const int* p = page_ref(jj + 32, meta, wr);
-        s_nmeta[warp][lane] = meta;
-        s_nwr[warp][lane] = wr;
-        if (p != nullptr) cp_async_4(&s_nblk[warp][lane], p);
-      }
-      const int i1 = (jj & 31) + (jj + 1 < n ? 1 : 0);
-      const uint32_t g0 = __shfl_sync(0xffffffffu, (uint32_t)cur, jj & 31);
-      const uint32_t g1 = __shfl_sync(0xffffffffu, (uint32_t)cur, i1);
-      if (step_write) {
-        write_new(g0, __shfl_sync(0xffffffffu, curw, jj & 31));
-        write_new(g1, __shfl_sync(0xffffffffu, curw, i1));
-      }
-      const uint32_t st = f4base + (uint32_t)s * 4u * (uint32_t)C::PT + 16u * (uint32_t)lane;
-      const size_t o0 = (size_t)g0 * C::PT, o1 = (size_t)g1 * C::PT;
-      cp_async_16_hint(st, k_lane + o0, pol);
-      cp_async_16_hint(st + 512, k_lane + o0 + 512, pol);
-      cp_async_16_hint(st + C::PT, k_lane + o1, pol);
-      cp_async_16_hint(st + C::PT + 512, k_lane + o1 + 512, pol);
-      cp_async_16_hint(st + 2 * C::PT, v_lane + o0, pol);
-      cp_async_16_hint(st + 2 * C::PT + 512, v_lane + o0 + 512, pol);
-      cp_async_16_hint(st + 3 * C::PT, v_lane + o1, pol);
-      cp_async_16_hint(st + 3 * C::PT + 512, v_lane + o1 + 512, pol);
-      cp_async_16_hint(st - 16u * (uint32_t)lane + rest_off,
-                       rest_lane + (size_t)((lane & 8) ? g1 : g0) * C::PT, pol);
-    }
-    cp_async_commit();
-  };
 
   auto issue = [&](int j, int s) {
     if (j > 0 && (j & 31) == 0) {
@@ -960,13 +821,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   static_assert(DEPTH < 32, "the prologue copies must come from the first batch of block ids");
   const int npro = n < DEPTH ? n : DEPTH;
   __syncwarp();
+  for (int j = 0; j < npro; ++j) issue(j, j);
   int issued = npro;
-  if constexpr (F4) {
-    issued = 0;
-    for (int j = 0; j < DEPTH; ++j) issue_pair(2 * j, j);
-  } else {
-    for (int j = 0; j < npro; ++j) issue(j, j);
-  }
   convert_q();
 
   // Shared-memory offsets of the K cells this lane reads (chunk of load si, token of n-tile
@@ -1004,12 +860,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 
   float m0 = neg_inf(), l0 = 0.f, m1 = neg_inf(), l1 = 0.f;
   float oacc[MT][NT][4];
-  // head_dim of O's row g (hi = 0) and g + 8 (hi = 1) of m-tile i.
-  auto drow = [&](int i, int hi) { return F4 ? 16 * g + 2 * i + hi : 16 * i + g + 8 * hi; };
 
-  // FP4: running maximum and sum of heads nt * 8 + 2r and the next.
-  [[maybe_unused]] float fm[NT][2], fl[NT][2], fmb[NT][2];  // fmb = kPExp - fm
-  [[maybe_unused]] const int tau = 4 * (g >> 1) + (g & 1);  // token of K row g (row g + 8: + 2)
   int jfail = -1;
   int s = 0;        // ring stage of page j
   uint32_t ph = 0;  // its mbarrier phase parity
@@ -1052,204 +903,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) oacc[i][nt][e] = 0.f;
 
-    if constexpr (F4) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          fm[nt][e] = neg_inf();
-          fmb[nt][e] = -neg_inf();
-          fl[nt][e] = 0.f;
-        }
-      // A stage's two pages per step; where a piece begins or ends inside a stage, the page that
-      // is not its own is masked (and met again by the other piece).
-      for (int k = 0; k < len;) {
-        const int first = j & 1;
-        const int cnt = min(2 - first, len - k);
-        if (first == 0) {  // the stage's copies: this lane's, then every lane's
-          cp_async_wait_groups<DEPTH - 1>();
-          __syncwarp();
-        }
-        const int left = cctx - (csp + k) * kSubTokens;  // tokens from the step's first page on
-        const int valid0 = first ? 0 : min(kSubTokens, left);
-        const int valid1 = first ? min(kSubTokens, left)
-                                 : (cnt == 2 ? min(kSubTokens, left - kSubTokens) : 0);
-        const bool full = valid0 == kSubTokens && valid1 == kSubTokens;
-        const uint32_t st = f4base + (uint32_t)s * 4u * (uint32_t)C::PT;
-        const uint32_t ka = st + tau * fp4::kCodeRow + 16 * r;
-        const uint32_t ksa = st + fp4::kCodes + tau * 8 + 2 * r;
-        const uint32_t va = st + 2 * C::PT + 4 * r * fp4::kCodeRow + 8 * g;
-        const uint32_t vsa = st + 2 * C::PT + fp4::kCodes + 16 * g + 4 * r;
-
-        // S^T = K Q^T: rows = tokens (row g: token tau, row g + 8: tau + 2), columns = heads, so
-        // that eight heads fill the MMA. A lane reads the 32 codes 32r .. 32r + 31 of its two
-        // tokens; codes -> fp16, times the block scale, is exact (fp4.cuh).
-        float x[2][NT][4];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const uint4 c0 = lds128(ka + u * C::PT), c1 = lds128(ka + u * C::PT + 2 * fp4::kCodeRow);
-          const uint32_t z0 = lds16(ksa + u * C::PT), z1 = lds16(ksa + u * C::PT + 16);
-          const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
-          const uint32_t s0 = fp4::scale_pair(z0), s1 = fp4::scale_pair(z1);
-          float acc[2][NT][4];  // even and odd steps: two shorter chains
-          auto mma = [](bool begin, float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                        uint32_t a3, uint32_t b0, uint32_t b1) {
-            if (begin) mma_16816_zero(d, a0, a1, a2, a3, b0, b1);
-            else mma_16816(d, a0, a1, a2, a3, b0, b1);
-          };
-#pragma unroll
-          for (int si = 0; si < NS; ++si) {
-            uint32_t h[4], i4[4];
-            fp4::codes_to_f16x2(w0[si], h[0], h[1], h[2], h[3]);
-            fp4::codes_to_f16x2(w1[si], i4[0], i4[1], i4[2], i4[3]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              h[e] = si < NS / 2 ? fp4::hmul2_half<false>(h[e], s0)
-                                 : fp4::hmul2_half<true>(h[e], s0);
-              i4[e] = si < NS / 2 ? fp4::hmul2_half<false>(i4[e], s1)
-                                  : fp4::hmul2_half<true>(i4[e], s1);
-            }
-            mma(si == 0, acc[0][0], h[0], i4[0], h[1], i4[1], qa[si].x, qa[si].y);
-            mma(si == 0, acc[1][0], h[2], i4[2], h[3], i4[3], qa[si].z, qa[si].w);
-            if constexpr (NT == 2) {
-              mma(si == 0, acc[0][1], h[0], i4[0], h[1], i4[1], qb[si].x, qb[si].y);
-              mma(si == 0, acc[1][1], h[2], i4[2], h[3], i4[3], qb[si].z, qb[si].w);
-            }
-          }
-          // Logits in log2 units: heads nt * 8 + 2r + (e & 1) of token tau (e < 2) and tau + 2.
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-              const float2 v = mul2(add2(make_float2(acc[0][nt][e], acc[0][nt][e + 1]),
-                                         make_float2(acc[1][nt][e], acc[1][nt][e + 1])),
-                                    make_float2(qs, qs));
-              x[u][nt][e] = v.x;
-              x[u][nt][e + 1] = v.y;
-            }
-        }
-        if (!full) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int vd = u ? valid1 : valid0;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (tau + (e & 2) >= vd) x[u][nt][e] = neg_inf();
-          }
-        }
-        // The reference maximum moves only when a score passes it by 2^kLazy: weights then stay
-        // below 2^(kPExp + kLazy) (far inside fp16), O and l carry the same factor, and most
-        // steps need neither a reduction over the lanes nor a rescale.
-        constexpr float kLazy = 8.f;
-        float tm[NT][2];
-        bool up = false;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            tm[nt][e] = fmaxf(fmaxf(x[0][nt][e], x[0][nt][2 + e]),
-                              fmaxf(x[1][nt][e], x[1][nt][2 + e]));
-            up = up || tm[nt][e] > fm[nt][e] + kLazy;
-          }
-        if (__any_sync(0xffffffffu, up)) {
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float c[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float v = tm[nt][e];
-#pragma unroll
-              for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-              c[e] = v > fm[nt][e] ? ex2(fm[nt][e] - v) : 1.f;
-              fm[nt][e] = fmaxf(v, fm[nt][e]);
-              fmb[nt][e] = kPExp - fm[nt][e];
-              fl[nt][e] *= c[e];
-            }
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {  // O's columns are the lane's own heads
-              oacc[i][nt][0] *= c[0];
-              oacc[i][nt][1] *= c[1];
-              oacc[i][nt][2] *= c[0];
-              oacc[i][nt][3] *= c[1];
-            }
-          }
-        }
-
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          // Weights, as two fp16 parts each (about 22 significant bits, as for the other
-          // caches); the transposed 8 x 8 tiles are the PV MMA's B fragments.
-          uint32_t ph0[NT], ph1[NT], pl0[NT], pl1[NT];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float p[4];
-#pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-              const float2 v = add2(make_float2(x[u][nt][e], x[u][nt][e + 1]),
-                                    make_float2(fmb[nt][0], fmb[nt][1]));
-              p[e] = ex2(v.x);
-              p[e + 1] = ex2(v.y);
-              const float2 l = add2(make_float2(fl[nt][0], fl[nt][1]),
-                                    make_float2(p[e], p[e + 1]));
-              fl[nt][0] = l.x;
-              fl[nt][1] = l.y;
-            }
-            split_f16x2_packed(p[0], p[1], ph0[nt], pl0[nt]);
-            split_f16x2_packed(p[2], p[3], ph1[nt], pl1[nt]);
-            ph0[nt] = transpose8x8(ph0[nt]);
-            ph1[nt] = transpose8x8(ph1[nt]);
-            pl0[nt] = transpose8x8(pl0[nt]);
-            pl1[nt] = transpose8x8(pl1[nt]);
-          }
-          // V: tokens 4r .. 4r + 3, values 16g .. 16g + 15 (one block a token). Scales of slots
-          // past the context may be anything: zero there (a finite code times zero is 0).
-          uint2 vq[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) vq[e] = lds64(va + u * C::PT + e * fp4::kCodeRow);
-          const uint32_t z = lds32(vsa + u * C::PT);
-          uint32_t s01 = fp4::scale_pair(z), s23 = fp4::scale_pair(z, 0x3424u);
-          if (!full) {
-            const int vd = u ? valid1 : valid0;
-            s01 &= ((4 * r < vd) ? 0x0000ffffu : 0u) | ((4 * r + 1 < vd) ? 0xffff0000u : 0u);
-            s23 &= ((4 * r + 2 < vd) ? 0x0000ffffu : 0u) | ((4 * r + 3 < vd) ? 0xffff0000u : 0u);
-          }
-          // O^T += V^T P^T. The MMA pairs tokens: the even and the odd head_dim codes of two
-          // tokens share a byte before they convert. Rows g and g + 8 of m-tile 4h + jj are
-          // head_dim 16g + 8h + 2jj and the next.
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t w0 = h ? vq[0].y : vq[0].x, w1 = h ? vq[1].y : vq[1].x;
-            const uint32_t w2 = h ? vq[2].y : vq[2].x, w3 = h ? vq[3].y : vq[3].x;
-            constexpr uint32_t kLow = 0x0f0f0f0fu;
-            uint32_t A0[4], A1[4], A2[4], A3[4];
-            fp4::codes_to_f16x2((w0 & kLow) | ((w1 << 4) & ~kLow), A0[0], A0[1], A0[2], A0[3]);
-            fp4::codes_to_f16x2(((w0 >> 4) & kLow) | (w1 & ~kLow), A1[0], A1[1], A1[2], A1[3]);
-            fp4::codes_to_f16x2((w2 & kLow) | ((w3 << 4) & ~kLow), A2[0], A2[1], A2[2], A2[3]);
-            fp4::codes_to_f16x2(((w2 >> 4) & kLow) | (w3 & ~kLow), A3[0], A3[1], A3[2], A3[3]);
-#pragma unroll
-            for (int jj = 0; jj < 4; ++jj) {
-              const int i = 4 * h + jj;
-              const uint32_t a0 = fp4::hmul2(A0[jj], s01), a1 = fp4::hmul2(A1[jj], s01);
-              const uint32_t a2 = fp4::hmul2(A2[jj], s23), a3 = fp4::hmul2(A3[jj], s23);
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma_16816(oacc[i][nt], a0, a1, a2, a3, ph0[nt], ph1[nt]);
-                mma_16816(oacc[i][nt], a0, a1, a2, a3, pl0[nt], pl1[nt]);
-              }
-            }
-          }
-        }
-        k += cnt;
-        j += cnt;
-        if ((j & 1) == 0) {  // both pages of the stage are done with: refill it
-          __syncwarp();
-          issue_pair(j + 2 * DEPTH - 2, s);
-          if (++s == DEPTH) s = 0;
-        }
-      }
-    } else {
     for (int k = 0; k < len; ++k) {
     if (!mbar_wait_bounded(&wbar[s], ph, a.status)) {
       jfail = j;
@@ -1563,21 +1216,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       ph ^= 1u;
     }
     }  // pages of the piece
-    }
     if (jfail >= 0) break;
     csp += len;
 
     {
       // ---- piece epilogue ---------------------------------------------------------------------
-      if constexpr (F4) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1)
-              fl[nt][e] += __shfl_xor_sync(0xffffffffu, fl[nt][e], o);
-      }
       float lt0 = l0 + __shfl_xor_sync(0xffffffffu, l0, 1);
       lt0 += __shfl_xor_sync(0xffffffffu, lt0, 2);
       float lt1 = 0.f;
@@ -1598,23 +1241,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         for (int i = 0; i < MT; ++i) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            *reinterpret_cast<float2*>(slot + drow(i, 0) * GT + nt * 8 + 2 * r) =
+            *reinterpret_cast<float2*>(slot + (16 * i + g) * GT + nt * 8 + 2 * r) =
                 make_float2(oacc[i][nt][0] * kUnscale, oacc[i][nt][1] * kUnscale);
-            *reinterpret_cast<float2*>(slot + drow(i, 1) * GT + nt * 8 + 2 * r) =
+            *reinterpret_cast<float2*>(slot + (16 * i + g + 8) * GT + nt * 8 + 2 * r) =
                 make_float2(oacc[i][nt][2] * kUnscale, oacc[i][nt][3] * kUnscale);
           }
         }
-        if constexpr (F4) {
-          if (g == 0) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              *reinterpret_cast<float2*>(slot + D * GT + nt * 8 + 2 * r) =
-                  make_float2(fm[nt][0], fm[nt][1]);
-              *reinterpret_cast<float2*>(slot + D * GT + GT + nt * 8 + 2 * r) =
-                  make_float2(fl[nt][0] * kUnscale, fl[nt][1] * kUnscale);
-            }
-          }
-        } else if (r == 0) {
+        if (r == 0) {
           slot[D * GT + g] = m0;
           slot[D * GT + GT + g] = lt0 * kUnscale;
           if constexpr (NT == 2) {
@@ -1629,63 +1262,30 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       } else if (piece_sp0 == 0 && csp == cpg) {
         // The whole segment was this warp's: normalise and store directly.
         if (a.mode == kModeStream) {
-          float ia, ib, ic = 0.f, id = 0.f;
-          if constexpr (F4) {
-            ia = 1.f / fl[0][0];
-            ib = 1.f / fl[0][1];
-            ic = 1.f / fl[NT - 1][0];
-            id = 1.f / fl[NT - 1][1];
-          } else {
-            const float inv0 = 1.f / lt0;
-            ia = __shfl_sync(0xffffffffu, inv0, 8 * r);
-            ib = __shfl_sync(0xffffffffu, inv0, 8 * r + 4);
-          }
-          if constexpr (NT == 2 && !F4) {
+          const float inv0 = 1.f / lt0;
+          const float ia = __shfl_sync(0xffffffffu, inv0, 8 * r);
+          const float ib = __shfl_sync(0xffffffffu, inv0, 8 * r + 4);
+          float ic = 0.f, id = 0.f;
+          if constexpr (NT == 2) {
             const float inv1 = 1.f / lt1;
             ic = __shfl_sync(0xffffffffu, inv1, 8 * r);
             id = __shfl_sync(0xffffffffu, inv1, 8 * r + 4);
           }
           __half* ob = a.out + ((size_t)cb * a.H + hbase) * D;
-          if constexpr (F4) {
-            // A lane holds values 16g .. 16g + 15 of its heads: 32 contiguous bytes each.
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int h = nt * 8 + 2 * r + e;
-                const float f = nt ? (e ? id : ic) : (e ? ib : ia);
-                uint32_t w[MT];
-#pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                  const float lo = oacc[i][nt][e] * f, hi = oacc[i][nt][2 + e] * f;
-                  if (a.act_bf16) {
-                    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-                    w[i] = *reinterpret_cast<const uint32_t*>(&v);
-                  } else {
-                    w[i] = pack_f16x2(lo, hi);
-                  }
-                }
-                if (h < hcnt) {
-                  uint4* o = reinterpret_cast<uint4*>(ob + (size_t)h * D + 16 * g);
-                  o[0] = make_uint4(w[0], w[1], w[2], w[3]);
-                  o[1] = make_uint4(w[4], w[5], w[6], w[7]);
-                }
-              }
-          }
-#pragma unroll
-          for (int i = 0; i < (F4 ? 0 : MT); ++i) {
+          for (int i = 0; i < MT; ++i) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               const int h = nt * 8 + 2 * r;
               const float fa = nt ? ic : ia;
               const float fb = nt ? id : ib;
               if (h < hcnt) {
-                ob[(size_t)h * D + drow(i, 0)] = __float2half_rn(oacc[i][nt][0] * fa);
-                ob[(size_t)h * D + drow(i, 1)] = __float2half_rn(oacc[i][nt][2] * fa);
+                ob[(size_t)h * D + 16 * i + g] = __float2half_rn(oacc[i][nt][0] * fa);
+                ob[(size_t)h * D + 16 * i + g + 8] = __float2half_rn(oacc[i][nt][2] * fa);
               }
               if (h + 1 < hcnt) {
-                ob[(size_t)(h + 1) * D + drow(i, 0)] = __float2half_rn(oacc[i][nt][1] * fb);
-                ob[(size_t)(h + 1) * D + drow(i, 1)] = __float2half_rn(oacc[i][nt][3] * fb);
+                ob[(size_t)(h + 1) * D + 16 * i + g] = __float2half_rn(oacc[i][nt][1] * fb);
+                ob[(size_t)(h + 1) * D + 16 * i + g + 8] = __float2half_rn(oacc[i][nt][3] * fb);
               }
             }
           }
@@ -1738,7 +1338,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     }
   }
 
-  if constexpr (F4) cp_async_wait_all();
   if (jfail >= 0) {
     // Let copies still in flight land before the CTA's shared memory is released.
     for (int jj = jfail; jj < issued; ++jj) {
@@ -1769,7 +1368,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     s_npend[warp] = k;
   }
   __syncthreads();  // every warp is past its page loop: the ring memory is free
-  constexpr size_t kRing = C::RING;
+  constexpr size_t kRing = (size_t)WARPS * DEPTH * (C::KT + C::VT + C::ST);
   constexpr int kStageCap = (int)(kRing / (SLOT * sizeof(float)));
   float* scratch = reinterpret_cast<float*>(k_tiles);
   const bool stream = (a.mode == kModeStream);
@@ -1791,16 +1390,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       }
       if (inwave == warp) {
         const int segid = pe[0], wf = pe[1], b = pe[3], hbase = pe[4], hcnt = pe[5];
-        __half* orow = stream ? a.out + ((size_t)b * a.H + hbase) * D : nullptr;
-        float* oslot = stream ? nullptr : a.part_out + (size_t)segid * SLOT;
-        float* stg = scratch + (size_t)used * SLOT;
-        const bool done =
-            F4 && a.act_bf16
-                ? staged_combine<D, GT, F4>(a.part, wf, np, lane, hcnt, orow, oslot, a.status, stg,
-                                            &s_mmb[warp], mph)
-                : staged_combine<D, GT>(a.part, wf, np, lane, hcnt, orow, oslot, a.status, stg,
-                                        &s_mmb[warp], mph);
-        if (!done) {
+        if (!staged_combine<D, GT>(a.part, wf, np, lane, hcnt,
+                                   stream ? a.out + ((size_t)b * a.H + hbase) * D : nullptr,
+                                   stream ? nullptr : a.part_out + (size_t)segid * SLOT,
+                                   a.status, scratch + (size_t)used * SLOT, &s_mmb[warp], mph)) {
           // Timed out: let the copies land before the memory is used again.
           (void)mbar_wait_bounded(&s_mmb[warp], mph, nullptr);
         }
@@ -1828,11 +1421,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       auto piece = [&](int k) -> const float* {
         return a.part + ((size_t)(wf + k) * 2 + (k == 0 ? 1 : 0)) * SLOT;
       };
-      if (F4 && stream && a.act_bf16) {
-        coop_combine<D, GT, NTHR, 8, F4>(piece, np, hcnt,
-                                         a.out + ((size_t)b * a.H + hbase) * D, nullptr,
-                                         a.status, scratch);
-      } else if (stream) {
+      if (stream) {
         coop_combine<D, GT, NTHR, 8>(piece, np, hcnt, a.out + ((size_t)b * a.H + hbase) * D,
                                      nullptr, a.status, scratch);
       } else {
@@ -1850,7 +1439,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 // ---------------------------------------------------------------------------------------
 constexpr int kReduceThreads = 512;
 
-template <int D, int GT, bool BF>
+template <int D, int GT>
 __global__ void __launch_bounds__(kReduceThreads, 1) reduce_kernel(const ReduceArgs a) {
   extern __shared__ __align__(16) float rsm[];
   const int SEGS = a.KVH * a.HT;
@@ -1876,7 +1465,7 @@ __global__ void __launch_bounds__(kReduceThreads, 1) reduce_kernel(const ReduceA
     return;
   }
   const float* base = a.part + (size_t)segid * a.seg_stride;
-  coop_combine<D, GT, kReduceThreads, 16, BF>(
+  coop_combine<D, GT, kReduceThreads, 16>(
       [&](int k) { return base + (size_t)k * a.piece_stride; }, np, hcnt, orow, nullptr,
       a.status, rsm);
 }
@@ -1903,14 +1492,6 @@ template <> struct Shape<1, 16> { static constexpr int W = 8, DP = 4; };
 template <> struct Shape<0, 16> { static constexpr int W = 8, DP = 3; };
 template <> struct Shape<2, 8> { static constexpr int W = 12, DP = 3; };
 template <> struct Shape<2, 16> { static constexpr int W = 8, DP = 4; };
-#ifndef PA_F4_WARPS
-#define PA_F4_WARPS 12
-#endif
-#ifndef PA_F4_DEPTH
-#define PA_F4_DEPTH 3
-#endif
-template <> struct Shape<3, 8> { static constexpr int W = PA_F4_WARPS, DP = PA_F4_DEPTH; };
-template <> struct Shape<3, 16> { static constexpr int W = 8, DP = 4; };
 
 template <int KVK, int GT>
 cudaError_t launch_one(const DecodeArgs& a, const CUtensorMap* maps, int grid,
@@ -1941,7 +1522,7 @@ cudaError_t launch_one(const DecodeArgs& a, const CUtensorMap* maps, int grid,
 }  // namespace
 
 int decode_warps_per_cta(int kv_i8, int gt) {
-  if (kv_i8 == 3) return gt == 8 ? Shape<3, 8>::W : Shape<3, 16>::W;
+  if (kv_i8 == 3) return decode_fp4_warps_per_cta(gt);
   if (kv_i8 == 2) return gt == 8 ? Shape<2, 8>::W : Shape<2, 16>::W;
   if (kv_i8) return gt == 8 ? Shape<1, 8>::W : Shape<1, 16>::W;
   return gt == 8 ? Shape<0, 8>::W : Shape<0, 16>::W;
@@ -1949,10 +1530,6 @@ int decode_warps_per_cta(int kv_i8, int gt) {
 
 cudaError_t launch_decode(int kv_i8, int gt, const DecodeArgs& a, const CUtensorMap* maps,
                           int grid, cudaStream_t stream) {
-  if (kv_i8 == 3) {
-    return gt == 8 ? launch_one<3, 8>(a, maps, grid, stream)
-                   : launch_one<3, 16>(a, maps, grid, stream);
-  }
   if (kv_i8 == 2) {
     return gt == 8 ? launch_one<2, 8>(a, maps, grid, stream)
                    : launch_one<2, 16>(a, maps, grid, stream);
@@ -1986,25 +1563,24 @@ cudaError_t launch_selftest_wait(int* status, cudaStream_t st) {
 cudaError_t launch_reduce(int gt, const ReduceArgs& a, int max_pieces, cudaStream_t stream) {
   const int segs = a.B * a.KVH * a.HT;
   if (segs == 0) return cudaSuccess;
+  if (a.bf16) return launch_reduce_bf16(gt, a, max_pieces, stream);
   size_t smem;
   cudaError_t e;
   if (Coop<128, 16, kReduceThreads, 16>::floats(max_pieces) * sizeof(float) > 200 * 1024)
     return cudaErrorInvalidValue;  // more splits than one CTA can merge (contexts > ~3M tokens)
-  auto launch = [&](auto kern, size_t floats) {
-    smem = floats * sizeof(float);
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) kern<<<segs, kReduceThreads, smem, stream>>>(a);
-  };
-  const size_t f8 = Coop<128, 8, kReduceThreads, 16>::floats(max_pieces);
-  const size_t f16 = Coop<128, 16, kReduceThreads, 16>::floats(max_pieces);
   if (gt == 8) {
-    if (a.bf16) launch(reduce_kernel<128, 8, true>, f8);
-    else launch(reduce_kernel<128, 8, false>, f8);
+    smem = Coop<128, 8, kReduceThreads, 16>::floats(max_pieces) * sizeof(float);
+    e = cudaFuncSetAttribute(reduce_kernel<128, 8>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)smem);
+    if (e != cudaSuccess) return e;
+    reduce_kernel<128, 8><<<segs, kReduceThreads, smem, stream>>>(a);
   } else {
-    if (a.bf16) launch(reduce_kernel<128, 16, true>, f16);
-    else launch(reduce_kernel<128, 16, false>, f16);
+    smem = Coop<128, 16, kReduceThreads, 16>::floats(max_pieces) * sizeof(float);
+    e = cudaFuncSetAttribute(reduce_kernel<128, 16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)smem);
+    if (e != cudaSuccess) return e;
+    reduce_kernel<128, 16><<<segs, kReduceThreads, smem, stream>>>(a);
   }
-  if (e != cudaSuccess) return e;
   return cudaGetLastError();
 }
 

@@ -1,0 +1,1228 @@
+// Paged-attention decode over the 4-bit K/V cache (format and layout: fp4.cuh).
+//
+// The work is cut and the partials are merged as in decode.cu (one warp per equal range of 16-token
+// pages of the flattened sequence x kv head x head tile x page list; a segment cut between warps
+// leaves partials that the last arrival merges, in piece order, so results do not depend on
+// timing). The page loop is its own, because at 144 bytes a token and kv head it is bound by
+// what the four schedulers of an SM can issue, not by memory:
+//  * two pages a step, copied by all lanes of the warp (16-byte asynchronous copies into the
+//    warp's ring), so a step's fixed costs are shared by 32 tokens;
+//  * S^T = K Q^T with tokens on the MMA's 16 rows and the (up to 8) heads of a kv head on its
+//    columns: half the MMAs of heads on rows. The weights' 8 x 8 tiles are transposed in registers
+//    (movmatrix) into the B fragments of O^T = V^T P^T;
+//  * codes convert two at a time (cvt e2m1x2 -> f16x2) and are multiplied by their block's scale,
+//    exactly, before the MMA: a lane's 32 K values are two blocks of one token, its 64 V values
+//    one block of four tokens;
+//  * a running maximum that moves only when a score passes it by 2^8, so most steps need no
+//    reduction over the lanes and no rescale;
+//  * weights enter PV as two fp16 parts, as in decode.cu: one rounding to fp16 would add as much
+//    error as the output's own.
+// 302 warp instructions a page (479 with decode.cu's loop): 64 conversions, 64 multiplies, 24
+// MMAs, 16 to pair the codes of neighbouring tokens for PV, the rest softmax, copies and loop.
+// Measured on a B200 (graph replay): 64 x 8192 tokens, 12/2 heads 47 us (3.2 TB/s); 8 x 64-128 K,
+// 64/8 heads 193 us (4.7 TB/s, 0.72 of the measured copy bandwidth). Conversions, fp16 multiplies
+// and MMAs hardly overlap on a scheduler (a group of one MMA and three of each takes 18.6 cycles
+// where the MMA alone takes 8 and the others 8), which is about 420 of the loop's 510 cycles a
+// page and scheduler; warps of 16 a CTA (128 registers) and the QK of the next step issued
+// between the PV of this one measured no better.
+
+#include "fp4.cuh"
+#include "pa_common.cuh"
+#include "pa_internal.h"
+#include "pa_rows.cuh"
+
+#include <atomic>
+
+namespace pa {
+namespace {
+
+// log2 of the factor by which the softmax weights are formed (as in decode.cu: keeps the fp16
+// parts of the weights normal; it cancels in O / l and is taken out of partials).
+constexpr float kPExp = 6.f;
+
+template <int D, int GT, int DEPTH, int WARPS>
+struct Tile {
+  static constexpr int NS = D / 32;          // words of eight codes a lane reads of a K token
+  static constexpr int MT = D / 16;          // PV m-tiles (head_dim rows)
+  static constexpr int NT = GT / 8;          // head tiles of eight
+  static constexpr int SLOT = (D + 2) * GT;  // partial slot floats
+  static constexpr int PT = fp4::kGroupBytes;
+  static constexpr int STAGE = 4 * PT;       // two pages: K, K, V, V
+  static constexpr size_t RING = (size_t)WARPS * DEPTH * STAGE;
+  static constexpr size_t SMEM = 128 + RING;
+};
+
+// The merges of decode.cu with fp16 or bf16 output rows. They are kept apart from that file's:
+// sharing them through a header left its kernels' resources as they were but made the FP8 decode
+// 2 % slower (66.3 -> 67.5 us at 64 x 8192 tokens, 12/2 heads).
+//
+// One output value, as fp16 or bf16.
+__device__ __forceinline__ void store_out(__half* p, float v, bool bf) {
+  if (bf) {
+    *reinterpret_cast<__nv_bfloat16*>(p) = __float2bfloat16_rn(v);
+  } else {
+    *p = __float2half_rn(v);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Log-sum-exp merge of `np` partial slots by one warp, from copies of the slots in shared
+// memory: the lanes bulk-copy the slots into `stage` (np * SLOT floats) on the warp's
+// mbarrier `bar`, so a merge waits for one L2 round trip however many pieces it has. Sums
+// run in piece order (k = 0, 1, ...): the arithmetic, and the output's bits, are the same
+// whichever CTA performs the merge. Piece k of the segment is warp (wf + k)'s slot: slot
+// 2 (wf + k) + 1 for the first piece (it starts the segment), 2 (wf + k) for the others.
+// Returns false (status flagged) if the copies did not arrive within the wait limit; the
+// caller then stops using the staging memory. Out of line: it runs a few times per CTA at
+// the end of the launch and should not add to the page loop's registers. BF: out rows are bf16.
+// ---------------------------------------------------------------------------------------
+template <int D, int GT, bool BF>
+__device__ __noinline__ bool staged_combine(const float* part, int wf, int np, int lane,
+                                            int hcnt, __half* out_rows, float* out_slot,
+                                            int* status, float* stage, uint64_t* bar,
+                                            uint32_t parity) {
+  constexpr int SLOT = (D + 2) * GT;
+  constexpr uint32_t SB = SLOT * sizeof(float);
+  constexpr int O4 = D * GT / 4 / 32;  // float4 outputs per lane
+  static_assert(D * GT / 4 % 32 == 0, "outputs must tile the warp");
+  // Earlier generic accesses (the ring's last reads, a previous merge's use of the staging
+  // memory, the acquire that made the slots visible) come before the copies.
+  fence_proxy_async_all();
+  if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)np * SB);
+  __syncwarp();
+  for (int k = lane; k < np; k += 32)
+    bulk_g2s(stage + (size_t)k * SLOT, part + ((size_t)(wf + k) * 2 + (k == 0 ? 1 : 0)) * SLOT,
+             SB, bar);
+  if (!mbar_wait_bounded(bar, parity, status)) return false;
+
+  // Weights: lane h < GT takes head h, M = max_k m_k, w_k = 2^(m_k - M) (written over m_k in
+  // the staged slot), L = sum_k w_k l_k.
+  float Lh = 0.f, Mh = neg_inf();
+  if (lane < GT) {
+    for (int k = 0; k < np; ++k) Mh = fmaxf(Mh, stage[(size_t)k * SLOT + D * GT + lane]);
+    for (int k = 0; k < np; ++k) {
+      float* mk = stage + (size_t)k * SLOT + D * GT + lane;
+      const float w = (Mh == neg_inf()) ? 0.f : ex2(*mk - Mh);
+      *mk = w;
+      Lh = fmaf(w, mk[GT], Lh);
+    }
+  }
+  __syncwarp();
+
+  // O = sum_k w_k O_k. Slots hold O as [D][GT]; float4 o covers row o / (GT/4), heads
+  // h0..h0+3 with h0 = 4 (o % (GT/4)), which is the same for all of a lane's outputs.
+  const int h0 = 4 * (lane % (GT / 4));
+  float4 acc[O4];
+#pragma unroll
+  for (int i = 0; i < O4; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k = 0; k < np; ++k) {
+    const float* sk = stage + (size_t)k * SLOT;
+    const float4 w4 = *reinterpret_cast<const float4*>(sk + D * GT + h0);
+#pragma unroll
+    for (int i = 0; i < O4; ++i) {
+      const float4 v = reinterpret_cast<const float4*>(sk)[lane + 32 * i];
+      acc[i].x = fmaf(w4.x, v.x, acc[i].x);
+      acc[i].y = fmaf(w4.y, v.y, acc[i].y);
+      acc[i].z = fmaf(w4.z, v.z, acc[i].z);
+      acc[i].w = fmaf(w4.w, v.w, acc[i].w);
+    }
+  }
+  if (out_rows != nullptr) {
+    float inv[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float L = __shfl_sync(0xffffffffu, Lh, h0 + e);
+      inv[e] = L > 0.f ? 1.f / L : 0.f;
+    }
+    if (lane < hcnt && !(Lh > 0.f)) flag_error(status, PA_ERR_EMPTY_CONTEXT);
+#pragma unroll
+    for (int i = 0; i < O4; ++i) {
+      const int d = (lane + 32 * i) / (GT / 4);
+      const float a4[4] = {acc[i].x, acc[i].y, acc[i].z, acc[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (h0 + e < hcnt) store_out(out_rows + (size_t)(h0 + e) * D + d, a4[e] * inv[e], BF);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < O4; ++i) reinterpret_cast<float4*>(out_slot)[lane + 32 * i] = acc[i];
+    if (lane < GT) {
+      out_slot[D * GT + lane] = Mh;
+      out_slot[D * GT + GT + lane] = Lh;
+    }
+  }
+  return true;
+}
+
+// ---------------------------------------------------------------------------------------
+// CTA-cooperative log-sum-exp merge of `np` partial slots (all NTHR threads of the block take
+// part; scratch is shared memory). Pass 1 forms the maxima, the per-piece weights (kept in
+// shared memory) and the denominators with every thread reading a different piece; pass 2
+// gives each thread one float4 of the [D][GT] output and U pieces' loads in flight per step,
+// so a merge costs a handful of dependent L2 round trips however many pieces there are.
+// ---------------------------------------------------------------------------------------
+template <int D, int GT, int NTHR, int U>
+struct Coop {
+  static constexpr int OUT4 = D * GT / 4;                        // float4 outputs
+  static constexpr int PG = NTHR >= OUT4 ? NTHR / OUT4 : 1;      // piece groups
+  static constexpr int OPT = NTHR >= OUT4 ? 1 : OUT4 / NTHR;     // outputs per thread
+  static constexpr int NW = NTHR / 32;
+  // Scratch floats needed for np pieces.
+  __host__ __device__ static constexpr size_t floats(int np) {
+    return 2 * GT + NW * GT + ((size_t)np * GT + 3) / 4 * 4 + (size_t)PG * OUT4 * 4;
+  }
+};
+
+template <int D, int GT, int NTHR, int U, bool BF, typename PieceFn>
+__device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __half* out_rows,
+                                             float* out_slot, int* status, float* sm) {
+  using CC = Coop<D, GT, NTHR, U>;
+  static_assert(NTHR >= CC::OUT4 || CC::OUT4 % NTHR == 0, "outputs must tile the block");
+  const int tid = threadIdx.x;
+  const int lane = tid & 31, warp = tid >> 5;
+  float* sM = sm;
+  float* sL = sm + GT;
+  float* sRed = sm + 2 * GT;
+  float* sW = sRed + CC::NW * GT;
+  float4* sAcc = reinterpret_cast<float4*>(sW + ((size_t)np * GT + 3) / 4 * 4);
+
+  float mx[GT];
+#pragma unroll
+  for (int h = 0; h < GT; ++h) mx[h] = neg_inf();
+  for (int k = tid; k < np; k += NTHR) {
+    const float4* mk = reinterpret_cast<const float4*>(piece(k) + D * GT);
+#pragma unroll
+    for (int h4 = 0; h4 < GT / 4; ++h4) {
+      const float4 v = __ldcg(mk + h4);
+      mx[4 * h4 + 0] = fmaxf(mx[4 * h4 + 0], v.x);
+      mx[4 * h4 + 1] = fmaxf(mx[4 * h4 + 1], v.y);
+      mx[4 * h4 + 2] = fmaxf(mx[4 * h4 + 2], v.z);
+      mx[4 * h4 + 3] = fmaxf(mx[4 * h4 + 3], v.w);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < GT; ++h) {
+    const float v = warp_max(mx[h]);
+    if (lane == 0) sRed[warp * GT + h] = v;
+  }
+  __syncthreads();
+  if (tid < GT) {
+    float v = neg_inf();
+    for (int w = 0; w < CC::NW; ++w) v = fmaxf(v, sRed[w * GT + tid]);
+    sM[tid] = v;
+  }
+  __syncthreads();
+  float ls[GT];
+#pragma unroll
+  for (int h = 0; h < GT; ++h) ls[h] = 0.f;
+  for (int k = tid; k < np; k += NTHR) {
+    const float4* mk = reinterpret_cast<const float4*>(piece(k) + D * GT);
+#pragma unroll
+    for (int h4 = 0; h4 < GT / 4; ++h4) {
+      const float4 m4 = __ldcg(mk + h4);
+      const float4 l4 = __ldcg(mk + GT / 4 + h4);
+      const float mm[4] = {m4.x, m4.y, m4.z, m4.w};
+      const float ll[4] = {l4.x, l4.y, l4.z, l4.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int h = 4 * h4 + e;
+        const float M = sM[h];
+        const float w = (M == neg_inf()) ? 0.f : ex2(mm[e] - M);
+        sW[(size_t)k * GT + h] = w;
+        ls[h] += w * ll[e];
+      }
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < GT; ++h) {
+    float v = ls[h];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (lane == 0) sRed[warp * GT + h] = v;
+  }
+  __syncthreads();
+  if (tid < GT) {
+    float v = 0.f;
+    for (int w = 0; w < CC::NW; ++w) v += sRed[w * GT + tid];
+    sL[tid] = v;
+  }
+  __syncthreads();
+
+  const int pg = (NTHR >= CC::OUT4) ? tid / CC::OUT4 : 0;
+  float4 acc[CC::OPT];
+#pragma unroll
+  for (int i = 0; i < CC::OPT; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (pg < CC::PG) {
+#pragma unroll
+    for (int i = 0; i < CC::OPT; ++i) {
+      const int o = (NTHR >= CC::OUT4) ? tid % CC::OUT4 : tid + i * NTHR;
+      const int h0 = (o % (GT / 4)) * 4;
+      for (int k0 = pg; k0 < np; k0 += CC::PG * U) {
+        float4 v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int k = k0 + u * CC::PG;
+          v[u] = (k < np) ? __ldcg(reinterpret_cast<const float4*>(piece(k)) + o)
+                          : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int k = k0 + u * CC::PG;
+          if (k < np) {
+            const float* w = sW + (size_t)k * GT + h0;
+            acc[i].x += w[0] * v[u].x;
+            acc[i].y += w[1] * v[u].y;
+            acc[i].z += w[2] * v[u].z;
+            acc[i].w += w[3] * v[u].w;
+          }
+        }
+      }
+    }
+  }
+  if constexpr (CC::PG > 1) {
+    if (pg < CC::PG) sAcc[pg * CC::OUT4 + tid % CC::OUT4] = acc[0];
+    __syncthreads();
+    if (pg == 0) {
+      for (int g2 = 1; g2 < CC::PG; ++g2) {
+        const float4 t = sAcc[g2 * CC::OUT4 + tid];
+        acc[0].x += t.x;
+        acc[0].y += t.y;
+        acc[0].z += t.z;
+        acc[0].w += t.w;
+      }
+    }
+  }
+  if (pg == 0) {
+#pragma unroll
+    for (int i = 0; i < CC::OPT; ++i) {
+      const int o = (NTHR >= CC::OUT4) ? tid : tid + i * NTHR;
+      const int d = o / (GT / 4);
+      const int h0 = (o % (GT / 4)) * 4;
+      const float a4[4] = {acc[i].x, acc[i].y, acc[i].z, acc[i].w};
+      if (out_rows != nullptr) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int h = h0 + e;
+          if (h < hcnt) {
+            const float L = sL[h];
+            store_out(out_rows + (size_t)h * D + d, L > 0.f ? a4[e] / L : 0.f, BF);
+          }
+        }
+      } else {
+        reinterpret_cast<float4*>(out_slot)[o] = acc[i];
+      }
+    }
+  }
+  if (tid < GT) {
+    if (out_slot != nullptr) {
+      out_slot[D * GT + tid] = sM[tid];
+      out_slot[D * GT + GT + tid] = sL[tid];
+    } else if (tid < hcnt && !(sL[tid] > 0.f)) {
+      flag_error(status, PA_ERR_EMPTY_CONTEXT);
+    }
+  }
+  __syncthreads();
+}
+
+// ---------------------------------------------------------------------------------------
+// LSE reduce of the split-K pair (and of partials gathered across GPUs): one CTA of
+// kReduceThreads threads per (sequence, kv-head, head tile) segment, merged cooperatively.
+// ---------------------------------------------------------------------------------------
+constexpr int kReduceThreads = 512;
+
+template <int D, int GT>
+__global__ void __launch_bounds__(kReduceThreads, 1) reduce_bf16_kernel(const ReduceArgs a) {
+  extern __shared__ __align__(16) float rsm[];
+  const int SEGS = a.KVH * a.HT;
+  const int segid = blockIdx.x;
+  const int b = segid / SEGS;
+  const int seg = segid - b * SEGS;
+  const int kvh = seg / a.HT;
+  const int ht = seg - kvh * a.HT;
+  const int hbase = kvh * a.G + ht * GT;
+  const int hcnt = min(GT, a.G - ht * GT);
+  int np = a.num_parts;
+  if (np <= 0) {
+    int c = __ldg(a.context_lens + b);
+    const int cap = a.max_blocks * a.bs;
+    c = c < 0 ? 0 : (c > cap ? cap : c);
+    const int pages = (c + kSubTokens - 1) / kSubTokens;
+    np = (pages + kSplitPages - 1) / kSplitPages;
+  }
+  __half* orow = a.out + ((size_t)b * a.H + hbase) * D;
+  if (np == 0) {
+    for (int i = threadIdx.x; i < hcnt * D; i += blockDim.x) orow[i] = __float2half_rn(0.f);
+    if (threadIdx.x == 0 && seg == 0) flag_error(a.status, PA_ERR_EMPTY_CONTEXT);
+    return;
+  }
+  const float* base = a.part + (size_t)segid * a.seg_stride;
+  coop_combine<D, GT, kReduceThreads, 16, true>(
+      [&](int k) { return base + (size_t)k * a.piece_stride; }, np, hcnt, orow, nullptr,
+      a.status, rsm);
+}
+
+// ---------------------------------------------------------------------------------------
+// Decode step over a 4-bit cache: one warp quantises the new token's K and V rows (16-bit, at
+// src_k / src_v) and stores them into the cache, at token `off` of page row `row`, before it
+// loads the page. Only the calling warp reads the page.
+// ---------------------------------------------------------------------------------------
+template <int D>
+__device__ __noinline__ void store_new_token_fp4(const uint8_t* src_k, const uint8_t* src_v,
+                                                 int new_dtype, uint8_t* kc, uint8_t* vc,
+                                                 size_t row, int off, int bs, int lane) {
+  static_assert(D == 128, "one lane per four head_dim values");
+  const size_t grp = fp4::group_offset(row, off, bs);
+  const int t = off % fp4::kGroupTokens;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const uint8_t* src = which ? src_v : src_k;
+    float x[4];
+    if (new_dtype == PA_DTYPE_BF16) {
+      load_vals<__nv_bfloat16, 4>(reinterpret_cast<const __nv_bfloat16*>(src) + 4 * lane, x);
+    } else {
+      load_vals<__half, 4>(reinterpret_cast<const __half*>(src) + 4 * lane, x);
+    }
+    uint32_t sb;
+    const uint32_t w = fp4::warp_quantize4<false>(x, sb);
+    uint8_t* dst = (which ? vc : kc) + grp;
+    *reinterpret_cast<uint16_t*>(dst + t * fp4::kCodeRow + 2 * lane) = (uint16_t)w;
+    if ((lane & 3) == 0) dst[fp4::scale_offset(which != 0, t, lane >> 2)] = (uint8_t)sb;
+  }
+  __syncwarp();
+}
+
+// ---------------------------------------------------------------------------------------
+// The decode kernel.
+// ---------------------------------------------------------------------------------------
+template <int D, int GT, int DEPTH, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeFp4Args a) {
+  using C = Tile<D, GT, DEPTH, WARPS>;
+  constexpr int NS = C::NS;
+  constexpr int MT = C::MT;
+  constexpr int NT = C::NT;
+  constexpr int SLOT = C::SLOT;
+  constexpr int NTHR = WARPS * 32;
+
+  __shared__ int s_pre[kBMax + 1];
+  __shared__ int s_ctx[kBMax];
+  __shared__ int s_tmp[32];
+  __shared__ int s_empty;
+  __shared__ unsigned s_over[kBMax / 32];  // sequences whose context exceeds the table
+  __shared__ int s_pend[WARPS][2][6];
+  __shared__ int s_npend[WARPS];
+  __shared__ uint64_t s_mmb[WARPS];     // per-warp barrier of the end-of-launch merges
+  __shared__ int s_nblk[WARPS][32];     // block ids of a warp's next batch of pages
+  __shared__ int s_nmeta[WARPS][32];    // their (kv_head << 3) | subpage
+  __shared__ int s_nwr[WARPS][32];      // their decode-step new-token sequence, or -1
+  extern __shared__ __align__(16) uint8_t dsm_raw[];
+  uint8_t* ring = dsm_raw + ((128u - (smem_u32(dsm_raw) & 127u)) & 127u);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int g = lane >> 2;  // MMA group (row / column index)
+  const int r = lane & 3;   // position inside the group
+
+  if (lane == 0) {
+    mbar_init(&s_mmb[warp], 1);
+    fence_mbar_init();
+  }
+  if (threadIdx.x == 0) {
+    s_empty = 0;
+    // This CTA's share of the block tables and q rows into L2, so the first block-id and q
+    // reads after the scan do not each wait for DRAM.
+    prefetch_l2_share(a.block_table, (size_t)a.B * a.max_blocks * sizeof(int), blockIdx.x,
+                      gridDim.x);
+    prefetch_l2_share(a.q, (size_t)a.B * a.H * D * sizeof(__half), blockIdx.x, gridDim.x);
+  }
+
+  // ---- 1. Scan of per-sequence page counts (all CTAs, identical result) -------------------
+  const int SEGS = a.KVH * a.HT;
+  const int cap = a.max_blocks * a.bs;
+  int carry = 0;
+  for (int i = threadIdx.x; i < kBMax / 32; i += NTHR) s_over[i] = 0u;
+  __syncthreads();
+  for (int base = 0; base < a.B; base += NTHR) {
+    const int b = base + threadIdx.x;
+    int w = 0;
+    if (b < a.B) {
+      int c = __ldg(a.context_lens + b);
+      if (c < 1) {
+        if (blockIdx.x == 0 && a.mode != kModePartial) flag_error(a.status, PA_ERR_EMPTY_CONTEXT);
+        if (blockIdx.x == 0 && c < 0) flag_error(a.status, PA_ERR_CONTEXT_RANGE);
+        s_empty = 1;
+        c = 0;
+      }
+      if (c > cap) {
+        if (blockIdx.x == 0) flag_error(a.status, PA_ERR_CONTEXT_RANGE);
+        atomicOr(&s_over[b >> 5], 1u << (b & 31));
+        c = cap;
+      }
+      s_ctx[b] = c;
+      w = ((c + kSubTokens - 1) / kSubTokens) * SEGS;
+    }
+    int v = w;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += t;
+    }
+    if (lane == 31) s_tmp[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+      int t = (lane < WARPS) ? s_tmp[lane] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, t, o);
+        if (lane >= o) t += u;
+      }
+      if (lane < WARPS) s_tmp[lane] = t;
+    }
+    __syncthreads();
+    if (b < a.B) s_pre[b] = carry + (warp ? s_tmp[warp - 1] : 0) + v - w;
+    carry += s_tmp[WARPS - 1];
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) s_pre[a.B] = carry;
+  __syncthreads();
+  const int T = carry;
+
+  // Sequences with no tokens: zero output (stream) or an empty partial (partial mode).
+  if (blockIdx.x == 0 && s_empty) {
+    if (a.mode == kModeStream) {
+      const int per_b = a.H * D / 8;
+      for (int i = threadIdx.x; i < a.B * per_b; i += NTHR) {
+        const int b = i / per_b;
+        if (s_ctx[b] == 0)
+          reinterpret_cast<uint4*>(a.out + (size_t)b * a.H * D)[i - b * per_b] =
+              make_uint4(0u, 0u, 0u, 0u);
+      }
+    } else if (a.mode == kModePartial) {
+      for (int i = threadIdx.x; i < a.B * SEGS * SLOT; i += NTHR) {
+        const int segid = i / SLOT;
+        const int b = segid / SEGS;
+        if (s_ctx[b] == 0) {
+          const int k = i - segid * SLOT;
+          a.part_out[i] = (k >= D * GT && k < D * GT + GT) ? neg_inf() : 0.f;
+        }
+      }
+    }
+  }
+  if (T == 0) return;
+
+  auto pages_of = [&](int b) { return (s_ctx[b] + kSubTokens - 1) / kSubTokens; };
+  // Flattened page index -> (sequence, segment inside the sequence, subpage).
+  auto locate = [&](int p, int& b, int& seg, int& sp) {
+    int lo = 0, hi = a.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (s_pre[mid] <= p) lo = mid; else hi = mid - 1;
+    }
+    b = lo;
+    const int rel = p - s_pre[b];
+    const int pg = pages_of(b);
+    seg = rel / pg;
+    sp = rel - seg * pg;
+  };
+  // Smallest split start >= p (split mode).
+  auto snap = [&](long long p) -> long long {
+    if (p >= T) return T;
+    int b, seg, sp;
+    locate((int)p, b, seg, sp);
+    const int pg = pages_of(b);
+    const int sp2 = (sp + kSplitPages - 1) / kSplitPages * kSplitPages;
+    if (sp2 >= pg) return (long long)s_pre[b] + (long long)(seg + 1) * pg;
+    return (long long)s_pre[b] + (long long)seg * pg + sp2;
+  };
+
+  // ---- 2. This warp's page range ------------------------------------------------------------
+  const long long Wt = min((long long)a.total_warps, (long long)T);
+  const int wg = blockIdx.x * WARPS + warp;
+  long long p0 = 0, p1 = 0;
+  if (wg < Wt) {
+    p0 = (long long)wg * T / Wt;
+    p1 = (long long)(wg + 1) * T / Wt;
+    if (a.mode == kModeSplit) {
+      p0 = snap(p0);
+      p1 = snap(p1);
+    }
+  }
+  const int n = (int)(p1 - p0);
+  int nrec = 0;              // shared segments whose arrival this warp recorded
+  int old0 = 0, old1 = 0;    // lane 0: the arrival counters' values before those arrivals
+  if (n > 0) {
+
+  // ---- 3. Consumer position and the first piece's q rows --------------------------------------
+  int cb, cseg, csp;
+  locate((int)p0, cb, cseg, csp);
+  int cpg = pages_of(cb);
+  int cctx = s_ctx[cb];
+  const float qs = a.qk_scale_log2;
+
+  // Q as the B fragments of the QK MMA (fp16): values 32r .. 32r + 31 of head g (qa) and, with 16
+  // heads to a tile, of head g + 8 (qb).
+  uint4 qa[NS], qb[NS];
+  uint4 ra[NS], rb[NS];  // q rows fetched ahead of the piece that uses them
+  int q_b = -1, q_seg = -1;
+
+  auto fetch_q = [&](int b, int seg) {
+    const int kvh = seg / a.HT;
+    const int ht = seg - kvh * a.HT;
+    const int hl = ht * GT + g;
+    const __half* qrow = a.q + ((size_t)b * a.H + (size_t)kvh * a.G + hl) * D + 32 * r;
+#pragma unroll
+    for (int si = 0; si < NS; ++si) {
+      ra[si] = (hl < a.G) ? __ldg(reinterpret_cast<const uint4*>(qrow) + si)
+                          : make_uint4(0u, 0u, 0u, 0u);
+      rb[si] = make_uint4(0u, 0u, 0u, 0u);
+      if (GT == 16 && hl + 8 < a.G) rb[si] = __ldg(reinterpret_cast<const uint4*>(qrow + 8 * D) + si);
+    }
+  };
+  // Eight bf16 values as fp16: exact inside the fp16 normal range; larger magnitudes saturate and
+  // are flagged, as by the conversion kernel of pa_decode_bf16q.
+  auto bf16_to_f16 = [&](uint4 v) {
+    const uint32_t src[4] = {v.x, v.y, v.z, v.w};
+    uint32_t dst[4];
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float lo = __uint_as_float(src[e] << 16), hi = __uint_as_float(src[e] & 0xffff0000u);
+      if (fabsf(lo) > 65504.f) {
+        bad = true;
+        lo = copysignf(65504.f, lo);
+      }
+      if (fabsf(hi) > 65504.f) {
+        bad = true;
+        hi = copysignf(65504.f, hi);
+      }
+      dst[e] = pack_f16x2(lo, hi);
+    }
+    if (bad) flag_error(a.status, PA_ERR_Q_RANGE);
+    return make_uint4(dst[0], dst[1], dst[2], dst[3]);
+  };
+  auto convert_q = [&]() {
+#pragma unroll
+    for (int si = 0; si < NS; ++si) {
+      qa[si] = a.act_bf16 ? bf16_to_f16(ra[si]) : ra[si];
+      if constexpr (NT == 2) qb[si] = a.act_bf16 ? bf16_to_f16(rb[si]) : rb[si];
+    }
+  };
+  // The first piece's q rows are requested before the page copies, so their latency overlaps
+  // the block-table reads and the first copies rather than queueing behind them.
+  fetch_q(cb, cseg);
+  q_b = cb;
+  q_seg = cseg;
+
+  // ---- 4. Producer: the group indices of 32 upcoming pages, one per lane. With a decode step, wr
+  // receives the sequence whose new token lies in the page (the last page of a segment whose
+  // context and block id are valid), else -1.
+  const bool step_write = a.new_k != nullptr;
+  const uint64_t pol = l2_policy_evict_first();
+  // Page jbase + lane of the range: the address of its block id, its (kv_head << 3) | subpage
+  // and, for a decode step, the sequence whose new token it holds (else -1).
+  auto page_ref = [&](int jbase, int& meta, int& wr) -> const int* {
+    meta = 0;
+    wr = -1;
+    const int jj = jbase + lane;
+    if (jj >= n) return nullptr;
+    int b, seg, sp;
+    locate((int)(p0 + jj), b, seg, sp);
+    const int bi = sp / a.subs;
+    meta = ((seg / a.HT) << 3) | (sp - bi * a.subs);
+    if (step_write && sp == pages_of(b) - 1 && !((s_over[b >> 5] >> (b & 31)) & 1u)) wr = b;
+    return a.block_table + (size_t)b * a.max_blocks + bi;
+  };
+  // Group index of a page (below 2^31); a block id outside the cache is flagged and read as block
+  // 0, and its new token (if any) is not written.
+  auto pack_page = [&](int blk, int meta, int& wr) -> uint32_t {
+    if (blk < 0 || blk >= a.NB) {
+      flag_error(a.status, PA_ERR_BLOCK_ID);
+      blk = 0;
+      wr = -1;
+    }
+    return (uint32_t)((blk * a.KVH + (meta >> 3)) * a.subs + (meta & 7));
+  };
+  int curw, meta0;
+  const int* bref0 = page_ref(0, meta0, curw);
+  const int blk0 = bref0 != nullptr ? __ldg(bref0) : 0;
+  uint32_t cur = pack_page(blk0, meta0, curw);
+
+  // Decode step: the new token in the page of group gi, if it holds one (sequence wb >= 0), is
+  // written into the cache before the page is copied.
+  auto write_new = [&](uint32_t gi, int wb) {
+    if (wb < 0) return;
+    const uint32_t row = gi / (uint32_t)a.subs;
+    const size_t so = ((size_t)wb * a.new_stride + (size_t)(row % (uint32_t)a.KVH) * D) * 2;
+    store_new_token_fp4<D>(static_cast<const uint8_t*>(a.new_k) + so,
+                           static_cast<const uint8_t*>(a.new_v) + so, a.new_dtype, a.k_write,
+                           a.v_write, row, (s_ctx[wb] - 1) % a.bs, a.bs, lane);
+    __threadfence();  // the copies read what the warp has just written, from L2
+  };
+  // The warp's ring is filled by 16-byte asynchronous copies of all its lanes, one commit group
+  // per stage of two pages. (Four bulk copies per stage, issued by one lane, cost 87 of the step's
+  // 640 instructions; nine copies a lane and their addresses cost about 25.) A page's K and V
+  // groups are 72 chunks each: two rounds of the warp, and the last eight chunks of all four
+  // groups in one more round.
+  const uint32_t my_ring = smem_u32(ring) + (uint32_t)(warp * DEPTH) * (uint32_t)C::STAGE;
+  const uint8_t* k_lane = a.k_cache + 16 * lane;
+  const uint8_t* v_lane = a.v_cache + 16 * lane;
+  const uint8_t* rest_lane = ((lane & 16) ? a.v_cache : a.k_cache) + 1024 + 16 * (lane & 7);
+  const uint32_t rest_off =
+      (uint32_t)(lane >> 3) * (uint32_t)C::PT + 1024u + 16u * (uint32_t)(lane & 7);
+  // Pages jj and jj + 1 (jj even; asked for in order) into stage s; past the range's end the
+  // group is empty, and a missing second page is the first once more. The ids of the next 32
+  // pages come along with a batch's first stage, sixteen groups before they are needed.
+  static_assert(2 * DEPTH < 32, "a batch's ids must arrive before the batch begins");
+  auto issue_pair = [&](int jj, int s) {
+    if (jj < n) {
+      if ((jj & 31) == 0) {
+        if (jj > 0) {
+          curw = s_nwr[warp][lane];
+          cur = pack_page(s_nblk[warp][lane], s_nmeta[warp][lane], curw);
+        }
+        int meta, wr;
+        const int* p = page_ref(jj + 32, meta, wr);
+        s_nmeta[warp][lane] = meta;
+        s_nwr[warp][lane] = wr;
+        if (p != nullptr) {
+          cp_async_4(&s_nblk[warp][lane], p);
+        } else {
+          s_nblk[warp][lane] = 0;  // past the range: any valid id
+        }
+      }
+      const int i1 = (jj & 31) + (jj + 1 < n ? 1 : 0);
+      const uint32_t g0 = __shfl_sync(0xffffffffu, cur, jj & 31);
+      const uint32_t g1 = __shfl_sync(0xffffffffu, cur, i1);
+      if (step_write) {
+        write_new(g0, __shfl_sync(0xffffffffu, curw, jj & 31));
+        write_new(g1, __shfl_sync(0xffffffffu, curw, i1));
+      }
+      const uint32_t st = my_ring + (uint32_t)s * (uint32_t)C::STAGE;
+      const uint32_t sl = st + 16u * (uint32_t)lane;
+      const size_t o0 = (size_t)g0 * C::PT, o1 = (size_t)g1 * C::PT;
+      cp_async_16_hint(sl, k_lane + o0, pol);
+      cp_async_16_hint(sl + 512, k_lane + o0 + 512, pol);
+      cp_async_16_hint(sl + C::PT, k_lane + o1, pol);
+      cp_async_16_hint(sl + C::PT + 512, k_lane + o1 + 512, pol);
+      cp_async_16_hint(sl + 2 * C::PT, v_lane + o0, pol);
+      cp_async_16_hint(sl + 2 * C::PT + 512, v_lane + o0 + 512, pol);
+      cp_async_16_hint(sl + 3 * C::PT, v_lane + o1, pol);
+      cp_async_16_hint(sl + 3 * C::PT + 512, v_lane + o1 + 512, pol);
+      cp_async_16_hint(st + rest_off, rest_lane + (size_t)((lane & 8) ? g1 : g0) * C::PT, pol);
+    }
+    cp_async_commit();
+  };
+  __syncwarp();
+  for (int j = 0; j < DEPTH; ++j) issue_pair(2 * j, j);
+  convert_q();
+
+  // Running maximum and sum of heads nt * 8 + 2r and the next; fmb = kPExp - fm.
+  float fm[NT][2], fl[NT][2], fmb[NT][2];
+  float oacc[MT][NT][4];
+  const int tau = 4 * (g >> 1) + (g & 1);  // token of K row g (row g + 8: + 2)
+
+  int s = 0;  // ring stage of page j
+  const bool split = (a.mode == kModeSplit);
+  int j = 0;
+  while (j < n) {
+    // ---- one piece: the pages of this warp's range inside one segment (one split in split
+    // mode), pages [csp, csp + len) of sequence cb, segment cseg.
+    const int piece_sp0 = csp;
+    int len = cpg - csp;
+    if (split) len = min(len, kSplitPages - csp % kSplitPages);
+    len = min(len, n - j);
+    if (q_b != cb || q_seg != cseg) {
+      fetch_q(cb, cseg);
+      convert_q();
+      q_b = cb;
+      q_seg = cseg;
+    }
+    // When this piece ends its segment and the range goes on, the next segment's q rows are
+    // brought into L1 while this piece runs, so the next piece's q fetch does not wait on L2.
+    if (csp + len == cpg && j + len < n) {
+      int nb = cb, ns = cseg + 1;
+      if (ns == SEGS) {
+        ns = 0;
+        do { ++nb; } while (pages_of(nb) == 0);
+      }
+      const int kvh = ns / a.HT;
+      const int hl = (ns - kvh * a.HT) * GT + (lane >> 1);
+      if (lane < 2 * GT && hl < a.G)
+        prefetch_l1(a.q + ((size_t)nb * a.H + (size_t)kvh * a.G + hl) * D + (lane & 1) * (D / 2));
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) oacc[i][nt][e] = 0.f;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          fm[nt][e] = neg_inf();
+          fmb[nt][e] = -neg_inf();
+          fl[nt][e] = 0.f;
+        }
+      // A stage's two pages per step; where a piece begins or ends inside a stage, the page that
+      // is not its own is masked (and met again by the other piece).
+      for (int k = 0; k < len;) {
+        const int first = j & 1;
+        const int cnt = min(2 - first, len - k);
+        if (first == 0) {  // the stage's copies: this lane's, then every lane's
+          cp_async_wait_groups<DEPTH - 1>();
+          __syncwarp();
+        }
+        const int left = cctx - (csp + k) * kSubTokens;  // tokens from the step's first page on
+        const int valid0 = first ? 0 : min(kSubTokens, left);
+        const int valid1 = first ? min(kSubTokens, left)
+                                 : (cnt == 2 ? min(kSubTokens, left - kSubTokens) : 0);
+        const bool full = valid0 == kSubTokens && valid1 == kSubTokens;
+        const uint32_t st = my_ring + (uint32_t)s * (uint32_t)C::STAGE;
+        const uint32_t ka = st + tau * fp4::kCodeRow + 16 * r;
+        const uint32_t ksa = st + fp4::kCodes + tau * 8 + 2 * r;
+        const uint32_t va = st + 2 * C::PT + 4 * r * fp4::kCodeRow + 8 * g;
+        const uint32_t vsa = st + 2 * C::PT + fp4::kCodes + 16 * g + 4 * r;
+
+        // S^T = K Q^T: rows = tokens (row g: token tau, row g + 8: tau + 2), columns = heads, so
+        // that eight heads fill the MMA. A lane reads the 32 codes 32r .. 32r + 31 of its two
+        // tokens; codes -> fp16, times the block scale, is exact (fp4.cuh).
+        float x[2][NT][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const uint4 c0 = lds128(ka + u * C::PT), c1 = lds128(ka + u * C::PT + 2 * fp4::kCodeRow);
+          const uint32_t z0 = lds16(ksa + u * C::PT), z1 = lds16(ksa + u * C::PT + 16);
+          const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
+          const uint32_t s0 = fp4::scale_pair(z0), s1 = fp4::scale_pair(z1);
+          float acc[2][NT][4];  // even and odd steps: two shorter chains
+          auto mma = [](bool begin, float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                        uint32_t a3, uint32_t b0, uint32_t b1) {
+            if (begin) mma_16816_zero(d, a0, a1, a2, a3, b0, b1);
+            else mma_16816(d, a0, a1, a2, a3, b0, b1);
+          };
+#pragma unroll
+          for (int si = 0; si < NS; ++si) {
+            uint32_t h[4], i4[4];
+            fp4::codes_to_f16x2(w0[si], h[0], h[1], h[2], h[3]);
+            fp4::codes_to_f16x2(w1[si], i4[0], i4[1], i4[2], i4[3]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              h[e] = si < NS / 2 ? fp4::hmul2_half<false>(h[e], s0)
+                                 : fp4::hmul2_half<true>(h[e], s0);
+              i4[e] = si < NS / 2 ? fp4::hmul2_half<false>(i4[e], s1)
+                                  : fp4::hmul2_half<true>(i4[e], s1);
+            }
+            mma(si == 0, acc[0][0], h[0], i4[0], h[1], i4[1], qa[si].x, qa[si].y);
+            mma(si == 0, acc[1][0], h[2], i4[2], h[3], i4[3], qa[si].z, qa[si].w);
+            if constexpr (NT == 2) {
+              mma(si == 0, acc[0][1], h[0], i4[0], h[1], i4[1], qb[si].x, qb[si].y);
+              mma(si == 0, acc[1][1], h[2], i4[2], h[3], i4[3], qb[si].z, qb[si].w);
+            }
+          }
+          // Logits in log2 units: heads nt * 8 + 2r + (e & 1) of token tau (e < 2) and tau + 2.
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              const float2 v = mul2(add2(make_float2(acc[0][nt][e], acc[0][nt][e + 1]),
+                                         make_float2(acc[1][nt][e], acc[1][nt][e + 1])),
+                                    make_float2(qs, qs));
+              x[u][nt][e] = v.x;
+              x[u][nt][e + 1] = v.y;
+            }
+        }
+        if (!full) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int vd = u ? valid1 : valid0;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (tau + (e & 2) >= vd) x[u][nt][e] = neg_inf();
+          }
+        }
+        // The reference maximum moves only when a score passes it by 2^kLazy: weights then stay
+        // below 2^(kPExp + kLazy) (far inside fp16), O and l carry the same factor, and most
+        // steps need neither a reduction over the lanes nor a rescale.
+        constexpr float kLazy = 8.f;
+        float tm[NT][2];
+        bool up = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            tm[nt][e] = fmaxf(fmaxf(x[0][nt][e], x[0][nt][2 + e]),
+                              fmaxf(x[1][nt][e], x[1][nt][2 + e]));
+            up = up || tm[nt][e] > fm[nt][e] + kLazy;
+          }
+        if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float c[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float v = tm[nt][e];
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+              c[e] = v > fm[nt][e] ? ex2(fm[nt][e] - v) : 1.f;
+              fm[nt][e] = fmaxf(v, fm[nt][e]);
+              fmb[nt][e] = kPExp - fm[nt][e];
+              fl[nt][e] *= c[e];
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {  // O's columns are the lane's own heads
+              oacc[i][nt][0] *= c[0];
+              oacc[i][nt][1] *= c[1];
+              oacc[i][nt][2] *= c[0];
+              oacc[i][nt][3] *= c[1];
+            }
+          }
+        }
+
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          // Weights, as two fp16 parts each (about 22 significant bits, as for the other
+          // caches); the transposed 8 x 8 tiles are the PV MMA's B fragments.
+          uint32_t ph0[NT], ph1[NT], pl0[NT], pl1[NT];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+              const float2 v = add2(make_float2(x[u][nt][e], x[u][nt][e + 1]),
+                                    make_float2(fmb[nt][0], fmb[nt][1]));
+              p[e] = ex2(v.x);
+              p[e + 1] = ex2(v.y);
+              const float2 l = add2(make_float2(fl[nt][0], fl[nt][1]),
+                                    make_float2(p[e], p[e + 1]));
+              fl[nt][0] = l.x;
+              fl[nt][1] = l.y;
+            }
+            split_f16x2_packed(p[0], p[1], ph0[nt], pl0[nt]);
+            split_f16x2_packed(p[2], p[3], ph1[nt], pl1[nt]);
+            ph0[nt] = transpose8x8(ph0[nt]);
+            ph1[nt] = transpose8x8(ph1[nt]);
+            pl0[nt] = transpose8x8(pl0[nt]);
+            pl1[nt] = transpose8x8(pl1[nt]);
+          }
+          // V: tokens 4r .. 4r + 3, values 16g .. 16g + 15 (one block a token). Scales of slots
+          // past the context may be anything: zero there (a finite code times zero is 0).
+          uint2 vq[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) vq[e] = lds64(va + u * C::PT + e * fp4::kCodeRow);
+          const uint32_t z = lds32(vsa + u * C::PT);
+          uint32_t s01 = fp4::scale_pair(z), s23 = fp4::scale_pair(z, 0x3424u);
+          if (!full) {
+            const int vd = u ? valid1 : valid0;
+            s01 &= ((4 * r < vd) ? 0x0000ffffu : 0u) | ((4 * r + 1 < vd) ? 0xffff0000u : 0u);
+            s23 &= ((4 * r + 2 < vd) ? 0x0000ffffu : 0u) | ((4 * r + 3 < vd) ? 0xffff0000u : 0u);
+          }
+          // O^T += V^T P^T. The MMA pairs tokens: the even and the odd head_dim codes of two
+          // tokens share a byte before they convert. Rows g and g + 8 of m-tile 4h + jj are
+          // head_dim 16g + 8h + 2jj and the next.
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t w0 = h ? vq[0].y : vq[0].x, w1 = h ? vq[1].y : vq[1].x;
+            const uint32_t w2 = h ? vq[2].y : vq[2].x, w3 = h ? vq[3].y : vq[3].x;
+            constexpr uint32_t kLow = 0x0f0f0f0fu;
+            uint32_t A0[4], A1[4], A2[4], A3[4];
+            fp4::codes_to_f16x2((w0 & kLow) | ((w1 << 4) & ~kLow), A0[0], A0[1], A0[2], A0[3]);
+            fp4::codes_to_f16x2(((w0 >> 4) & kLow) | (w1 & ~kLow), A1[0], A1[1], A1[2], A1[3]);
+            fp4::codes_to_f16x2((w2 & kLow) | ((w3 << 4) & ~kLow), A2[0], A2[1], A2[2], A2[3]);
+            fp4::codes_to_f16x2(((w2 >> 4) & kLow) | (w3 & ~kLow), A3[0], A3[1], A3[2], A3[3]);
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+              const int i = 4 * h + jj;
+              const uint32_t a0 = fp4::hmul2(A0[jj], s01), a1 = fp4::hmul2(A1[jj], s01);
+              const uint32_t a2 = fp4::hmul2(A2[jj], s23), a3 = fp4::hmul2(A3[jj], s23);
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma_16816(oacc[i][nt], a0, a1, a2, a3, ph0[nt], ph1[nt]);
+                mma_16816(oacc[i][nt], a0, a1, a2, a3, pl0[nt], pl1[nt]);
+              }
+            }
+          }
+        }
+        k += cnt;
+        j += cnt;
+        if ((j & 1) == 0) {  // both pages of the stage are done with: refill it
+          __syncwarp();
+          issue_pair(j + 2 * DEPTH - 2, s);
+          if (++s == DEPTH) s = 0;
+        }
+      }
+    csp += len;
+
+    {
+      // ---- piece epilogue ---------------------------------------------------------------------
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1)
+            fl[nt][e] += __shfl_xor_sync(0xffffffffu, fl[nt][e], o);
+      const int segid = cb * SEGS + cseg;
+      const int kvh = cseg / a.HT;
+      const int ht = cseg - kvh * a.HT;
+      const int hbase = kvh * a.G + ht * GT;
+      const int hcnt = min(GT, a.G - ht * GT);
+
+      // Partial slots hold O and l without the 2^kPExp weight factor (an exact rescale).
+      auto write_slot = [&](float* slot) {
+        constexpr float kUnscale = 1.f / (float)(1 << (int)kPExp);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            *reinterpret_cast<float2*>(slot + (16 * g + 2 * i) * GT + nt * 8 + 2 * r) =
+                make_float2(oacc[i][nt][0] * kUnscale, oacc[i][nt][1] * kUnscale);
+            *reinterpret_cast<float2*>(slot + (16 * g + 2 * i + 1) * GT + nt * 8 + 2 * r) =
+                make_float2(oacc[i][nt][2] * kUnscale, oacc[i][nt][3] * kUnscale);
+          }
+        }
+        if (g == 0) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            *reinterpret_cast<float2*>(slot + D * GT + nt * 8 + 2 * r) =
+                make_float2(fm[nt][0], fm[nt][1]);
+            *reinterpret_cast<float2*>(slot + D * GT + GT + nt * 8 + 2 * r) =
+                make_float2(fl[nt][0] * kUnscale, fl[nt][1] * kUnscale);
+          }
+        }
+      };
+
+      if (split) {
+        write_slot(a.part + ((size_t)segid * a.s_max + piece_sp0 / kSplitPages) * SLOT);
+      } else if (piece_sp0 == 0 && csp == cpg) {
+        // The whole segment was this warp's: normalise and store directly.
+        if (a.mode == kModeStream) {
+          // A lane holds values 16g .. 16g + 15 of its heads: 32 contiguous bytes each.
+          __half* ob = a.out + ((size_t)cb * a.H + hbase) * D;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int h = nt * 8 + 2 * r + e;
+              const float f = 1.f / fl[nt][e];
+              uint32_t w[MT];
+#pragma unroll
+              for (int i = 0; i < MT; ++i) {
+                const float lo = oacc[i][nt][e] * f, hi = oacc[i][nt][2 + e] * f;
+                if (a.act_bf16) {
+                  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+                  w[i] = *reinterpret_cast<const uint32_t*>(&v);
+                } else {
+                  w[i] = pack_f16x2(lo, hi);
+                }
+              }
+              if (h < hcnt) {
+                uint4* o = reinterpret_cast<uint4*>(ob + (size_t)h * D + 16 * g);
+                o[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                o[1] = make_uint4(w[4], w[5], w[6], w[7]);
+              }
+            }
+        } else {
+          write_slot(a.part_out + (size_t)segid * SLOT);
+        }
+      } else {
+        // A piece of a segment shared with neighbouring warps.
+        write_slot(a.part + ((size_t)wg * 2 + (piece_sp0 == 0 ? 1 : 0)) * SLOT);
+        __syncwarp();
+        const long long s_start = (long long)s_pre[cb] + (long long)cseg * cpg;
+        const long long s_end = s_start + cpg;
+        const int wf = (int)(((s_start + 1) * Wt - 1) / T);
+        const int wl = (int)((s_end * Wt - 1) / T);
+        const int np = wl - wf + 1;
+        // Release this piece; the arrival that completes the count acquires all of them and
+        // owes the merge, which runs after the page loop, when the registers are free. The
+        // merge is recorded now and kept if the atomic's old value shows the last arrival;
+        // that value is first read after the loop, so the loop does not wait for the atomic.
+        // A warp shares at most two segments (its first and its last).
+        if (lane == 0 && nrec < 2) {
+          if (nrec == 0) {
+            old0 = atom_add_acq_rel_gpu(a.counters + segid, 1);
+          } else {
+            old1 = atom_add_acq_rel_gpu(a.counters + segid, 1);
+          }
+          int* pe = s_pend[warp][nrec];
+          pe[0] = segid;
+          pe[1] = wf;
+          pe[2] = np;
+          pe[3] = cb;
+          pe[4] = hbase;
+          pe[5] = hcnt;
+        }
+        ++nrec;
+      }
+    }
+
+    // ---- next segment
+    if (csp == cpg) {
+      csp = 0;
+      if (++cseg == SEGS) {
+        cseg = 0;
+        if (j < n) {
+          do { ++cb; } while (pages_of(cb) == 0);
+          cctx = s_ctx[cb];
+        }
+      }
+      if (j < n) cpg = pages_of(cb);
+    }
+  }
+
+  cp_async_wait_all();
+  }  // n > 0
+
+  // ---- 5. Merges of the segments whose last piece this CTA's warps finished ------------------
+  // The pieces of a recorded merge are visible: the recording arrival acquired them, and the
+  // barrier below orders that arrival before every warp's reads.
+  // Each merge of up to kStageCap pieces is one warp's: it bulk-copies the pieces into the
+  // (now idle) ring memory and merges them from there, side by side with the CTA's other
+  // merges; merges are packed into the ring memory in a fixed order, in waves when they do not
+  // all fit at once. Only a merge of more pieces than the ring memory holds runs on the whole
+  // CTA, reading the pieces from L2.
+  if (lane == 0) {
+    // The recorded merges this warp owes: those whose arrival completed the count.
+    int k = 0;
+    for (int e = 0; e < min(nrec, 2); ++e) {
+      const int* pe = s_pend[warp][e];
+      if ((e == 0 ? old0 : old1) == pe[2] - 1) {
+        if (k != e)
+          for (int f = 0; f < 6; ++f) s_pend[warp][k][f] = pe[f];
+        ++k;
+      }
+    }
+    s_npend[warp] = k;
+  }
+  __syncthreads();  // every warp is past its page loop: the ring memory is free
+  constexpr size_t kRing = C::RING;
+  constexpr int kStageCap = (int)(kRing / (SLOT * sizeof(float)));
+  float* scratch = reinterpret_cast<float*>(ring);
+  const bool stream = (a.mode == kModeStream);
+  int used = 0, inwave = 0;
+  uint32_t mph = 0;  // phase parity of this warp's merge barrier
+  bool any_big = false;
+  for (int w = 0; w < WARPS; ++w) {
+    for (int e = 0; e < s_npend[w]; ++e) {
+      const int* pe = s_pend[w][e];
+      const int np = pe[2];
+      if (np > kStageCap) {
+        any_big = true;
+        continue;
+      }
+      if (used + np > kStageCap || inwave == WARPS) {
+        __syncthreads();  // the wave's merges are done with the ring memory
+        used = 0;
+        inwave = 0;
+      }
+      if (inwave == warp) {
+        const int segid = pe[0], wf = pe[1], b = pe[3], hbase = pe[4], hcnt = pe[5];
+        __half* orow = stream ? a.out + ((size_t)b * a.H + hbase) * D : nullptr;
+        float* oslot = stream ? nullptr : a.part_out + (size_t)segid * SLOT;
+        float* stg = scratch + (size_t)used * SLOT;
+        const bool done =
+            a.act_bf16
+                ? staged_combine<D, GT, true>(a.part, wf, np, lane, hcnt, orow, oslot, a.status, stg,
+                                              &s_mmb[warp], mph)
+                : staged_combine<D, GT, false>(a.part, wf, np, lane, hcnt, orow, oslot, a.status,
+                                               stg, &s_mmb[warp], mph);
+        if (!done) {
+          // Timed out: let the copies land before the memory is used again.
+          (void)mbar_wait_bounded(&s_mmb[warp], mph, nullptr);
+        }
+        mph ^= 1u;
+        if (lane == 0) a.counters[segid] = 0;
+      }
+      used += np;
+      ++inwave;
+    }
+  }
+  if (!any_big) return;
+  __syncthreads();  // the staged merges are done with the ring memory
+  for (int w = 0; w < WARPS; ++w) {
+    for (int e = 0; e < s_npend[w]; ++e) {
+      const int* pe = s_pend[w][e];
+      const int segid = pe[0], wf = pe[1], np = pe[2], b = pe[3], hbase = pe[4], hcnt = pe[5];
+      if (np <= kStageCap) continue;
+      if (Coop<D, GT, NTHR, 8>::floats(np) * sizeof(float) > kRing) {
+        if (threadIdx.x == 0) {
+          flag_error(a.status, PA_ERR_WORKSPACE);
+          a.counters[segid] = 0;  // leave the counter ready for the next call
+        }
+        continue;
+      }
+      auto piece = [&](int k) -> const float* {
+        return a.part + ((size_t)(wf + k) * 2 + (k == 0 ? 1 : 0)) * SLOT;
+      };
+      if (stream && a.act_bf16) {
+        coop_combine<D, GT, NTHR, 8, true>(piece, np, hcnt,
+                                         a.out + ((size_t)b * a.H + hbase) * D, nullptr,
+                                         a.status, scratch);
+      } else if (stream) {
+        coop_combine<D, GT, NTHR, 8, false>(piece, np, hcnt, a.out + ((size_t)b * a.H + hbase) * D,
+                                     nullptr, a.status, scratch);
+      } else {
+        coop_combine<D, GT, NTHR, 8, false>(piece, np, hcnt, nullptr,
+                                     a.part_out + (size_t)segid * SLOT, a.status, scratch);
+      }
+      if (threadIdx.x == 0) a.counters[segid] = 0;
+    }
+  }
+}
+
+// Warps per CTA and ring stages per warp, by head tile (16 heads keep twice the accumulators).
+// Twelve warps: 168 registers. 64 x 8192 / 8 x 64-128 K tokens: 47.2 / 192.8 us with three stages,
+// 50.7 / 192.3 with two, 49.1 / 212.9 with eight warps, 51.4 / 196.1 with sixteen.
+template <int GT> struct Shape;
+template <> struct Shape<8> { static constexpr int W = 12, DP = 3; };
+template <> struct Shape<16> { static constexpr int W = 8, DP = 4; };
+
+template <int GT>
+cudaError_t launch_one(const DecodeFp4Args& a, int grid, cudaStream_t stream) {
+  constexpr int W = Shape<GT>::W;
+  constexpr int DP = Shape<GT>::DP;
+  using C = Tile<128, GT, DP, W>;
+  static_assert(C::SMEM + 14 * 1024 <= 227 * 1024, "shared memory of a launch");
+  auto kern = decode_fp4_kernel<128, GT, DP, W>;
+  // The shared-memory opt-in is a per-device function attribute: set it once per device.
+  static std::atomic<uint64_t> configured{0};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (!(configured.load(std::memory_order_acquire) & bit)) {
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
+    if (e != cudaSuccess) return e;
+    configured.fetch_or(bit, std::memory_order_acq_rel);
+  }
+  kern<<<grid, W * 32, C::SMEM, stream>>>(a);
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+int decode_fp4_warps_per_cta(int gt) { return gt == 8 ? Shape<8>::W : Shape<16>::W; }
+
+cudaError_t launch_decode_fp4(int gt, const DecodeFp4Args& a, int grid, cudaStream_t stream) {
+  return gt == 8 ? launch_one<8>(a, grid, stream) : launch_one<16>(a, grid, stream);
+}
+
+// launch_reduce with bf16 output rows (its checks done).
+cudaError_t launch_reduce_bf16(int gt, const ReduceArgs& a, int max_pieces, cudaStream_t stream) {
+  const int segs = a.B * a.KVH * a.HT;
+  auto launch = [&](auto kern, size_t floats) {
+    const size_t smem = floats * sizeof(float);
+    cudaError_t e =
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+    kern<<<segs, kReduceThreads, smem, stream>>>(a);
+    return cudaGetLastError();
+  };
+  return gt == 8 ? launch(reduce_bf16_kernel<128, 8>,
+                          Coop<128, 8, kReduceThreads, 16>::floats(max_pieces))
+                 : launch(reduce_bf16_kernel<128, 16>,
+                          Coop<128, 16, kReduceThreads, 16>::floats(max_pieces));
+}
+
+}  // namespace pa

@@ -59,8 +59,6 @@ struct DecodeArgs {
   void* vc_w;
   float* ks_w;
   float* vs_w;
-  const uint8_t* k_base;       // K cache base (fp4)
-  int act_bf16;                // fp4: q and out are bf16
 };
 
 struct ReduceArgs {
@@ -80,6 +78,17 @@ cudaError_t launch_decode(int kv_i8, int gt, const DecodeArgs& a, const CUtensor
                           int grid, cudaStream_t stream);
 cudaError_t launch_reduce(int gt, const ReduceArgs& a, int max_pieces, cudaStream_t stream);
 int decode_warps_per_cta(int kv_i8, int gt);
+// The decode over a 4-bit cache (decode_fp4.cu).
+struct DecodeFp4Args : DecodeArgs {
+  const uint8_t* k_cache;      // [num_blocks * kv_heads * block_size / 16] groups (fp4.cuh)
+  const uint8_t* v_cache;
+  uint8_t* k_write;            // the same caches, for a decode step's new tokens
+  uint8_t* v_write;
+  int act_bf16;                // q and out are bf16
+};
+cudaError_t launch_decode_fp4(int gt, const DecodeFp4Args& a, int grid, cudaStream_t stream);
+cudaError_t launch_reduce_bf16(int gt, const ReduceArgs& a, int max_pieces, cudaStream_t stream);
+int decode_fp4_warps_per_cta(int gt);
 // Token-granular cache writes; kind selects the cache type.
 enum RowKind {
   kRowsF16 = 0,  // fp16 copy

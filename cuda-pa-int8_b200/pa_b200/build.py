@@ -18,7 +18,8 @@ INCLUDE_DIR = os.path.join(REPO_DIR, "include")
 LIB_NAME = "libpa_b200.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 
-SOURCES = ["decode.cu", "quant.cu", "fp4.cu", "rope.cu", "tables.cu", "capi.cu", "noalloc.cu"]
+SOURCES = ["decode.cu", "decode_fp4.cu", "quant.cu", "fp4.cu", "rope.cu", "tables.cu", "capi.cu",
+           "noalloc.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ARCH_FLAGS + [
     "-O3", "-lineinfo", "-std=c++17",

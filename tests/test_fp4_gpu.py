@@ -369,3 +369,49 @@ def test_c_abi_needs_a_large_enough_workspace():
     rc = L.pa_decode_fp4(p[0], *p, 2, 8, 2, 128, kc.shape[0], 16, bt.shape[1], 0.1, ws.data_ptr(),
                          need - 1 if bt.shape[1] == 4 else 1024, None)
     assert rc == _lib.PA_ERR_WORKSPACE
+
+
+def test_long_ranges_take_many_batches_of_block_ids():
+    """Each warp's range is longer than a batch of 32 block ids and ends inside one; the shared
+    memory the ids pass through holds another launch's leavings. The single pass must agree with
+    the split-K pair and flag nothing."""
+    g = torch.Generator(device="cuda").manual_seed(17)
+    S, H, KVH, n = 24, 8, 2, 32768 - 7
+    nb = S * 2048 + 1
+    kc, vc = _ops().fp4_cache(nb, KVH)
+    for c in (kc, vc):
+        c[..., :1024] = torch.randint(0, 256, c[..., :1024].shape, generator=g, device="cuda",
+                                      dtype=torch.uint8)
+        c[..., 1024:] = torch.randint(96, 128, c[..., 1024:].shape, generator=g, device="cuda",
+                                      dtype=torch.uint8)
+    bt = torch.randperm(nb, generator=g, device="cuda")[:S * 2048].int().view(S, 2048)
+    lens = torch.tensor([n - 977 * b for b in range(S)], dtype=torch.int32, device="cuda")
+    q = torch.randn(S, H, 128, generator=g, device="cuda").half()
+    outs = []
+    for splitk in (False, True, False):
+        junk = torch.full((1 << 20,), -1.0, device="cuda").softmax(0)  # another kernel's traces
+        out = torch.empty_like(q)
+        _ops().decode(out, q, kc, vc, bt, lens, scale_for(), splitk=splitk)
+        outs.append(out)
+        del junk
+    _ops().check_status(q.device)
+    assert torch.equal(outs[0], outs[2])
+    # One sequence against 64 bits; the two forms against each other within both roundings.
+    b = 3
+    c = dict(q=q[b:b + 1].cpu(), bt=np.arange(2048, dtype=np.int32)[None],
+             kc=kc[bt[b].long()].cpu().numpy(), vc=vc[bt[b].long()].cpu().numpy(),
+             lens=lens[b:b + 1].cpu().numpy())
+    for out in outs[:2]:
+        _close(out[b:b + 1], c)
+    assert float((outs[0].float() - outs[1].float()).abs().max()) <= 2.0 ** -9
+
+
+def test_bf16_values_outside_the_fp16_range_are_flagged():
+    c = _case(18, [40, 90], 12, 2, dt=torch.bfloat16)
+    q, kc, vc, bt, cl = _gpu(c)
+    out = torch.empty_like(q)
+    _ops().decode_bf16(out, q, kc, vc, bt, cl, scale_for())
+    _ops().check_status(q.device)
+    q[1, 5, 77] = 1e6
+    _ops().decode_bf16(out, q, kc, vc, bt, cl, scale_for())
+    assert _ops().read_status(q.device) == 512  # PA_ERR_Q_RANGE
