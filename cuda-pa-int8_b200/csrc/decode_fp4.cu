@@ -394,8 +394,12 @@ __device__ __noinline__ void store_new_token_fp4(const uint8_t* src_k, const uin
 // ---------------------------------------------------------------------------------------
 // The decode kernel.
 // ---------------------------------------------------------------------------------------
-template <int D, int GT, int DEPTH, int WARPS>
+// PACK (kv heads of at most four q heads): the PV MMA's columns 0-3 take the weights' high parts
+// and columns 4-7 their low parts, one MMA instead of two; the two halves of O are added at the
+// end of a piece.
+template <int D, int GT, bool PACK, int DEPTH, int WARPS>
 __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeFp4Args a) {
+  static_assert(!PACK || GT == 8, "packed weights need the idle columns of one head tile");
   using C = Tile<D, GT, DEPTH, WARPS>;
   constexpr int NS = C::NS;
   constexpr int MT = C::MT;
@@ -868,6 +872,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
               fm[nt][e] = fmaxf(v, fm[nt][e]);
               fmb[nt][e] = kPExp - fm[nt][e];
               fl[nt][e] *= c[e];
+              if constexpr (PACK) {  // columns 4-7 belong to the heads of columns 0-3
+                const float other = __shfl_xor_sync(0xffffffffu, c[e], 2);
+                if (r >= 2) c[e] = other;
+              }
             }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {  // O's columns are the lane's own heads
@@ -900,10 +908,20 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
             }
             split_f16x2_packed(p[0], p[1], ph0[nt], pl0[nt]);
             split_f16x2_packed(p[2], p[3], ph1[nt], pl1[nt]);
+            if constexpr (PACK) {
+              const uint32_t o0 = __shfl_xor_sync(0xffffffffu, pl0[nt], 2);
+              const uint32_t o1 = __shfl_xor_sync(0xffffffffu, pl1[nt], 2);
+              if (r >= 2) {
+                ph0[nt] = o0;
+                ph1[nt] = o1;
+              }
+            }
             ph0[nt] = transpose8x8(ph0[nt]);
             ph1[nt] = transpose8x8(ph1[nt]);
-            pl0[nt] = transpose8x8(pl0[nt]);
-            pl1[nt] = transpose8x8(pl1[nt]);
+            if constexpr (!PACK) {
+              pl0[nt] = transpose8x8(pl0[nt]);
+              pl1[nt] = transpose8x8(pl1[nt]);
+            }
           }
           // V: tokens 4r .. 4r + 3, values 16g .. 16g + 15 (one block a token). Scales of slots
           // past the context may be anything: zero there (a finite code times zero is 0).
@@ -938,7 +956,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 mma_16816(oacc[i][nt], a0, a1, a2, a3, ph0[nt], ph1[nt]);
-                mma_16816(oacc[i][nt], a0, a1, a2, a3, pl0[nt], pl1[nt]);
+                if constexpr (!PACK)
+                  mma_16816(oacc[i][nt], a0, a1, a2, a3, pl0[nt], pl1[nt]);
               }
             }
           }
@@ -955,6 +974,13 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
 
     {
       // ---- piece epilogue ---------------------------------------------------------------------
+      if constexpr (PACK) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            oacc[i][0][e] += __shfl_xor_sync(0xffffffffu, oacc[i][0][e], 2);
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -1178,13 +1204,13 @@ template <int GT> struct Shape;
 template <> struct Shape<8> { static constexpr int W = 12, DP = 3; };
 template <> struct Shape<16> { static constexpr int W = 8, DP = 4; };
 
-template <int GT>
+template <int GT, bool PACK>
 cudaError_t launch_one(const DecodeFp4Args& a, int grid, cudaStream_t stream) {
   constexpr int W = Shape<GT>::W;
   constexpr int DP = Shape<GT>::DP;
   using C = Tile<128, GT, DP, W>;
   static_assert(C::SMEM + 14 * 1024 <= 227 * 1024, "shared memory of a launch");
-  auto kern = decode_fp4_kernel<128, GT, DP, W>;
+  auto kern = decode_fp4_kernel<128, GT, PACK, DP, W>;
   // The shared-memory opt-in is a per-device function attribute: set it once per device.
   static std::atomic<uint64_t> configured{0};
   int dev = 0;
@@ -1205,7 +1231,11 @@ cudaError_t launch_one(const DecodeFp4Args& a, int grid, cudaStream_t stream) {
 int decode_fp4_warps_per_cta(int gt) { return gt == 8 ? Shape<8>::W : Shape<16>::W; }
 
 cudaError_t launch_decode_fp4(int gt, const DecodeFp4Args& a, int grid, cudaStream_t stream) {
-  return gt == 8 ? launch_one<8>(a, grid, stream) : launch_one<16>(a, grid, stream);
+  if (gt != 8) return launch_one<16, false>(a, grid, stream);
+#ifdef PA_NOPACK
+  return launch_one<8, false>(a, grid, stream);
+#endif
+  return a.G <= 4 ? launch_one<8, true>(a, grid, stream) : launch_one<8, false>(a, grid, stream);
 }
 
 // launch_reduce with bf16 output rows (its checks done).

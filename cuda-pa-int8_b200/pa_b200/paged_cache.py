@@ -6,6 +6,9 @@ methods (prefill, decode_append, context_lens, kv_bytes, kv_bytes_for_len, reset
 reference quantises and scatters with torch ops; here prefill is one block-granular kernel
 (pa_prefill_into_cache) and decode_append one token-granular kernel (pa_quantize_into_cache
 or pa_write_into_cache_f16), with bit-identical cache contents.
+
+A fourth variant, "fp4", has no counterpart there: the 4-bit cache of ops.fp4_cache, 144 bytes a
+token and kv head for K and V against 264 (int8) and 512 (fp16).
 """
 
 import torch
@@ -16,7 +19,7 @@ from . import _lib, ops
 class PagedKVCache:
     def __init__(self, num_layers, num_kv_heads, head_dim, max_len, block_size=16, x=8,
                  variant="fp16", device="cuda"):
-        assert variant in ("fp16", "int8_per_token", "int8_per_tensor")
+        assert variant in ("fp16", "int8_per_token", "int8_per_tensor", "fp4")
         assert head_dim % x == 0
         self.num_layers = num_layers
         self.num_kv_heads = num_kv_heads
@@ -24,15 +27,22 @@ class PagedKVCache:
         self.block_size = block_size
         self.x = x
         self.variant = variant
-        self.is_int8 = variant != "fp16"
+        self.is_int8 = variant.startswith("int8")
+        self.is_fp4 = variant == "fp4"
         self.device = device
 
         self.num_blocks = (max_len + block_size - 1) // block_size
-        store_dtype = torch.int8 if self.is_int8 else torch.float16
-        self.k_cache = torch.zeros(num_layers, self.num_blocks, num_kv_heads, head_dim // x,
-                                   block_size, x, dtype=store_dtype, device=device)
-        self.v_cache = torch.zeros(num_layers, self.num_blocks, num_kv_heads, head_dim,
-                                   block_size, dtype=store_dtype, device=device)
+        if self.is_fp4:
+            assert head_dim == ops.HEAD_DIM
+            self.k_cache, self.v_cache = (
+                c.unflatten(0, (num_layers, self.num_blocks)) for c in ops.fp4_cache(
+                    num_layers * self.num_blocks, num_kv_heads, block_size, device))
+        else:
+            store_dtype = torch.int8 if self.is_int8 else torch.float16
+            self.k_cache = torch.zeros(num_layers, self.num_blocks, num_kv_heads, head_dim // x,
+                                       block_size, x, dtype=store_dtype, device=device)
+            self.v_cache = torch.zeros(num_layers, self.num_blocks, num_kv_heads, head_dim,
+                                       block_size, dtype=store_dtype, device=device)
         if self.is_int8:
             self.k_scales = torch.zeros(num_layers, self.num_blocks, num_kv_heads, block_size,
                                         dtype=torch.float32, device=device)
@@ -56,6 +66,13 @@ class PagedKVCache:
         """Scatter the prompt's K/V [L, num_kv_heads, head_dim] into positions [0, L)."""
         L, H, D = k.shape
         assert H == self.num_kv_heads and D == self.head_dim
+        if self.is_fp4:
+            assert L <= self.num_blocks * self.block_size
+            slots = torch.arange(L, dtype=torch.int32, device=self.device)
+            ops.quantize_into_cache_fp4(k.contiguous(), v.contiguous(), self.k_cache[layer_idx],
+                                        self.v_cache[layer_idx], slots, self.block_size)
+            self.lengths[layer_idx] = L
+            return
         k4 = k.contiguous().view(1, L, H, D)
         v4 = v.contiguous().view(1, L, H, D)
         lens = torch.tensor([L], dtype=torch.int32, device=self.device)
@@ -87,6 +104,9 @@ class PagedKVCache:
             ops.quantize_into_cache(k3, v3, self.k_cache[layer_idx], self.v_cache[layer_idx],
                                     self.k_scales[layer_idx], self.v_scales[layer_idx], slot,
                                     self.block_size, **kw)
+        elif self.is_fp4:
+            ops.quantize_into_cache_fp4(k3, v3, self.k_cache[layer_idx], self.v_cache[layer_idx],
+                                        slot, self.block_size)
         else:
             ops.write_into_cache(k3, v3, self.k_cache[layer_idx], self.v_cache[layer_idx], slot,
                                  self.block_size)
@@ -130,6 +150,9 @@ class PagedKVCache:
 
     def kv_bytes_for_len(self, n):
         blocks = (n + self.block_size - 1) // self.block_size
+        if self.is_fp4:
+            return (blocks * 2 * self.num_kv_heads * self.block_size *
+                    (ops.FP4_GROUP_BYTES // ops.FP4_GROUP_TOKENS) * self.num_layers)
         elem = 1 if self.is_int8 else 2
         per_blk = 2 * self.num_kv_heads * self.head_dim * self.block_size
         b = blocks * per_blk * elem * self.num_layers

@@ -179,3 +179,15 @@ def test_fp4_decode_entry_points_refuse_bad_arguments(lib):
     for bit, word in ((_lib.PA_ERR_FREE_BLOCKS, b"free"), (_lib.PA_ERR_TOKENS, b"max_tokens"),
                       (_lib.PA_ERR_POSITION, b"position")):
         assert word in lib.pa_status_string(bit)
+
+
+def test_paged_cache_variant():
+    from pa_b200.paged_cache import PagedKVCache
+    c = PagedKVCache(3, 2, 128, 50, 16, variant="fp4", device="cpu")
+    assert tuple(c.k_cache.shape) == tuple(c.v_cache.shape) == (3, 4, 2, 1, 1152)
+    assert c.kv_bytes() == 3 * 64 * 2 * 2 * 72 and not c.is_int8
+    assert c.kv_bytes_for_len(17) == 3 * 32 * 2 * 2 * 72
+    with pytest.raises(AssertionError):
+        PagedKVCache(1, 2, 64, 50, 16, variant="fp4", device="cpu")
+    with pytest.raises(AssertionError):
+        PagedKVCache(1, 2, 128, 50, 16, variant="int4", device="cpu")

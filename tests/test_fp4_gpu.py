@@ -415,3 +415,35 @@ def test_bf16_values_outside_the_fp16_range_are_flagged():
     q[1, 5, 77] = 1e6
     _ops().decode_bf16(out, q, kc, vc, bt, cl, scale_for())
     assert _ops().read_status(q.device) == 512  # PA_ERR_Q_RANGE
+
+
+def test_paged_cache_loop():
+    """PagedKVCache("fp4") over two layers: a prompt, then tokens appended and decoded."""
+    from pa_b200.paged_cache import PagedKVCache
+    rng = np.random.default_rng(19)
+    cache = PagedKVCache(2, 2, 128, 60, 16, variant="fp4")
+    held = [[np.zeros((0, 2, 128))] * 2 for _ in range(2)]
+    for step in range(6):
+        n = 37 if step == 0 else 1
+        for layer in range(2):
+            k, kd = _rows(rng, n, 2, torch.float16)
+            v, vd = _rows(rng, n, 2, torch.float16)
+            held[layer] = [np.concatenate([h, x]) for h, x in zip(held[layer], (kd, vd))]
+            L = 37 + step
+            q = torch.from_numpy(rng.standard_normal((1, 12, 128)).astype(np.float16))
+            if step == 0:
+                cache.prefill(layer, k.cuda(), v.cuda())
+                continue
+            if step % 2:
+                out = cache.append_and_decode(layer, k[0].cuda(), v[0].cuda(), q.cuda(), scale_for())
+            else:
+                assert cache.decode_append(layer, k[0].cuda(), v[0].cuda()) == L
+                out = torch.empty(1, 12, 128, dtype=torch.float16, device="cuda")
+                _ops().decode(out, q.cuda(), cache.k_cache[layer], cache.v_cache[layer],
+                              cache.block_table, cache.context_lens(layer), scale_for())
+            caches = [np.zeros((4, 2, 1, 1152), np.uint8) for _ in "kv"]
+            for c, rows, is_v in zip(caches, held[layer], (False, True)):
+                pa_oracle.fp4_put(c, is_v, rows, np.arange(L), 16)
+            _close(out, dict(q=q, kc=caches[0], vc=caches[1], lens=np.array([L]),
+                             bt=np.arange(4)[None]))
+    _ops().check_status(cache.k_cache.device)
