@@ -32,6 +32,7 @@
 #include "pa_rows.cuh"
 
 #include <atomic>
+#include <type_traits>
 
 namespace pa {
 namespace {
@@ -560,7 +561,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
   locate((int)p0, cb, cseg, csp);
   int cpg = pages_of(cb);
   int cctx = s_ctx[cb];
-  const float qs = a.qk_scale_log2;
+  // Scores are taken times |scale| log2 e; a negative scale turns q's signs. (A zero scale becomes
+  // one whose scores vanish against each other all the same.)
+  const float qs = fmaxf(fabsf(a.qk_scale_log2), 1e-30f);
+  const uint32_t qsign = a.qk_scale_log2 < 0.f ? 0x80008000u : 0u;
 
   // Q as the B fragments of the QK MMA (fp16): values 32r .. 32r + 31 of head g (qa) and, with 16
   // heads to a tile, of head g + 8 (qb).
@@ -604,10 +608,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
     return make_uint4(dst[0], dst[1], dst[2], dst[3]);
   };
   auto convert_q = [&]() {
+    auto turn = [&](uint4 v) {
+      if (a.act_bf16) v = bf16_to_f16(v);
+      return make_uint4(v.x ^ qsign, v.y ^ qsign, v.z ^ qsign, v.w ^ qsign);
+    };
 #pragma unroll
     for (int si = 0; si < NS; ++si) {
-      qa[si] = a.act_bf16 ? bf16_to_f16(ra[si]) : ra[si];
-      if constexpr (NT == 2) qb[si] = a.act_bf16 ? bf16_to_f16(rb[si]) : rb[si];
+      qa[si] = turn(ra[si]);
+      if constexpr (NT == 2) qb[si] = turn(rb[si]);
     }
   };
   // The first piece's q rows are requested before the page copies, so their latency overlaps
@@ -672,6 +680,20 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
   const uint8_t* rest_lane = ((lane & 16) ? a.v_cache : a.k_cache) + 1024 + 16 * (lane & 7);
   const uint32_t rest_off =
       (uint32_t)(lane >> 3) * (uint32_t)C::PT + 1024u + 16u * (uint32_t)(lane & 7);
+  auto copy_pair = [&](uint32_t g0, uint32_t g1, int s) {
+    const uint32_t st = my_ring + (uint32_t)s * (uint32_t)C::STAGE;
+    const uint32_t sl = st + 16u * (uint32_t)lane;
+    const size_t o0 = (size_t)g0 * C::PT, o1 = (size_t)g1 * C::PT;
+    cp_async_16_hint(sl, k_lane + o0, pol);
+    cp_async_16_hint(sl + 512, k_lane + o0 + 512, pol);
+    cp_async_16_hint(sl + C::PT, k_lane + o1, pol);
+    cp_async_16_hint(sl + C::PT + 512, k_lane + o1 + 512, pol);
+    cp_async_16_hint(sl + 2 * C::PT, v_lane + o0, pol);
+    cp_async_16_hint(sl + 2 * C::PT + 512, v_lane + o0 + 512, pol);
+    cp_async_16_hint(sl + 3 * C::PT, v_lane + o1, pol);
+    cp_async_16_hint(sl + 3 * C::PT + 512, v_lane + o1 + 512, pol);
+    cp_async_16_hint(st + rest_off, rest_lane + (size_t)((lane & 8) ? g1 : g0) * C::PT, pol);
+  };
   // Pages jj and jj + 1 (jj even; asked for in order) into stage s; past the range's end the
   // group is empty, and a missing second page is the first once more. The ids of the next 32
   // pages come along with a batch's first stage, sixteen groups before they are needed.
@@ -700,18 +722,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
         write_new(g0, __shfl_sync(0xffffffffu, curw, jj & 31));
         write_new(g1, __shfl_sync(0xffffffffu, curw, i1));
       }
-      const uint32_t st = my_ring + (uint32_t)s * (uint32_t)C::STAGE;
-      const uint32_t sl = st + 16u * (uint32_t)lane;
-      const size_t o0 = (size_t)g0 * C::PT, o1 = (size_t)g1 * C::PT;
-      cp_async_16_hint(sl, k_lane + o0, pol);
-      cp_async_16_hint(sl + 512, k_lane + o0 + 512, pol);
-      cp_async_16_hint(sl + C::PT, k_lane + o1, pol);
-      cp_async_16_hint(sl + C::PT + 512, k_lane + o1 + 512, pol);
-      cp_async_16_hint(sl + 2 * C::PT, v_lane + o0, pol);
-      cp_async_16_hint(sl + 2 * C::PT + 512, v_lane + o0 + 512, pol);
-      cp_async_16_hint(sl + 3 * C::PT, v_lane + o1, pol);
-      cp_async_16_hint(sl + 3 * C::PT + 512, v_lane + o1 + 512, pol);
-      cp_async_16_hint(st + rest_off, rest_lane + (size_t)((lane & 8) ? g1 : g0) * C::PT, pol);
+      copy_pair(g0, g1, s);
     }
     cp_async_commit();
   };
@@ -719,8 +730,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
   for (int j = 0; j < DEPTH; ++j) issue_pair(2 * j, j);
   convert_q();
 
-  // Running maximum and sum of heads nt * 8 + 2r and the next; fmb = kPExp - fm.
-  float fm[NT][2], fl[NT][2], fmb[NT][2];
+  // Of heads nt * 8 + 2r and the next: the reference maximum m (a whole number, so that rescaling
+  // by a change of it is exact) as fmb = kPExp - m, the score at which it moves, and the sum.
+  float fmb[NT][2], thr[NT][2], fl[NT][2];
   float oacc[MT][NT][4];
   const int tau = 4 * (g >> 1) + (g & 1);  // token of K row g (row g + 8: + 2)
 
@@ -760,28 +772,19 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
 #pragma unroll
         for (int e = 0; e < 4; ++e) oacc[i][nt][e] = 0.f;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          fm[nt][e] = neg_inf();
-          fmb[nt][e] = -neg_inf();
-          fl[nt][e] = 0.f;
-        }
-      // A stage's two pages per step; where a piece begins or ends inside a stage, the page that
-      // is not its own is masked (and met again by the other piece).
-      for (int k = 0; k < len;) {
-        const int first = j & 1;
-        const int cnt = min(2 - first, len - k);
-        if (first == 0) {  // the stage's copies: this lane's, then every lane's
-          cp_async_wait_groups<DEPTH - 1>();
-          __syncwarp();
-        }
-        const int left = cctx - (csp + k) * kSubTokens;  // tokens from the step's first page on
-        const int valid0 = first ? 0 : min(kSubTokens, left);
-        const int valid1 = first ? min(kSubTokens, left)
-                                 : (cnt == 2 ? min(kSubTokens, left - kSubTokens) : 0);
-        const bool full = valid0 == kSubTokens && valid1 == kSubTokens;
-        const uint32_t st = my_ring + (uint32_t)s * (uint32_t)C::STAGE;
+      for (int e = 0; e < 2; ++e) {
+        fmb[nt][e] = -neg_inf();
+        thr[nt][e] = neg_inf();
+        fl[nt][e] = 0.f;
+      }
+    // One step: the two pages of stage s. FULL: all their tokens count; else valid0 and valid1 of
+    // them do (where a piece begins or ends inside a stage, the page that is not its own has
+    // none, and is met again by the other piece).
+    auto step = [&](auto full, int s, int valid0, int valid1) {
+      constexpr bool FULL = decltype(full)::value;
+      const uint32_t st = my_ring + (uint32_t)s * (uint32_t)C::STAGE;
         const uint32_t ka = st + tau * fp4::kCodeRow + 16 * r;
         const uint32_t ksa = st + fp4::kCodes + tau * 8 + 2 * r;
         const uint32_t va = st + 2 * C::PT + 4 * r * fp4::kCodeRow + 8 * g;
@@ -822,19 +825,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
               mma(si == 0, acc[1][1], h[2], i4[2], h[3], i4[3], qb[si].z, qb[si].w);
             }
           }
-          // Logits in log2 units: heads nt * 8 + 2r + (e & 1) of token tau (e < 2) and tau + 2.
+          // Raw scores: heads nt * 8 + 2r + (e & 1) of token tau (e < 2) and tau + 2.
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; e += 2) {
-              const float2 v = mul2(add2(make_float2(acc[0][nt][e], acc[0][nt][e + 1]),
-                                         make_float2(acc[1][nt][e], acc[1][nt][e + 1])),
-                                    make_float2(qs, qs));
+              const float2 v = add2(make_float2(acc[0][nt][e], acc[0][nt][e + 1]),
+                                    make_float2(acc[1][nt][e], acc[1][nt][e + 1]));
               x[u][nt][e] = v.x;
               x[u][nt][e + 1] = v.y;
             }
         }
-        if (!full) {
+        if constexpr (!FULL) {
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int vd = u ? valid1 : valid0;
@@ -857,7 +859,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
           for (int e = 0; e < 2; ++e) {
             tm[nt][e] = fmaxf(fmaxf(x[0][nt][e], x[0][nt][2 + e]),
                               fmaxf(x[1][nt][e], x[1][nt][2 + e]));
-            up = up || tm[nt][e] > fm[nt][e] + kLazy;
+            up = up || tm[nt][e] > thr[nt][e];
           }
         if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
@@ -868,9 +870,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
               float v = tm[nt][e];
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-              c[e] = v > fm[nt][e] ? ex2(fm[nt][e] - v) : 1.f;
-              fm[nt][e] = fmaxf(v, fm[nt][e]);
-              fmb[nt][e] = kPExp - fm[nt][e];
+              const float m = kPExp - fmb[nt][e], mn = fmaxf(m, ceilf(v * qs));
+              c[e] = mn > m ? ex2(m - mn) : 1.f;
+              fmb[nt][e] = kPExp - mn;
+              thr[nt][e] = __fdividef(mn + kLazy, qs);
               fl[nt][e] *= c[e];
               if constexpr (PACK) {  // columns 4-7 belong to the heads of columns 0-3
                 const float other = __shfl_xor_sync(0xffffffffu, c[e], 2);
@@ -897,8 +900,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
             float p[4];
 #pragma unroll
             for (int e = 0; e < 4; e += 2) {
-              const float2 v = add2(make_float2(x[u][nt][e], x[u][nt][e + 1]),
-                                    make_float2(fmb[nt][0], fmb[nt][1]));
+              const float2 v = fma2(make_float2(x[u][nt][e], x[u][nt][e + 1]),
+                                    make_float2(qs, qs), make_float2(fmb[nt][0], fmb[nt][1]));
               p[e] = ex2(v.x);
               p[e + 1] = ex2(v.y);
               const float2 l = add2(make_float2(fl[nt][0], fl[nt][1]),
@@ -930,7 +933,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
           for (int e = 0; e < 4; ++e) vq[e] = lds64(va + u * C::PT + e * fp4::kCodeRow);
           const uint32_t z = lds32(vsa + u * C::PT);
           uint32_t s01 = fp4::scale_pair(z), s23 = fp4::scale_pair(z, 0x3424u);
-          if (!full) {
+          if constexpr (!FULL) {
             const int vd = u ? valid1 : valid0;
             s01 &= ((4 * r < vd) ? 0x0000ffffu : 0u) | ((4 * r + 1 < vd) ? 0xffff0000u : 0u);
             s23 &= ((4 * r + 2 < vd) ? 0x0000ffffu : 0u) | ((4 * r + 3 < vd) ? 0xffff0000u : 0u);
@@ -962,14 +965,45 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
             }
           }
         }
-        k += cnt;
-        j += cnt;
-        if ((j & 1) == 0) {  // both pages of the stage are done with: refill it
+    };
+    for (int k = 0; k < len;) {
+      const int first = j & 1;
+      // Steps with nothing to check: full pages whose refill lies inside the range and inside the
+      // present batch of block ids.
+      if (first == 0 && !step_write) {
+        const int jr = j + 2 * DEPTH;  // the next refill's first page
+        int m = min(len - k, (cctx - (csp + k) * kSubTokens) / kSubTokens) / 2;
+        m = min(min(m, (n - jr) / 2), (-jr & 31) / 2);
+        for (int i = 0; i < m; ++i) {
+          cp_async_wait_groups<DEPTH - 1>();
           __syncwarp();
-          issue_pair(j + 2 * DEPTH - 2, s);
+          step(std::true_type{}, s, kSubTokens, kSubTokens);
+          __syncwarp();
+          const int e = (j + 2 * DEPTH) & 31;
+          copy_pair(__shfl_sync(0xffffffffu, cur, e), __shfl_sync(0xffffffffu, cur, e + 1), s);
+          cp_async_commit();
           if (++s == DEPTH) s = 0;
+          k += 2;
+          j += 2;
         }
+        if (k >= len) break;
       }
+      const int cnt = min(2 - first, len - k);
+      if (first == 0) {  // the stage's copies: this lane's, then every lane's
+        cp_async_wait_groups<DEPTH - 1>();
+        __syncwarp();
+      }
+      const int left = cctx - (csp + k) * kSubTokens;  // tokens from the step's first page on
+      step(std::false_type{}, s, first ? 0 : min(kSubTokens, left),
+           first ? min(kSubTokens, left) : (cnt == 2 ? min(kSubTokens, left - kSubTokens) : 0));
+      k += cnt;
+      j += cnt;
+      if ((j & 1) == 0) {  // both pages of the stage are done with: refill it
+        __syncwarp();
+        issue_pair(j + 2 * DEPTH - 2, s);
+        if (++s == DEPTH) s = 0;
+      }
+    }
     csp += len;
 
     {
@@ -1011,7 +1045,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             *reinterpret_cast<float2*>(slot + D * GT + nt * 8 + 2 * r) =
-                make_float2(fm[nt][0], fm[nt][1]);
+                make_float2(kPExp - fmb[nt][0], kPExp - fmb[nt][1]);
             *reinterpret_cast<float2*>(slot + D * GT + GT + nt * 8 + 2 * r) =
                 make_float2(fl[nt][0] * kUnscale, fl[nt][1] * kUnscale);
           }
