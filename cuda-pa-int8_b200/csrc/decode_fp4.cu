@@ -17,14 +17,17 @@
 //    reduction over the lanes and no rescale;
 //  * weights enter PV as two fp16 parts, as in decode.cu: one rounding to fp16 would add as much
 //    error as the output's own.
-// 302 warp instructions a page (479 with decode.cu's loop): 64 conversions, 64 multiplies, 24
+//  * steps of two full pages run in a loop with nothing to check; a step's scale and maximum are
+//    one multiply-add before the exponential (raw scores are compared with a threshold).
+// 277 warp instructions a page (479 with decode.cu's loop): 64 conversions, 64 multiplies, 24
 // MMAs, 16 to pair the codes of neighbouring tokens for PV, the rest softmax, copies and loop.
-// Measured on a B200 (graph replay): 64 x 8192 tokens, 12/2 heads 47 us (3.2 TB/s); 8 x 64-128 K,
-// 64/8 heads 193 us (4.7 TB/s, 0.72 of the measured copy bandwidth). Conversions, fp16 multiplies
-// and MMAs hardly overlap on a scheduler (a group of one MMA and three of each takes 18.6 cycles
-// where the MMA alone takes 8 and the others 8), which is about 420 of the loop's 510 cycles a
-// page and scheduler; warps of 16 a CTA (128 registers) and the QK of the next step issued
-// between the PV of this one measured no better.
+// Measured on a B200 (graph replay): 64 x 8192 tokens, 12/2 heads 45.2 us (3.35 TB/s); 8 x 64-128
+// K, 64/8 heads 175.5 us (5.16 TB/s, 0.79 of the measured copy bandwidth). The loop takes 467
+// cycles a page and scheduler, of which the ALU pipe (conversions, logic) is busy for 255, the
+// tensor pipe for 192 and the multiplies for 180; the three hardly overlap (a group of one MMA
+// and three of each takes 18.6 cycles where the MMA alone takes 8 and the others 8). Warps of 16 a
+// CTA (128 registers), the QK of the next step issued between the PV of this one, and a choice of
+// refill inside one loop for all full pages measured no better.
 
 #include "fp4.cuh"
 #include "pa_common.cuh"
