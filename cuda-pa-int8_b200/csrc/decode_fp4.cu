@@ -1239,8 +1239,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
 }
 
 // Warps per CTA and ring stages per warp, by head tile (16 heads keep twice the accumulators).
-// Twelve warps: 168 registers. 64 x 8192 / 8 x 64-128 K tokens: 47.2 / 192.8 us with three stages,
-// 50.7 / 192.3 with two, 49.1 / 212.9 with eight warps, 51.4 / 196.1 with sixteen.
+// Twelve warps: 168 registers, three to a scheduler. 64 x 8192 / 8 x 64-128 K tokens: 45.3 / 176.1
+// us with three stages, 48.2 / 175.4 with two; eight warps (four stages) 45.2 / 185.9, ten (four)
+// 49.3 / 207.2, fourteen (three) 52.7 / 209.7, sixteen (two) 49.3 / 180.4.
 template <int GT> struct Shape;
 template <> struct Shape<8> { static constexpr int W = 12, DP = 3; };
 template <> struct Shape<16> { static constexpr int W = 8, DP = 4; };
