@@ -209,7 +209,7 @@ int check_common(int B, int H, int KVH, int D, int NB, int bs, int max_blocks) {
                 "num_blocks * num_kv_heads = %lld page rows; this build addresses fewer than "
                 "2^28",
                 (long long)NB * KVH);
-  if (bs % 16 != 0 || 128 % bs != 0)
+  if (bs <= 0 || bs % 16 != 0 || 128 % bs != 0)
     return fail(PA_ERR_INVALID_ARG,
                 "block_size must divide TILE (multiple of 16); got %d (supported: 16, 32, 64, "
                 "128)",
@@ -282,7 +282,7 @@ int decode_impl(int mode, int kv_i8, void* out, float* part_out, const void* q,
     return fail(PA_ERR_INVALID_ARG, "null pointer argument");
   if (mode == pa::kModePartial ? part_out == nullptr : out == nullptr)
     return fail(PA_ERR_INVALID_ARG, "null output pointer");
-  const bool fp4 = kv_i8 == 3;  // scales inside the cache, untiled bulk copies: no tensor maps
+  const bool fp4 = kv_i8 == 3;  // scales inside the cache; copied without tensor maps
   const bool scaled = kv_i8 != 0 && !fp4;
   if (scaled && (k_scales == nullptr || v_scales == nullptr))
     return fail(PA_ERR_INVALID_ARG, "int8 cache needs k_scales and v_scales");
@@ -1065,7 +1065,8 @@ int pa_extend_block_tables(int32_t* block_table, const int32_t* context_lens,
   if (num_blocks <= 0 || max_tokens < 0) return fail(PA_ERR_INVALID_ARG, "invalid sizes");
   if ((long long)num_blocks * block_size > 0x80000000LL)
     return fail(PA_ERR_UNSUPPORTED, "num_blocks * block_size must be at most 2^31 slots");
-  if (query_start == nullptr || (max_tokens > 0 && (slot_mapping == nullptr || positions == nullptr)))
+  if (query_start == nullptr ||
+      (max_tokens > 0 && (slot_mapping == nullptr || positions == nullptr)))
     return fail(PA_ERR_INVALID_ARG, "null pointer argument");
   a.status = status;
   cudaError_t e = pa::launch_extend(a, static_cast<cudaStream_t>(stream));

@@ -585,7 +585,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
       ra[si] = (hl < a.G) ? __ldg(reinterpret_cast<const uint4*>(qrow) + si)
                           : make_uint4(0u, 0u, 0u, 0u);
       rb[si] = make_uint4(0u, 0u, 0u, 0u);
-      if (GT == 16 && hl + 8 < a.G) rb[si] = __ldg(reinterpret_cast<const uint4*>(qrow + 8 * D) + si);
+      if (GT == 16 && hl + 8 < a.G)
+        rb[si] = __ldg(reinterpret_cast<const uint4*>(qrow + 8 * D) + si);
     }
   };
   // Eight bf16 values as fp16: exact inside the fp16 normal range; larger magnitudes saturate and
@@ -670,7 +671,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
     store_new_token_fp4<D>(static_cast<const uint8_t*>(a.new_k) + so,
                            static_cast<const uint8_t*>(a.new_v) + so, a.new_dtype, a.k_write,
                            a.v_write, row, (s_ctx[wb] - 1) % a.bs, a.bs, lane);
-    __threadfence();  // the copies read what the warp has just written, from L2
+    __threadfence();  // the copies read what the warp's lanes have just written, from L2
+    __syncwarp();
   };
   // The warp's ring is filled by 16-byte asynchronous copies of all its lanes, one commit group
   // per stage of two pages. (Four bulk copies per stage, issued by one lane, cost 87 of the step's
@@ -1222,16 +1224,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
       auto piece = [&](int k) -> const float* {
         return a.part + ((size_t)(wf + k) * 2 + (k == 0 ? 1 : 0)) * SLOT;
       };
-      if (stream && a.act_bf16) {
-        coop_combine<D, GT, NTHR, 8, true>(piece, np, hcnt,
-                                         a.out + ((size_t)b * a.H + hbase) * D, nullptr,
-                                         a.status, scratch);
-      } else if (stream) {
-        coop_combine<D, GT, NTHR, 8, false>(piece, np, hcnt, a.out + ((size_t)b * a.H + hbase) * D,
-                                     nullptr, a.status, scratch);
+      __half* orow = stream ? a.out + ((size_t)b * a.H + hbase) * D : nullptr;
+      float* oslot = stream ? nullptr : a.part_out + (size_t)segid * SLOT;
+      if (a.act_bf16) {
+        coop_combine<D, GT, NTHR, 8, true>(piece, np, hcnt, orow, oslot, a.status, scratch);
       } else {
-        coop_combine<D, GT, NTHR, 8, false>(piece, np, hcnt, nullptr,
-                                     a.part_out + (size_t)segid * SLOT, a.status, scratch);
+        coop_combine<D, GT, NTHR, 8, false>(piece, np, hcnt, orow, oslot, a.status, scratch);
       }
       if (threadIdx.x == 0) a.counters[segid] = 0;
     }

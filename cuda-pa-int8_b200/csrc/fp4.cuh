@@ -1,5 +1,5 @@
 // The 4-bit K/V cache format: device helpers shared by its writes and reads (fp4.cu), the
-// norm-and-rotation kernel (rope.cu) and the decode kernel (decode.cu).
+// norm-and-rotation kernel (rope.cu) and the decode kernel (decode_fp4.cu).
 //
 // A value is code * scale. Codes are e2m1 (sign, two exponent bits, one mantissa bit: 0, .5, 1,
 // 1.5, 2, 3, 4, 6); sixteen neighbouring head_dim values of a row share one scale byte, an
@@ -20,7 +20,7 @@
 //   group: codes [16 tokens][64 bytes], byte j = head_dim 2j (low half) and 2j + 1 (high half);
 //          scales: K [16 tokens][8], V [8][16 tokens].
 // A token owns whole bytes (no two tokens share one), so tokens of a group are written
-// independently. One group is one bulk copy for the decode kernel. The code rows are what a
+// independently. A group is one contiguous copy for the decode kernel. The code rows are what a
 // lane of the QK MMA reads as 16 bytes; the V scales' order lets a lane of the PV MMA read its
 // four tokens' scales as one word.
 #pragma once

@@ -721,12 +721,14 @@ def quantize_into_cache_fp4(key, value, k_cache, v_cache, slot_mapping, block_si
     dev, dt = key.device, key.dtype
     if not (key.is_cuda and dt in _DTYPE_CODE and value.dtype == dt and value.device == dev):
         raise RuntimeError("key/value must both be fp16, bf16 or fp32, on one CUDA device")
-    shape, stride = key.shape, key.stride()
+    shape, stride, vstride = key.shape, key.stride(), value.stride()
     if not (len(shape) == 3 and value.shape == shape and shape[2] == HEAD_DIM):
         raise RuntimeError("key/value must be [num_tokens, num_kv_heads, 128]")
     N, KVH, D = shape
-    if not (stride[2] == 1 and stride[1] == D and value.stride() == stride):
-        raise RuntimeError("key/value rows must be contiguous")
+    if not (stride[2] == 1 == vstride[2] and
+            (KVH == 1 or stride[1] == D == vstride[1]) and
+            (N == 1 or stride[0] == vstride[0])):
+        raise RuntimeError("key/value rows must be contiguous per token, with one token stride")
     _check_slots(slot_mapping, N, dev)
     NB, kvh = _check_fp4_caches(k_cache, v_cache, block_size)
     if kvh != KVH:
@@ -734,8 +736,9 @@ def quantize_into_cache_fp4(key, value, k_cache, v_cache, slot_mapping, block_si
     _check_on(dev, k_cache, v_cache)
     with _Guard(dev):
         rc = _lib.lib().pa_quantize_into_cache_fp4(
-            key.data_ptr(), value.data_ptr(), _DTYPE_CODE[dt], stride[0],
-            slot_mapping.data_ptr(), N, KVH, D, k_cache.data_ptr(), v_cache.data_ptr(), NB,
+            key.data_ptr(), value.data_ptr(), _DTYPE_CODE[dt],
+            stride[0] if N > 1 else KVH * D, slot_mapping.data_ptr(), N, KVH, D,
+            k_cache.data_ptr(), v_cache.data_ptr(), NB,
             block_size, workspace(dev, 256).data_ptr(), _stream(dev))
         _lib.check(rc, "quantize_into_cache (fp4)")
 
@@ -869,8 +872,9 @@ def norm_rope_into_cache(q, k, v, q_weight, k_weight, positions, table, k_cache,
     slot_mapping, in one launch: bit for bit what qk_norm_rope followed by the cache's write
     (write_into_cache, quantize_into_cache with per-token scales, or quantize_into_cache_fp4)
     gives. The cache is fp16, int8 or float8_e4m3fn (with k_scales and v_scales), or 4-bit (with
-    rot_dim a multiple of 32 unless interleaved). A negative slot writes nothing to the cache, a negative position skips the token. Returns
-    q_out [num_tokens, heads, 128]; it may be q."""
+    rot_dim a multiple of 32 unless interleaved). A negative slot writes nothing to the cache, a
+    negative position skips the token; slots of one call have to differ. Returns q_out
+    [num_tokens, heads, 128]; it may be q."""
     N, H, qs, KVH, ks = _check_norm_rope(q, k, q_weight, k_weight, positions, table, eps)
     dev, dt = q.device, q.dtype
     _, vs = _head_rows("v", v, N, KVH, dt, dev)

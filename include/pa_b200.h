@@ -297,16 +297,17 @@ int pa_quantize_into_cache_fp8(const void* k, const void* v, int in_dtype, int64
  *   scale = the nearest scale byte's value to amax / 6, ties to even, at most 10240
  *   code  = the nearest e2m1 to x / scale, ties to the even code, magnitudes above 6 as 6
  * (a zero may carry either sign). A block with a zero scale holds zeros; one with a NaN or an
- * infinity gets a NaN scale and reads as NaN. No counterpart in the reference. */
+ * infinity gets a NaN scale and reads as NaN. Slots of one call have to differ: two rows of one
+ * slot leave a mixture of their blocks. No counterpart in the reference. */
 int pa_quantize_into_cache_fp4(const void* k, const void* v, int in_dtype, int64_t token_stride,
                                const int32_t* slot_mapping, int num_tokens, int num_kv_heads,
                                int head_dim, void* k_cache, void* v_cache, int num_blocks,
                                int block_size, int* status, void* stream);
 
 /* Rows read back from an fp4 cache (for instance a cached prefix, for the attention of a prompt's
- * next chunk): k_out, v_out [num_tokens, num_kv_heads, head_dim] in out_dtype (F16, BF16 or F32; held
- * values are exact in each). Rows of tokens with a negative slot are left as they are; so are
- * rows of slots outside the cache, which set PA_ERR_SLOT. */
+ * next chunk): k_out, v_out [num_tokens, num_kv_heads, head_dim] in out_dtype (F16, BF16 or F32;
+ * held values are exact in each). Rows of tokens with a negative slot are left as they are; so
+ * are rows of slots outside the cache, which set PA_ERR_SLOT. */
 int pa_read_from_cache_fp4(void* k_out, void* v_out, int out_dtype, const void* k_cache,
                            const void* v_cache, const int32_t* slot_mapping, int num_tokens,
                            int num_kv_heads, int head_dim, int num_blocks, int block_size,
@@ -332,8 +333,8 @@ int pa_qk_norm_rope(void* q_out, int64_t q_out_stride, void* k_out, int64_t k_ou
                     int interleaved, int num_tokens, int num_heads, int num_kv_heads,
                     int head_dim, int* status, void* stream);
 
-/* The same, with the new K rows and the V rows written into the paged cache at slot_mapping instead of
- * k_out: cache_dtype F16, I8 (per-token scales), FP8E4M3 or FP4E2M1, bit for bit what
+/* The same, with the new K rows and the V rows written into the paged cache at slot_mapping
+ * instead of k_out: cache_dtype F16, I8 (per-token scales), FP8E4M3 or FP4E2M1, bit for bit what
  * pa_qk_norm_rope followed by that cache's write gives, in one launch. A negative slot writes
  * nothing to the cache (q_out is still written). For an fp4 cache rot_dim is a multiple of 32
  * unless interleaved. */

@@ -191,3 +191,10 @@ def test_paged_cache_variant():
         PagedKVCache(1, 2, 64, 50, 16, variant="fp4", device="cpu")
     with pytest.raises(AssertionError):
         PagedKVCache(1, 2, 128, 50, 16, variant="int4", device="cpu")
+
+
+def test_decodes_refuse_an_empty_block_size(lib):
+    for fn in (lib.pa_decode_fp4, lib.pa_splitk_fp4, lib.pa_decode_f16):
+        for bs in (0, -16):
+            assert fn(P, P, P, P, P, P, 1, 8, 2, 128, 4, bs, 2, 0.1, P, 1 << 30,
+                      None) == _lib.PA_ERR_INVALID_ARG

@@ -447,3 +447,70 @@ def test_paged_cache_loop():
             _close(out, dict(q=q, kc=caches[0], vc=caches[1], lens=np.array([L]),
                              bt=np.arange(4)[None]))
     _ops().check_status(cache.k_cache.device)
+
+
+@pytest.mark.parametrize("scale", [-0.11, 0.0, 1e-38, 1.0, 3.0])
+@pytest.mark.parametrize("H,KVH", [(12, 2), (8, 4), (32, 2)])
+def test_scales_of_either_sign(scale, H, KVH):
+    """A negative scale is a positive one over -q, for the 64-bit form as well."""
+    c = _case(20, [1, 30, 1700], H, KVH, pad=0xFF)
+    q, kc, vc, bt, cl = _gpu(c)
+    sign = -1.0 if scale < 0 else 1.0
+    ref, qk, vmax = pa_oracle.fp4_decode(sign * c["q"].double().numpy(), c["kc"], c["vc"], c["bt"],
+                                         c["lens"], abs(scale))
+    e = 2 * (2.0 ** -17 * qk + 2.0 ** -20) + c["lens"] / 16 * 2.0 ** -22
+    tol = 2.0 ** -11 * np.abs(ref) + 2.0 ** -25 + (e * vmax)[:, None, None]
+    for splitk in (False, True):
+        out = torch.full_like(q, float("nan"))
+        _ops().decode(out, q, kc, vc, bt, cl, scale, splitk=splitk)
+        assert (np.abs(out.double().cpu().numpy() - ref) <= tol).all()
+
+
+def test_one_token_of_any_strides():
+    """A single token's strides between tokens (and one head's between heads) do not matter."""
+    rng = np.random.default_rng(21)
+    qkv = torch.from_numpy(rng.standard_normal((1, 8, 128)).astype(np.float16)).cuda()
+    for kvh in (2, 1):
+        k, v = qkv[:, 4:4 + kvh], torch.empty(1, kvh, 128, dtype=torch.float16, device="cuda")
+        v.copy_(qkv[:, 6:6 + kvh])
+        k = k.as_strided(k.shape, (k.stride(0), 1024 if kvh == 1 else 128, 1), k.storage_offset())
+        kc, vc = _ops().fp4_cache(1, kvh)
+        sl = torch.tensor([5], dtype=torch.int32, device="cuda")
+        _ops().quantize_into_cache_fp4(k, v, kc, vc, sl)
+        for cache, rows, is_v in ((kc, k, False), (vc, v, True)):
+            want = _want(rows.double().cpu().numpy(), cache, is_v, [5], 16)
+            assert np.array_equal(_held(cache, is_v), want)
+
+
+def test_partials_of_empty_contexts_merge():
+    """A rank without tokens of a sequence gives an empty partial."""
+    c = _case(22, [40, 7, 900], 28, 4)
+    q, kc, vc, bt, cl = _gpu(c)
+    part = _ops().decode_partial(q, kc, vc, bt, cl, scale_for())
+    gone = torch.tensor([0, 1, 0], dtype=torch.int32, device="cuda") * 0
+    empty = _ops().decode_partial(q, kc, vc, bt, gone, scale_for())
+    out = torch.empty_like(q)
+    _ops().merge_partials(out, torch.stack([empty, part, empty]), 28, 4)
+    _close(out, c)
+    _ops().check_status(q.device)
+
+
+def test_two_batches_on_two_streams():
+    cs = [_case(23 + i, [3000, 1, 77 + 900 * i], 12, 2) for i in range(2)]
+    ts = [_gpu(c) for c in cs]
+    want = []
+    for q, kc, vc, bt, cl in ts:
+        want.append(torch.empty_like(q))
+        _ops().decode(want[-1], q, kc, vc, bt, cl, scale_for())
+    outs = [torch.empty_like(t[0]) for t in ts]
+    streams = [torch.cuda.Stream() for _ in ts]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, o, (q, kc, vc, bt, cl), c in zip(streams, outs, ts, cs):
+            with torch.cuda.stream(s):
+                _ops().decode(o, q, kc, vc, bt, cl, scale_for(),
+                              host_context_lens=torch.from_numpy(c["lens"]))
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        assert torch.equal(o, w)
+    _ops().check_status(outs[0].device)

@@ -245,3 +245,67 @@ def test_serving_steps_through_all_the_calls():
         e = 2 * (2.0 ** -17 * qk + 2.0 ** -20) + lens.cpu().numpy() / 16 * 2.0 ** -22
         tol = 2.0 ** -11 * np.abs(ref) + 2.0 ** -25 + (e * vmax)[:, None, None]
         assert (np.abs(out.double().cpu().numpy() - ref) <= tol).all()
+
+
+def test_a_captured_step_equals_the_eager_calls():
+    """One graph of release, extend, norm and rotation into the cache and decode, replayed with
+    new lengths and rows, against the same calls made one by one: every byte alike."""
+    ops = _ops()
+    S, H, KVH, bs, MB, NB, T = 5, 12, 2, 16, 8, 34, 24
+    rope = ops.rope_table(256)
+    rng = np.random.default_rng(8)
+    perm = rng.permutation(NB)
+
+    def state():
+        kc, vc = ops.fp4_cache(NB, KVH, bs)
+        z = torch.zeros
+        return dict(kc=kc, vc=vc, table=_i(np.zeros((S, MB))), lens=_i([0] * S), free=_i(perm),
+                    count=_i([NB]), new=_i([0] * S), done=_i([0] * S), slots=_i([-1] * T),
+                    pos=_i([-1] * T), start=_i([0] * (S + 1)),
+                    qkv=z(T, H + 2 * KVH, 128, dtype=torch.float16, device="cuda"),
+                    q=z(T, H, 128, dtype=torch.float16, device="cuda"),
+                    out=z(S, H, 128, dtype=torch.float16, device="cuda"))
+
+    def step(s):
+        ops.release_blocks(s["table"], s["lens"], s["done"], s["free"], s["count"], bs,
+                           context_lens_out=s["lens"], free_count_out=s["count"])
+        ops.extend_block_tables(s["table"], s["lens"], s["new"], s["free"], s["count"], NB, bs,
+                                max_tokens=T, slot_mapping=s["slots"], positions=s["pos"],
+                                query_start=s["start"], context_lens_out=s["lens"],
+                                free_count_out=s["count"])
+        x = s["qkv"]
+        ops.norm_rope_into_cache(x[:, :H], x[:, H:H + KVH], x[:, H + KVH:], None, None, s["pos"],
+                                 rope, s["kc"], s["vc"], s["slots"], bs, q_out=s["q"])
+        last = s["q"].index_select(0, (s["start"][1:] - 1).clamp(min=0))
+        ops.decode(s["out"], last, s["kc"], s["vc"], s["table"], s["lens"], scale_for(), bs,
+                   validate=False)
+
+    a, b = state(), state()
+    for s in (a, b):
+        s["new"].fill_(1)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        step(a)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            step(a)
+    torch.cuda.synchronize()
+    step(b)
+    for i in range(10):
+        # Every sequence gets a token at least; some leave and come back with a prompt.
+        done = (rng.random(S) < 0.3).astype(np.int32)
+        add = np.where(done, rng.integers(1, 5, S), 1)
+        x = torch.from_numpy(rng.standard_normal((T, H + 2 * KVH, 128)).astype(np.float16)).cuda()
+        for s in (a, b):
+            s["new"].copy_(_i(add))
+            s["done"].copy_(_i(done))
+            s["qkv"].copy_(x)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        step(b)
+        torch.cuda.synchronize()
+        for name in a:
+            assert torch.equal(a[name], b[name]), (i, name)
+    ops.check_status(a["out"].device)
