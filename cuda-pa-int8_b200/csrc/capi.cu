@@ -415,8 +415,8 @@ int decode_impl(int mode, int kv_i8, void* out, float* part_out, const void* q,
       ra.num_parts = 0;
       ra.piece_stride = s.SLOT;
       ra.seg_stride = (long long)s.s_max * s.SLOT;
-      ra.bf16 = act_bf16 ? 1 : 0;
-      e = pa::launch_reduce(s.GT, ra, s.s_max, st);
+      e = fp4 ? pa::launch_reduce_fp4(s.GT, ra, act_bf16, s.s_max, st)
+              : pa::launch_reduce(s.GT, ra, s.s_max, st);
       if (e != cudaSuccess) return cuda_fail(e, "reduce launch");
     }
   }

@@ -1563,7 +1563,6 @@ cudaError_t launch_selftest_wait(int* status, cudaStream_t st) {
 cudaError_t launch_reduce(int gt, const ReduceArgs& a, int max_pieces, cudaStream_t stream) {
   const int segs = a.B * a.KVH * a.HT;
   if (segs == 0) return cudaSuccess;
-  if (a.bf16) return launch_reduce_bf16(gt, a, max_pieces, stream);
   size_t smem;
   cudaError_t e;
   if (Coop<128, 16, kReduceThreads, 16>::floats(max_pieces) * sizeof(float) > 200 * 1024)

@@ -56,7 +56,8 @@ struct Tile {
   static constexpr size_t SMEM = 128 + RING;
 };
 
-// The merges of decode.cu with fp16 or bf16 output rows. They are kept apart from that file's:
+// The merges of decode.cu with fp16 or bf16 output rows, and with NaN (a block of the cache that
+// holds one) passed on instead of taken for an empty sequence. They are kept apart from that file's:
 // sharing them through a header left its kernels' resources as they were but made the FP8 decode
 // 2 % slower (66.3 -> 67.5 us at 64 x 8192 tokens, 12/2 heads).
 //
@@ -136,9 +137,9 @@ __device__ __noinline__ bool staged_combine(const float* part, int wf, int np, i
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float L = __shfl_sync(0xffffffffu, Lh, h0 + e);
-      inv[e] = L > 0.f ? 1.f / L : 0.f;
+      inv[e] = L == 0.f ? 0.f : 1.f / L;
     }
-    if (lane < hcnt && !(Lh > 0.f)) flag_error(status, PA_ERR_EMPTY_CONTEXT);
+    if (lane < hcnt && Lh == 0.f) flag_error(status, PA_ERR_EMPTY_CONTEXT);
 #pragma unroll
     for (int i = 0; i < O4; ++i) {
       const int d = (lane + 32 * i) / (GT / 4);
@@ -309,7 +310,7 @@ __device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __
           const int h = h0 + e;
           if (h < hcnt) {
             const float L = sL[h];
-            store_out(out_rows + (size_t)h * D + d, L > 0.f ? a4[e] / L : 0.f, BF);
+            store_out(out_rows + (size_t)h * D + d, L == 0.f ? 0.f : a4[e] / L, BF);
           }
         }
       } else {
@@ -321,7 +322,7 @@ __device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __
     if (out_slot != nullptr) {
       out_slot[D * GT + tid] = sM[tid];
       out_slot[D * GT + GT + tid] = sL[tid];
-    } else if (tid < hcnt && !(sL[tid] > 0.f)) {
+    } else if (tid < hcnt && sL[tid] == 0.f) {
       flag_error(status, PA_ERR_EMPTY_CONTEXT);
     }
   }
@@ -329,13 +330,13 @@ __device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __
 }
 
 // ---------------------------------------------------------------------------------------
-// LSE reduce of the split-K pair (and of partials gathered across GPUs): one CTA of
-// kReduceThreads threads per (sequence, kv-head, head tile) segment, merged cooperatively.
+// LSE reduce of the split-K pair: one CTA of kReduceThreads threads per (sequence, kv-head, head
+// tile) segment, merged cooperatively.
 // ---------------------------------------------------------------------------------------
 constexpr int kReduceThreads = 512;
 
-template <int D, int GT>
-__global__ void __launch_bounds__(kReduceThreads, 1) reduce_bf16_kernel(const ReduceArgs a) {
+template <int D, int GT, bool BF>
+__global__ void __launch_bounds__(kReduceThreads, 1) reduce_fp4_kernel(const ReduceArgs a) {
   extern __shared__ __align__(16) float rsm[];
   const int SEGS = a.KVH * a.HT;
   const int segid = blockIdx.x;
@@ -345,14 +346,11 @@ __global__ void __launch_bounds__(kReduceThreads, 1) reduce_bf16_kernel(const Re
   const int ht = seg - kvh * a.HT;
   const int hbase = kvh * a.G + ht * GT;
   const int hcnt = min(GT, a.G - ht * GT);
-  int np = a.num_parts;
-  if (np <= 0) {
-    int c = __ldg(a.context_lens + b);
-    const int cap = a.max_blocks * a.bs;
-    c = c < 0 ? 0 : (c > cap ? cap : c);
-    const int pages = (c + kSubTokens - 1) / kSubTokens;
-    np = (pages + kSplitPages - 1) / kSplitPages;
-  }
+  int c = __ldg(a.context_lens + b);
+  const int cap = a.max_blocks * a.bs;
+  c = c < 0 ? 0 : (c > cap ? cap : c);
+  const int pages = (c + kSubTokens - 1) / kSubTokens;
+  const int np = (pages + kSplitPages - 1) / kSplitPages;
   __half* orow = a.out + ((size_t)b * a.H + hbase) * D;
   if (np == 0) {
     for (int i = threadIdx.x; i < hcnt * D; i += blockDim.x) orow[i] = __float2half_rn(0.f);
@@ -360,7 +358,7 @@ __global__ void __launch_bounds__(kReduceThreads, 1) reduce_bf16_kernel(const Re
     return;
   }
   const float* base = a.part + (size_t)segid * a.seg_stride;
-  coop_combine<D, GT, kReduceThreads, 16, true>(
+  coop_combine<D, GT, kReduceThreads, 16, BF>(
       [&](int k) { return base + (size_t)k * a.piece_stride; }, np, hcnt, orow, nullptr,
       a.status, rsm);
 }
@@ -1278,21 +1276,27 @@ cudaError_t launch_decode_fp4(int gt, const DecodeFp4Args& a, int grid, cudaStre
   return a.G <= 4 ? launch_one<8, true>(a, grid, stream) : launch_one<8, false>(a, grid, stream);
 }
 
-// launch_reduce with bf16 output rows (its checks done).
-cudaError_t launch_reduce_bf16(int gt, const ReduceArgs& a, int max_pieces, cudaStream_t stream) {
+cudaError_t launch_reduce_fp4(int gt, const ReduceArgs& a, bool bf16, int max_pieces,
+                              cudaStream_t stream) {
   const int segs = a.B * a.KVH * a.HT;
+  if (segs == 0) return cudaSuccess;
   auto launch = [&](auto kern, size_t floats) {
     const size_t smem = floats * sizeof(float);
+    if (smem > 200 * 1024) return cudaErrorInvalidValue;  // contexts above 1.5 M tokens
     cudaError_t e =
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return e;
     kern<<<segs, kReduceThreads, smem, stream>>>(a);
     return cudaGetLastError();
   };
-  return gt == 8 ? launch(reduce_bf16_kernel<128, 8>,
-                          Coop<128, 8, kReduceThreads, 16>::floats(max_pieces))
-                 : launch(reduce_bf16_kernel<128, 16>,
-                          Coop<128, 16, kReduceThreads, 16>::floats(max_pieces));
+  if (gt == 8) {
+    const size_t floats = Coop<128, 8, kReduceThreads, 16>::floats(max_pieces);
+    return bf16 ? launch(reduce_fp4_kernel<128, 8, true>, floats)
+                : launch(reduce_fp4_kernel<128, 8, false>, floats);
+  }
+  const size_t floats = Coop<128, 16, kReduceThreads, 16>::floats(max_pieces);
+  return bf16 ? launch(reduce_fp4_kernel<128, 16, true>, floats)
+              : launch(reduce_fp4_kernel<128, 16, false>, floats);
 }
 
 }  // namespace pa

@@ -70,7 +70,6 @@ struct ReduceArgs {
   int num_parts;               // > 0: fixed number of pieces per segment (cross-GPU merge)
   long long piece_stride;      // floats between consecutive pieces of one segment
   long long seg_stride;        // floats between consecutive segments
-  int bf16;                    // out is bf16
 };
 
 // Launch helpers implemented in decode.cu. They return a cudaError_t.
@@ -87,7 +86,8 @@ struct DecodeFp4Args : DecodeArgs {
   int act_bf16;                // q and out are bf16
 };
 cudaError_t launch_decode_fp4(int gt, const DecodeFp4Args& a, int grid, cudaStream_t stream);
-cudaError_t launch_reduce_bf16(int gt, const ReduceArgs& a, int max_pieces, cudaStream_t stream);
+cudaError_t launch_reduce_fp4(int gt, const ReduceArgs& a, bool bf16, int max_pieces,
+                              cudaStream_t stream);
 int decode_fp4_warps_per_cta(int gt);
 // Token-granular cache writes; kind selects the cache type.
 enum RowKind {

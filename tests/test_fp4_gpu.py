@@ -514,3 +514,35 @@ def test_two_batches_on_two_streams():
     for o, w in zip(outs, want):
         assert torch.equal(o, w)
     _ops().check_status(outs[0].device)
+
+
+@pytest.mark.parametrize("dt", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("lens,H,KVH", [([5, 40], 8, 4), ([3000, 70], 12, 2), ([33000], 8, 1),
+                                        ([2000, 9], 32, 2), ([9000], 32, 2)])
+def test_nan_rows_reach_their_heads_and_no_others(lens, H, KVH, dt):
+    """A NaN block in K makes every head of its kv head NaN, one in V the block's 16 values of
+    them, whichever way the pieces are merged; a NaN behind the context does nothing."""
+    c = _case(30, lens, H, KVH, dt=dt, pad=0xFF)
+    q, kc, vc, bt, cl = _gpu(c)
+    G, last = H // KVH, c["lens"][0] - 1
+    blk, off = int(c["bt"][0, last // 16]), int(last % 16)
+    run = _ops().decode if dt == torch.float16 else _ops().decode_bf16
+    for splitk in (False, True):
+        clean = torch.empty_like(q)
+        run(clean, q, kc, vc, bt, cl, scale_for(), splitk=splitk)
+        assert bool(torch.isfinite(clean).all())
+        for is_v in (False, True):
+            k2, v2 = kc.clone(), vc.clone()
+            if is_v:
+                v2[blk, 0, 0, 1024 + 3 * 16 + off] = 0xFF
+            else:
+                k2[blk, 0, 0, 1024 + off * 8 + 3] = 0xFF
+            out = torch.empty_like(q)
+            run(out, q, k2, v2, bt, cl, scale_for(), splitk=splitk)
+            want = torch.zeros(len(lens), H, 128, dtype=torch.bool, device="cuda")
+            want[0, :G, 48:64] = True
+            if not is_v:
+                want[0, :G] = True
+            assert torch.equal(torch.isnan(out), want)
+            assert torch.equal(out[~want], clean[~want])
+    _ops().check_status(q.device)
