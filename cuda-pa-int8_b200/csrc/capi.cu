@@ -190,6 +190,7 @@ int get_map(const MapKey& k, CUtensorMap* out) {
 // ---- decode shapes and workspace -------------------------------------------------------
 struct Shape {
   int G, GT, HT, SEGS, SLOT, s_max, warps_per_cta, sms, chunk_b;
+  int part_owners;  // single pass: warps or, for the fp4 cache, CTAs that leave two partials each
 };
 
 int check_common(int B, int H, int KVH, int D, int NB, int bs, int max_blocks) {
@@ -229,6 +230,7 @@ int make_shape(int kv_i8, int mode, int B, int H, int KVH, int D, int bs, int ma
   s->warps_per_cta = pa::decode_warps_per_cta(kv_i8, s->GT);
   s->sms = num_sms_current(nullptr);
   if (s->sms <= 0) return fail(PA_ERR_CUDA, "cannot query the current device");
+  s->part_owners = kv_i8 == 3 ? s->sms : s->sms * s->warps_per_cta;
   // Sequences per launch: the in-kernel scan holds kBMax, and the flattened page count must
   // stay below 2^31.
   long long per_seq = subpages * s->SEGS;
@@ -251,7 +253,7 @@ size_t ws_bytes_for(const Shape& s, int mode, int B) {
   if (mode == pa::kModeSplit) {
     parts = (size_t)(cb > 0 ? cb : 1) * s.SEGS * s.s_max * s.SLOT * sizeof(float);
   } else {
-    parts = (size_t)s.sms * s.warps_per_cta * 2 * s.SLOT * sizeof(float);
+    parts = (size_t)s.part_owners * 2 * s.SLOT * sizeof(float);
   }
   return off + parts;
 }

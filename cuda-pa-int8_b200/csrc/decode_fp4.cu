@@ -53,7 +53,13 @@ struct Tile {
   static constexpr int PT = fp4::kGroupBytes;
   static constexpr int STAGE = 4 * PT;       // two pages: K, K, V, V
   static constexpr size_t RING = (size_t)WARPS * DEPTH * STAGE;
-  static constexpr size_t SMEM = 128 + RING;
+  // A piece's partial as it lies in shared memory: rows of GT heads, four floats of padding every
+  // sixteen rows (the lanes that store a column of rows then meet in a bank two at a time instead
+  // of eight), maxima, sums.
+  static constexpr int PIECE = SLOT + D / 4;
+  static constexpr size_t EARLY = (size_t)WARPS * PIECE * sizeof(float);
+  static constexpr size_t SMEM = 128 + RING + EARLY;
+  static_assert((size_t)DEPTH * STAGE >= PIECE * sizeof(float), "a warp's ring holds its last piece");
 };
 
 // The merges of decode.cu with fp16 or bf16 output rows, and with NaN (a block of the cache that
@@ -71,92 +77,94 @@ __device__ __forceinline__ void store_out(__half* p, float v, bool bf) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Log-sum-exp merge of `np` partial slots by one warp, from copies of the slots in shared
-// memory: the lanes bulk-copy the slots into `stage` (np * SLOT floats) on the warp's
-// mbarrier `bar`, so a merge waits for one L2 round trip however many pieces it has. Sums
-// run in piece order (k = 0, 1, ...): the arithmetic, and the output's bits, are the same
-// whichever CTA performs the merge. Piece k of the segment is warp (wf + k)'s slot: slot
-// 2 (wf + k) + 1 for the first piece (it starts the segment), 2 (wf + k) for the others.
-// Returns false (status flagged) if the copies did not arrive within the wait limit; the
-// caller then stops using the staging memory. Out of line: it runs a few times per CTA at
-// the end of the launch and should not add to the page loop's registers. BF: out rows are bf16.
+// Log-sum-exp merge of rows `slice` * D / kSlices .. of `np` partials by one warp: m = max m_k,
+// o = sum 2^(m_k - m) o_k, l likewise. piece(k) is partial k, in shared memory (SMEM, with its
+// padding) or a global slot [D][GT], [GT] maxima, [GT] sums. Four partials are in flight at once,
+// and they enter in the order of k, so the bits do not depend on timing. The result is the
+// normalised output rows (out_rows, fp16 or with bf bf16), or a slot (out_slot).
 // ---------------------------------------------------------------------------------------
-template <int D, int GT, bool BF>
-__device__ __noinline__ bool staged_combine(const float* part, int wf, int np, int lane,
-                                            int hcnt, __half* out_rows, float* out_slot,
-                                            int* status, float* stage, uint64_t* bar,
-                                            uint32_t parity) {
-  constexpr int SLOT = (D + 2) * GT;
-  constexpr uint32_t SB = SLOT * sizeof(float);
-  constexpr int O4 = D * GT / 4 / 32;  // float4 outputs per lane
-  static_assert(D * GT / 4 % 32 == 0, "outputs must tile the warp");
-  // Earlier generic accesses (the ring's last reads, a previous merge's use of the staging
-  // memory, the acquire that made the slots visible) come before the copies.
-  fence_proxy_async_all();
-  if (lane == 0) mbar_arrive_expect_tx(bar, (uint32_t)np * SB);
-  __syncwarp();
-  for (int k = lane; k < np; k += 32)
-    bulk_g2s(stage + (size_t)k * SLOT, part + ((size_t)(wf + k) * 2 + (k == 0 ? 1 : 0)) * SLOT,
-             SB, bar);
-  if (!mbar_wait_bounded(bar, parity, status)) return false;
+constexpr int kSlices = 4;
 
-  // Weights: lane h < GT takes head h, M = max_k m_k, w_k = 2^(m_k - M) (written over m_k in
-  // the staged slot), L = sum_k w_k l_k.
-  float Lh = 0.f, Mh = neg_inf();
-  if (lane < GT) {
-    for (int k = 0; k < np; ++k) Mh = fmaxf(Mh, stage[(size_t)k * SLOT + D * GT + lane]);
-    for (int k = 0; k < np; ++k) {
-      float* mk = stage + (size_t)k * SLOT + D * GT + lane;
-      const float w = (Mh == neg_inf()) ? 0.f : ex2(*mk - Mh);
-      *mk = w;
-      Lh = fmaf(w, mk[GT], Lh);
-    }
-  }
-  __syncwarp();
-
-  // O = sum_k w_k O_k. Slots hold O as [D][GT]; float4 o covers row o / (GT/4), heads
-  // h0..h0+3 with h0 = 4 (o % (GT/4)), which is the same for all of a lane's outputs.
+template <int D, int GT, bool SMEM, typename PieceFn>
+__device__ __forceinline__ void merge_rows(PieceFn piece, int np, int slice, int lane, int hcnt,
+                                           __half* out_rows, bool bf, float* out_slot,
+                                           int* status) {
+  constexpr int ROWS = D / kSlices;
+  constexpr int O4 = ROWS * GT / 4 / 32;  // float4 outputs of a lane
+  constexpr int U = 4;
+  constexpr int ML = D * GT + (SMEM ? D / 4 : 0);  // where the maxima are
+  static_assert(ROWS * GT / 4 % 32 == 0, "outputs must tile the warp");
+  auto load = [](const float* s) {
+    float4 v;
+    if constexpr (SMEM) v = *reinterpret_cast<const float4*>(s);
+    else v = __ldcg(reinterpret_cast<const float4*>(s));
+    return v;
+  };
+  // Output i: row d_of(i), heads h0 .. h0 + 3.
   const int h0 = 4 * (lane % (GT / 4));
-  float4 acc[O4];
+  auto d_of = [&](int i) { return slice * ROWS + (lane + 32 * i) / (GT / 4); };
+  float M[4], L[4], acc[O4][4];
 #pragma unroll
-  for (int i = 0; i < O4; ++i) acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k = 0; k < np; ++k) {
-    const float* sk = stage + (size_t)k * SLOT;
-    const float4 w4 = *reinterpret_cast<const float4*>(sk + D * GT + h0);
+  for (int e = 0; e < 4; ++e) {
+    M[e] = neg_inf();
+    L[e] = 0.f;
 #pragma unroll
-    for (int i = 0; i < O4; ++i) {
-      const float4 v = reinterpret_cast<const float4*>(sk)[lane + 32 * i];
-      acc[i].x = fmaf(w4.x, v.x, acc[i].x);
-      acc[i].y = fmaf(w4.y, v.y, acc[i].y);
-      acc[i].z = fmaf(w4.z, v.z, acc[i].z);
-      acc[i].w = fmaf(w4.w, v.w, acc[i].w);
+    for (int i = 0; i < O4; ++i) acc[i][e] = 0.f;
+  }
+  for (int k0 = 0; k0 < np; k0 += U) {
+    float4 m[U], l[U], v[U][O4];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float* s = piece(min(k0 + u, np - 1));
+      m[u] = load(s + ML + h0);
+      l[u] = load(s + ML + GT + h0);
+#pragma unroll
+      for (int i = 0; i < O4; ++i)
+        v[u][i] = load(s + d_of(i) * GT + (SMEM ? d_of(i) / 16 * 4 : 0) + h0);
+      if (k0 + u >= np) m[u] = make_float4(neg_inf(), neg_inf(), neg_inf(), neg_inf());
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      auto at = [&](const float4& x) { return e == 0 ? x.x : e == 1 ? x.y : e == 2 ? x.z : x.w; };
+      float mn = M[e];
+#pragma unroll
+      for (int u = 0; u < U; ++u) mn = fmaxf(mn, at(m[u]));
+      const float from = mn == neg_inf() ? 0.f : mn;
+      const float c = ex2(M[e] - from);
+      M[e] = mn;
+      L[e] *= c;
+#pragma unroll
+      for (int i = 0; i < O4; ++i) acc[i][e] *= c;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float w = ex2(at(m[u]) - from);
+        L[e] = fmaf(w, at(l[u]), L[e]);
+#pragma unroll
+        for (int i = 0; i < O4; ++i) acc[i][e] = fmaf(w, at(v[u][i]), acc[i][e]);
+      }
     }
   }
   if (out_rows != nullptr) {
-    float inv[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const float L = __shfl_sync(0xffffffffu, Lh, h0 + e);
-      inv[e] = L == 0.f ? 0.f : 1.f / L;
-    }
-    if (lane < hcnt && Lh == 0.f) flag_error(status, PA_ERR_EMPTY_CONTEXT);
+      if (h0 + e >= hcnt) continue;
+      const float inv = L[e] == 0.f ? 0.f : 1.f / L[e];
+      if (L[e] == 0.f) flag_error(status, PA_ERR_EMPTY_CONTEXT);
 #pragma unroll
-    for (int i = 0; i < O4; ++i) {
-      const int d = (lane + 32 * i) / (GT / 4);
-      const float a4[4] = {acc[i].x, acc[i].y, acc[i].z, acc[i].w};
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (h0 + e < hcnt) store_out(out_rows + (size_t)(h0 + e) * D + d, a4[e] * inv[e], BF);
+      for (int i = 0; i < O4; ++i)
+        store_out(out_rows + (size_t)(h0 + e) * D + d_of(i), acc[i][e] * inv, bf);
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < O4; ++i) reinterpret_cast<float4*>(out_slot)[lane + 32 * i] = acc[i];
-    if (lane < GT) {
-      out_slot[D * GT + lane] = Mh;
-      out_slot[D * GT + GT + lane] = Lh;
+    for (int i = 0; i < O4; ++i)
+      *reinterpret_cast<float4*>(out_slot + d_of(i) * GT + h0) =
+          make_float4(acc[i][0], acc[i][1], acc[i][2], acc[i][3]);
+    if (slice == 0 && lane < GT / 4) {
+      *reinterpret_cast<float4*>(out_slot + D * GT + h0) = make_float4(M[0], M[1], M[2], M[3]);
+      *reinterpret_cast<float4*>(out_slot + D * GT + GT + h0) =
+          make_float4(L[0], L[1], L[2], L[3]);
     }
   }
-  return true;
 }
 
 // ---------------------------------------------------------------------------------------
@@ -178,9 +186,10 @@ struct Coop {
   }
 };
 
-template <int D, int GT, int NTHR, int U, bool BF, typename PieceFn>
+template <int D, int GT, int NTHR, int U, typename PieceFn>
 __device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __half* out_rows,
-                                             float* out_slot, int* status, float* sm) {
+                                             bool bf, float* out_slot, int* status,
+                                             float* sm) {
   using CC = Coop<D, GT, NTHR, U>;
   static_assert(NTHR >= CC::OUT4 || CC::OUT4 % NTHR == 0, "outputs must tile the block");
   const int tid = threadIdx.x;
@@ -310,7 +319,7 @@ __device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __
           const int h = h0 + e;
           if (h < hcnt) {
             const float L = sL[h];
-            store_out(out_rows + (size_t)h * D + d, L == 0.f ? 0.f : a4[e] / L, BF);
+            store_out(out_rows + (size_t)h * D + d, L == 0.f ? 0.f : a4[e] / L, bf);
           }
         }
       } else {
@@ -358,8 +367,8 @@ __global__ void __launch_bounds__(kReduceThreads, 1) reduce_fp4_kernel(const Red
     return;
   }
   const float* base = a.part + (size_t)segid * a.seg_stride;
-  coop_combine<D, GT, kReduceThreads, 16, BF>(
-      [&](int k) { return base + (size_t)k * a.piece_stride; }, np, hcnt, orow, nullptr,
+  coop_combine<D, GT, kReduceThreads, 16>(
+      [&](int k) { return base + (size_t)k * a.piece_stride; }, np, hcnt, orow, BF, nullptr,
       a.status, rsm);
 }
 
@@ -414,9 +423,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
   __shared__ int s_tmp[32];
   __shared__ int s_empty;
   __shared__ unsigned s_over[kBMax / 32];  // sequences whose context exceeds the table
-  __shared__ int s_pend[WARPS][2][6];
+  __shared__ int s_pend[WARPS][2][6];   // a warp's partials: see the piece epilogue
   __shared__ int s_npend[WARPS];
-  __shared__ uint64_t s_mmb[WARPS];     // per-warp barrier of the end-of-launch merges
+  __shared__ int s_last[2];
   __shared__ int s_nblk[WARPS][32];     // block ids of a warp's next batch of pages
   __shared__ int s_nmeta[WARPS][32];    // their (kv_head << 3) | subpage
   __shared__ int s_nwr[WARPS][32];      // their decode-step new-token sequence, or -1
@@ -428,10 +437,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
   const int g = lane >> 2;  // MMA group (row / column index)
   const int r = lane & 3;   // position inside the group
 
-  if (lane == 0) {
-    mbar_init(&s_mmb[warp], 1);
-    fence_mbar_init();
-  }
   if (threadIdx.x == 0) {
     s_empty = 0;
     // This CTA's share of the block tables and q rows into L2, so the first block-id and q
@@ -553,8 +558,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
     }
   }
   const int n = (int)(p1 - p0);
-  int nrec = 0;              // shared segments whose arrival this warp recorded
-  int old0 = 0, old1 = 0;    // lane 0: the arrival counters' values before those arrivals
+  int nrec = 0;  // partials of segments shared with other warps
   if (n > 0) {
 
   // ---- 3. Consumer position and the first piece's q rows --------------------------------------
@@ -1036,18 +1040,20 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
       const int hcnt = min(GT, a.G - ht * GT);
 
       // Partial slots hold O and l without the 2^kPExp weight factor (an exact rescale).
-      auto write_slot = [&](float* slot) {
+      auto write_slot = [&](float* slot, int pad) {  // pad: floats after every sixteen rows
         constexpr float kUnscale = 1.f / (float)(1 << (int)kPExp);
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            *reinterpret_cast<float2*>(slot + (16 * g + 2 * i) * GT + nt * 8 + 2 * r) =
+            *reinterpret_cast<float2*>(slot + (16 * GT + pad) * g + 2 * i * GT + nt * 8 + 2 * r) =
                 make_float2(oacc[i][nt][0] * kUnscale, oacc[i][nt][1] * kUnscale);
-            *reinterpret_cast<float2*>(slot + (16 * g + 2 * i + 1) * GT + nt * 8 + 2 * r) =
+            *reinterpret_cast<float2*>(slot + (16 * GT + pad) * g + (2 * i + 1) * GT + nt * 8 +
+                                       2 * r) =
                 make_float2(oacc[i][nt][2] * kUnscale, oacc[i][nt][3] * kUnscale);
           }
         }
+        slot += pad * (D / 16);
         if (g == 0) {
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -1060,7 +1066,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
       };
 
       if (split) {
-        write_slot(a.part + ((size_t)segid * a.s_max + piece_sp0 / kSplitPages) * SLOT);
+        write_slot(a.part + ((size_t)segid * a.s_max + piece_sp0 / kSplitPages) * SLOT, 0);
       } else if (piece_sp0 == 0 && csp == cpg) {
         // The whole segment was this warp's: normalise and store directly.
         if (a.mode == kModeStream) {
@@ -1090,35 +1096,27 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
               }
             }
         } else {
-          write_slot(a.part_out + (size_t)segid * SLOT);
+          write_slot(a.part_out + (size_t)segid * SLOT, 0);
         }
       } else {
-        // A piece of a segment shared with neighbouring warps.
-        write_slot(a.part + ((size_t)wg * 2 + (piece_sp0 == 0 ? 1 : 0)) * SLOT);
+        // A piece of a segment shared with neighbouring warps: at most two, the one that ends
+        // the segment the range begins in and the one the range ends with. The latter goes into
+        // the warp's ring, which is done with.
+        const int early = j < n ? 1 : 0;
+        const int off = early ? (int)(C::RING / sizeof(float)) + warp * C::PIECE
+                              : warp * (DEPTH * C::STAGE / (int)sizeof(float));
         __syncwarp();
-        const long long s_start = (long long)s_pre[cb] + (long long)cseg * cpg;
-        const long long s_end = s_start + cpg;
-        const int wf = (int)(((s_start + 1) * Wt - 1) / T);
-        const int wl = (int)((s_end * Wt - 1) / T);
-        const int np = wl - wf + 1;
-        // Release this piece; the arrival that completes the count acquires all of them and
-        // owes the merge, which runs after the page loop, when the registers are free. The
-        // merge is recorded now and kept if the atomic's old value shows the last arrival;
-        // that value is first read after the loop, so the loop does not wait for the atomic.
-        // A warp shares at most two segments (its first and its last).
+        write_slot(reinterpret_cast<float*>(ring) + off, 4);
         if (lane == 0 && nrec < 2) {
-          if (nrec == 0) {
-            old0 = atom_add_acq_rel_gpu(a.counters + segid, 1);
-          } else {
-            old1 = atom_add_acq_rel_gpu(a.counters + segid, 1);
-          }
+          const long long s_start = (long long)s_pre[cb] + (long long)cseg * cpg;
+          const long long s_end = s_start + cpg;
           int* pe = s_pend[warp][nrec];
           pe[0] = segid;
-          pe[1] = wf;
-          pe[2] = np;
-          pe[3] = cb;
-          pe[4] = hbase;
-          pe[5] = hcnt;
+          pe[1] = off;
+          pe[2] = cb;
+          pe[3] = (hbase << 5) | hcnt;
+          pe[4] = (int)(((s_start + 1) * Wt - 1) / T) / WARPS;  // the segment's first CTA
+          pe[5] = (int)((s_end * Wt - 1) / T) / WARPS;          // and its last
         }
         ++nrec;
       }
@@ -1141,96 +1139,101 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
   cp_async_wait_all();
   }  // n > 0
 
-  // ---- 5. Merges of the segments whose last piece this CTA's warps finished ------------------
-  // The pieces of a recorded merge are visible: the recording arrival acquired them, and the
-  // barrier below orders that arrival before every warp's reads.
-  // Each merge of up to kStageCap pieces is one warp's: it bulk-copies the pieces into the
-  // (now idle) ring memory and merges them from there, side by side with the CTA's other
-  // merges; merges are packed into the ring memory in a fixed order, in waves when they do not
-  // all fit at once. Only a merge of more pieces than the ring memory holds runs on the whole
-  // CTA, reading the pieces from L2.
-  if (lane == 0) {
-    // The recorded merges this warp owes: those whose arrival completed the count.
-    int k = 0;
-    for (int e = 0; e < min(nrec, 2); ++e) {
-      const int* pe = s_pend[warp][e];
-      if ((e == 0 ? old0 : old1) == pe[2] - 1) {
-        if (k != e)
-          for (int f = 0; f < 6; ++f) s_pend[warp][k][f] = pe[f];
-        ++k;
-      }
-    }
-    s_npend[warp] = k;
-  }
-  __syncthreads();  // every warp is past its page loop: the ring memory is free
-  constexpr size_t kRing = C::RING;
-  constexpr int kStageCap = (int)(kRing / (SLOT * sizeof(float)));
-  float* scratch = reinterpret_cast<float*>(ring);
+  // ---- 5. Merges. A CTA's warps hold neighbouring ranges, so the partials of a segment lie side
+  // by side: first the CTA's own are merged in shared memory. A segment that it holds alone is
+  // done; of others (at most two, the first and the last) the CTA leaves one partial in the
+  // workspace, and the CTA that arrives last merges those. (With a partial of every warp in the
+  // workspace one segment of 8192 tokens was up to 512 of them: 1 x 8192 tokens took 60 us.)
+  if (lane == 0) s_npend[warp] = min(nrec, 2);
+  __syncthreads();
+  // Entry i = 2 * warp + e in lane i; groups of entries of one segment.
+  static_assert(2 * WARPS <= 32, "a lane for each partial");
+  const bool have = lane < 2 * WARPS && (lane & 1) < s_npend[min(lane >> 1, WARPS - 1)];
+  const int* pe = s_pend[min(lane >> 1, WARPS - 1)][lane & 1];
+  const int e_seg = have ? pe[0] : -1, e_off = have ? pe[1] : 0, e_b = have ? pe[2] : 0;
+  const int e_heads = have ? pe[3] : 0, e_c0 = have ? pe[4] : 0, e_c1 = have ? pe[5] : 0;
+  const unsigned entries = __ballot_sync(0xffffffffu, have);
+  const unsigned below = entries & ((1u << lane) - 1u);
+  int* const s_off = s_nblk[warp];  // (done with) the entries' places, packed
+  if (have) s_off[__popc(below)] = e_off;
+  __syncwarp();
+  const int prev_seg = __shfl_sync(0xffffffffu, e_seg, below ? 31 - __clz(below) : 0);
+  const unsigned heads = __ballot_sync(0xffffffffu, have && (below == 0u || prev_seg != e_seg));
+  const unsigned cross = heads & __ballot_sync(0xffffffffu, have && e_c0 != e_c1);
   const bool stream = (a.mode == kModeStream);
-  int used = 0, inwave = 0;
-  uint32_t mph = 0;  // phase parity of this warp's merge barrier
-  bool any_big = false;
-  for (int w = 0; w < WARPS; ++w) {
-    for (int e = 0; e < s_npend[w]; ++e) {
-      const int* pe = s_pend[w][e];
-      const int np = pe[2];
-      if (np > kStageCap) {
-        any_big = true;
-        continue;
-      }
-      if (used + np > kStageCap || inwave == WARPS) {
-        __syncthreads();  // the wave's merges are done with the ring memory
-        used = 0;
-        inwave = 0;
-      }
-      if (inwave == warp) {
-        const int segid = pe[0], wf = pe[1], b = pe[3], hbase = pe[4], hcnt = pe[5];
-        __half* orow = stream ? a.out + ((size_t)b * a.H + hbase) * D : nullptr;
-        float* oslot = stream ? nullptr : a.part_out + (size_t)segid * SLOT;
-        float* stg = scratch + (size_t)used * SLOT;
-        const bool done =
-            a.act_bf16
-                ? staged_combine<D, GT, true>(a.part, wf, np, lane, hcnt, orow, oslot, a.status, stg,
-                                              &s_mmb[warp], mph)
-                : staged_combine<D, GT, false>(a.part, wf, np, lane, hcnt, orow, oslot, a.status,
-                                               stg, &s_mmb[warp], mph);
-        if (!done) {
-          // Timed out: let the copies land before the memory is used again.
-          (void)mbar_wait_bounded(&s_mmb[warp], mph, nullptr);
-        }
-        mph ^= 1u;
-        if (lane == 0) a.counters[segid] = 0;
-      }
-      used += np;
-      ++inwave;
-    }
+  const bool bf = a.act_bf16 != 0;
+  const int cta = blockIdx.x;
+  float* const smem = reinterpret_cast<float*>(ring);
+  // Slots of the workspace: two a CTA, the second for a segment that starts in it.
+  auto global_slot = [&](int c, int first) {
+    return a.part + ((size_t)c * 2 + (c == first ? 1 : 0)) * SLOT;
+  };
+  struct Group {
+    int segid, c0, c1, hcnt;
+    __half* rows;  // where the segment's output goes
+    float* slot;
+  };
+  auto group_at = [&](int i0) {
+    Group x;
+    x.segid = __shfl_sync(0xffffffffu, e_seg, i0);
+    x.c0 = __shfl_sync(0xffffffffu, e_c0, i0);
+    x.c1 = __shfl_sync(0xffffffffu, e_c1, i0);
+    const int b = __shfl_sync(0xffffffffu, e_b, i0), hh = __shfl_sync(0xffffffffu, e_heads, i0);
+    x.hcnt = hh & 31;
+    x.rows = stream ? a.out + ((size_t)b * a.H + (hh >> 5)) * D : nullptr;
+    x.slot = stream ? nullptr : a.part_out + (size_t)x.segid * SLOT;
+    return x;
+  };
+  // Merges the entries of the group that begins with entry i0.
+  auto merge_own = [&](int i0, int slice, int hcnt, __half* rows, float* slot) {
+    const unsigned from = ~((1u << i0) - 1u);
+    const unsigned later = heads & from & (heads - (1u << i0));  // heads of later groups
+    const unsigned own = entries & from & (later ? (later & (0u - later)) - 1u : ~0u);
+    const int* offs = s_off + __popc(entries & ~from);
+    merge_rows<D, GT, true>([&](int k) -> const float* { return smem + offs[k]; }, __popc(own),
+                            slice, lane, hcnt, rows, bf, slot, a.status);
+  };
+  // The shared segments' partials first; while their arrivals are on the way, the others.
+  static_assert(2 * kSlices <= WARPS, "one item a warp");
+  if (warp < __popc(cross) * kSlices) {
+    const int i0 = warp < kSlices ? __ffs(cross) - 1 : 31 - __clz(cross);
+    const Group x = group_at(i0);
+    merge_own(i0, warp % kSlices, x.hcnt, nullptr, global_slot(cta, x.c0));
   }
-  if (!any_big) return;
-  __syncthreads();  // the staged merges are done with the ring memory
-  for (int w = 0; w < WARPS; ++w) {
-    for (int e = 0; e < s_npend[w]; ++e) {
-      const int* pe = s_pend[w][e];
-      const int segid = pe[0], wf = pe[1], np = pe[2], b = pe[3], hbase = pe[4], hcnt = pe[5];
-      if (np <= kStageCap) continue;
-      if (Coop<D, GT, NTHR, 8>::floats(np) * sizeof(float) > kRing) {
-        if (threadIdx.x == 0) {
-          flag_error(a.status, PA_ERR_WORKSPACE);
-          a.counters[segid] = 0;  // leave the counter ready for the next call
-        }
-        continue;
-      }
-      auto piece = [&](int k) -> const float* {
-        return a.part + ((size_t)(wf + k) * 2 + (k == 0 ? 1 : 0)) * SLOT;
-      };
-      __half* orow = stream ? a.out + ((size_t)b * a.H + hbase) * D : nullptr;
-      float* oslot = stream ? nullptr : a.part_out + (size_t)segid * SLOT;
-      if (a.act_bf16) {
-        coop_combine<D, GT, NTHR, 8, true>(piece, np, hcnt, orow, oslot, a.status, scratch);
-      } else {
-        coop_combine<D, GT, NTHR, 8, false>(piece, np, hcnt, orow, oslot, a.status, scratch);
-      }
-      if (threadIdx.x == 0) a.counters[segid] = 0;
+  int last = 0;
+  if (cross != 0u) {
+    // Release the CTA's partials; the arrival that completes a segment's count acquires the
+    // others'.
+    __syncthreads();
+    if (warp == 0 && ((cross >> lane) & 1u))
+      last = atom_add_acq_rel_gpu(a.counters + e_seg, 1) == e_c1 - e_c0 ? 1 : 0;
+  }
+  unsigned todo = heads & ~cross;
+  for (int item = WARPS - 1 - warp, n_items = __popc(todo) * kSlices, at = 0; item < n_items;
+       item += WARPS) {
+    for (; at < item / kSlices; ++at) todo &= todo - 1u;
+    const int i0 = __ffs(todo) - 1;
+    const Group x = group_at(i0);
+    merge_own(i0, item % kSlices, x.hcnt, x.rows, x.slot);
+  }
+  if (cross == 0u) return;
+  if (warp == 0 && ((cross >> lane) & 1u)) s_last[below & cross ? 1 : 0] = last;
+  __syncthreads();
+  todo = cross;
+  for (int x = 0; todo != 0u; ++x, todo &= todo - 1u) {
+    if (!s_last[x]) continue;
+    const Group gr = group_at(__ffs(todo) - 1);
+    const int np = gr.c1 - gr.c0 + 1;
+    auto piece = [&](int k) -> const float* { return global_slot(gr.c0 + k, gr.c0); };
+    if (np <= 8) {  // two rounds of loads
+      const int w = warp - x * kSlices;
+      if (w >= 0 && w < kSlices)
+        merge_rows<D, GT, false>(piece, np, w, lane, gr.hcnt, gr.rows, bf, gr.slot, a.status);
+    } else {
+      static_assert(Coop<D, GT, NTHR, 16>::floats(1024) * sizeof(float) <= C::RING, "scratch");
+      coop_combine<D, GT, NTHR, 16>(piece, np, gr.hcnt, gr.rows, bf, gr.slot, a.status, smem);
     }
+    if (threadIdx.x == 0) a.counters[gr.segid] = 0;
   }
 }
 
