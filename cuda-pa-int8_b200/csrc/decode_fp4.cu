@@ -1,10 +1,13 @@
 // Paged-attention decode over the 4-bit K/V cache (format and layout: fp4.cuh).
 //
-// The work is cut and the partials are merged as in decode.cu (one warp per equal range of 16-token
-// pages of the flattened sequence x kv head x head tile x page list; a segment cut between warps
-// leaves partials that the last arrival merges, in piece order, so results do not depend on
-// timing). The page loop is its own, because at 144 bytes a token and kv head it is bound by
-// what the four schedulers of an SM can issue, not by memory:
+// The work is cut as in decode.cu: one warp per equal range of 16-token pages of the flattened
+// sequence x kv head x head tile x page list. A segment cut between warps leaves partials; those of
+// one CTA are merged in its shared memory, those of several CTAs by the one that arrives last, in
+// page order, so results do not depend on timing. (A partial of every warp in the workspace, as
+// decode.cu has it, cost 2.5 us a launch and, where few sequences have many pages, much more:
+// 1 x 8192 tokens, 12/2 heads, 58 us instead of 16.)
+// The page loop is its own, because at 144 bytes a token and kv head it is bound by what the four
+// schedulers of an SM can issue, not by memory:
 //  * two pages a step, copied by all lanes of the warp (16-byte asynchronous copies into the
 //    warp's ring), so a step's fixed costs are shared by 32 tokens;
 //  * S^T = K Q^T with tokens on the MMA's 16 rows and the (up to 8) heads of a kv head on its
@@ -21,13 +24,13 @@
 //    one multiply-add before the exponential (raw scores are compared with a threshold).
 // 277 warp instructions a page (479 with decode.cu's loop): 64 conversions, 64 multiplies, 24
 // MMAs, 16 to pair the codes of neighbouring tokens for PV, the rest softmax, copies and loop.
-// Measured on a B200 (graph replay): 64 x 8192 tokens, 12/2 heads 45.2 us (3.35 TB/s); 8 x 64-128
-// K, 64/8 heads 175.5 us (5.16 TB/s, 0.79 of the measured copy bandwidth). The loop takes 467
-// cycles a page and scheduler, of which the ALU pipe (conversions, logic) is busy for 255, the
-// tensor pipe for 192 and the multiplies for 180; the three hardly overlap (a group of one MMA
-// and three of each takes 18.6 cycles where the MMA alone takes 8 and the others 8). Warps of 16 a
-// CTA (128 registers), the QK of the next step issued between the PV of this one, and a choice of
-// refill inside one loop for all full pages measured no better.
+// Measured on a B200 (graph replay): 64 x 8192 tokens, 12/2 heads 41.3 us (3.67 TB/s); 8 x 64-128
+// K, 64/8 heads 167 us (5.43 TB/s, 0.83 of the measured copy bandwidth). With twelve warps the loop
+// took 467 cycles a page and scheduler, of which the ALU pipe (conversions, logic) was busy for
+// 255, the tensor pipe for 192 and the multiplies for 180; the three hardly overlap (a group of
+// one MMA and three of each takes 18.6 cycles where the MMA alone takes 8 and the others 8). The
+// QK of the next step issued between the PV of this one, two chains of QK MMAs a page instead of
+// one, and a choice of refill inside one loop for all full pages measured no better.
 
 #include "fp4.cuh"
 #include "pa_common.cuh"
@@ -62,10 +65,10 @@ struct Tile {
   static_assert((size_t)DEPTH * STAGE >= PIECE * sizeof(float), "a warp's ring holds its last piece");
 };
 
-// The merges of decode.cu with fp16 or bf16 output rows, and with NaN (a block of the cache that
-// holds one) passed on instead of taken for an empty sequence. They are kept apart from that file's:
-// sharing them through a header left its kernels' resources as they were but made the FP8 decode
-// 2 % slower (66.3 -> 67.5 us at 64 x 8192 tokens, 12/2 heads).
+// Merges take bf16 output rows too, and pass NaN on (a block of the cache that holds one) instead of
+// taking it for an empty sequence. This file shares no code with decode.cu's: sharing it through a
+// header left its kernels' resources as they were but made the FP8 decode 2 % slower (66.3 -> 67.5
+// us at 64 x 8192 tokens, 12/2 heads).
 //
 // One output value, as fp16 or bf16.
 __device__ __forceinline__ void store_out(__half* p, float v, bool bf) {
@@ -791,10 +794,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
     // none, and is met again by the other piece).
     auto step = [&](auto full, int s, int valid0, int valid1) {
       constexpr bool FULL = decltype(full)::value;
-      // Chains of MMAs a page's scores are summed in. One wants no additions, two wait less.
-      // 64 x 4096 tokens, 32/8 heads: 66.8 us with one, 68.2 with two; 64 x 8192, 32/2: 62.5 and
-      // 63.1; 8 x 65536, 64/8 (one tile of eight, no PACK): 132.1 and 130.3.
-      constexpr int CH = PACK || NT == 2 ? 1 : 2;
       const uint32_t st = my_ring + (uint32_t)s * (uint32_t)C::STAGE;
       const uint32_t ka = st + tau * fp4::kCodeRow + 16 * r;
       const uint32_t ksa = st + fp4::kCodes + tau * 8 + 2 * r;
@@ -811,7 +810,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
         const uint32_t z0 = lds16(ksa + u * C::PT), z1 = lds16(ksa + u * C::PT + 16);
         const uint32_t w0[4] = {c0.x, c0.y, c0.z, c0.w}, w1[4] = {c1.x, c1.y, c1.z, c1.w};
         const uint32_t s0 = fp4::scale_pair(z0), s1 = fp4::scale_pair(z1);
-        float acc[CH][NT][4];
+        float acc[NT][4];
         auto mma = [](bool begin, float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                       uint32_t a3, uint32_t b0, uint32_t b1) {
           if (begin) mma_16816_zero(d, a0, a1, a2, a3, b0, b1);
@@ -829,23 +828,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
             i4[e] = si < NS / 2 ? fp4::hmul2_half<false>(i4[e], s1)
                                 : fp4::hmul2_half<true>(i4[e], s1);
           }
-          mma(si == 0, acc[0][0], h[0], i4[0], h[1], i4[1], qa[si].x, qa[si].y);
-          mma(CH == 2 && si == 0, acc[CH - 1][0], h[2], i4[2], h[3], i4[3], qa[si].z, qa[si].w);
+          mma(si == 0, acc[0], h[0], i4[0], h[1], i4[1], qa[si].x, qa[si].y);
+          mma(false, acc[0], h[2], i4[2], h[3], i4[3], qa[si].z, qa[si].w);
           if constexpr (NT == 2) {
-            mma(si == 0, acc[0][1], h[0], i4[0], h[1], i4[1], qb[si].x, qb[si].y);
-            mma(CH == 2 && si == 0, acc[CH - 1][1], h[2], i4[2], h[3], i4[3], qb[si].z, qb[si].w);
+            mma(si == 0, acc[1], h[0], i4[0], h[1], i4[1], qb[si].x, qb[si].y);
+            mma(false, acc[1], h[2], i4[2], h[3], i4[3], qb[si].z, qb[si].w);
           }
         }
         // Raw scores: heads nt * 8 + 2r + (e & 1) of token tau (e < 2) and tau + 2.
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            float2 v = make_float2(acc[0][nt][e], acc[0][nt][e + 1]);
-            if constexpr (CH == 2) v = add2(v, make_float2(acc[1][nt][e], acc[1][nt][e + 1]));
-            x[u][nt][e] = v.x;
-            x[u][nt][e + 1] = v.y;
-          }
+          for (int e = 0; e < 4; ++e) x[u][nt][e] = acc[nt][e];
       }
       if constexpr (!FULL) {
 #pragma unroll
@@ -1238,11 +1232,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
 }
 
 // Warps per CTA and ring stages per warp, by head tile (16 heads keep twice the accumulators).
-// Twelve warps: 168 registers, three to a scheduler. 64 x 8192 / 8 x 64-128 K tokens: 45.3 / 176.1
-// us with three stages, 48.2 / 175.4 with two; eight warps (four stages) 45.2 / 185.9, ten (four)
-// 49.3 / 207.2, fourteen (three) 52.7 / 209.7, sixteen (two) 49.3 / 180.4.
+// 64 x 8192 / ragged 256 / 8 x 64-128 K tokens (12/2, 28/4 and 64/8 heads): 41.4 / 108.8 / 169.5 us
+// with sixteen warps of two stages (128 registers), 43.2 / 110.1 / 170.9 with twelve of two, 43.3 /
+// 110.7 / 171.6 with twelve of three, 43.2 / 119.7 / 184.2 with eight of four.
 template <int GT> struct Shape;
-template <> struct Shape<8> { static constexpr int W = 12, DP = 3; };
+template <> struct Shape<8> { static constexpr int W = 16, DP = 2; };
 template <> struct Shape<16> { static constexpr int W = 8, DP = 4; };
 
 template <int GT, bool PACK>
@@ -1250,7 +1244,7 @@ cudaError_t launch_one(const DecodeFp4Args& a, int grid, cudaStream_t stream) {
   constexpr int W = Shape<GT>::W;
   constexpr int DP = Shape<GT>::DP;
   using C = Tile<128, GT, DP, W>;
-  static_assert(C::SMEM + 14 * 1024 <= 227 * 1024, "shared memory of a launch");
+  static_assert(C::SMEM + 15 * 1024 + 512 <= 227 * 1024, "shared memory of a launch");
   auto kern = decode_fp4_kernel<128, GT, PACK, DP, W>;
   // The shared-memory opt-in is a per-device function attribute: set it once per device.
   static std::atomic<uint64_t> configured{0};
@@ -1274,8 +1268,8 @@ int decode_fp4_warps_per_cta(int gt) { return gt == 8 ? Shape<8>::W : Shape<16>:
 cudaError_t launch_decode_fp4(int gt, const DecodeFp4Args& a, int grid, cudaStream_t stream) {
   if (gt != 8) return launch_one<16, false>(a, grid, stream);
   // PACK: the PV of at most four heads leaves half of the MMA's columns empty, which then hold the
-  // weights' second parts: 8 MMAs a page instead of 16. 32/8 heads, 64 x 4096 tokens: 76.6 us
-  // without, 73.0 with; 8 x 65536: 140.3 and 133.7.
+  // weights' second parts: 8 MMAs a page instead of 16. 32/8 heads, 64 x 4096 tokens: 69.9 us
+  // without, 65.1 with; 8 x 65536: 123.0 and 111.1.
   return a.G <= 4 ? launch_one<8, true>(a, grid, stream) : launch_one<8, false>(a, grid, stream);
 }
 
