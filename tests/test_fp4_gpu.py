@@ -546,3 +546,25 @@ def test_nan_rows_reach_their_heads_and_no_others(lens, H, KVH, dt):
             assert torch.equal(torch.isnan(out), want)
             assert torch.equal(out[~want], clean[~want])
     _ops().check_status(q.device)
+
+
+@pytest.mark.parametrize("H,KVH", [(12, 2), (32, 2), (4, 1), (20, 1)])
+@pytest.mark.parametrize("lens", [[16] * 200, [17] * 150, [33] * 64, [20000], [6000, 1, 6000],
+                                  [250, 2000, 31, 500] * 8, [1] * 30 + [9000] + [1] * 30])
+def test_merges_inside_and_across_ctas(lens, H, KVH):
+    """Segments within one warp, one CTA, neighbouring CTAs and up to all of them; the same bits in
+    every run; partials of the same launch shape merge to the same rows."""
+    c = _case(40 + len(lens), lens, H, KVH)
+    q, kc, vc, bt, cl = _gpu(c)
+    out = torch.full_like(q, float("nan"))
+    _ops().decode(out, q, kc, vc, bt, cl, scale_for())
+    _close(out, c)
+    for _ in range(3):
+        again = torch.full_like(q, float("nan"))
+        _ops().decode(again, q, kc, vc, bt, cl, scale_for())
+        assert torch.equal(out, again)
+    part = _ops().decode_partial(q, kc, vc, bt, cl, scale_for())
+    merged = torch.full_like(q, float("nan"))
+    _ops().merge_partials(merged, part[None], H, KVH)
+    _close(merged, c)
+    _ops().check_status(q.device)
