@@ -246,6 +246,13 @@ int make_shape(int kv_i8, int mode, int B, int H, int KVH, int D, int bs, int ma
   return PA_OK;
 }
 
+// The fp4 cache has one decode kernel: it cuts long contexts at page granularity and merges inside
+// the launch, so a launch pair of 512-token splits would only be coarser (183 sequences of 352-704
+// tokens, 28/4 heads: 66 us as a pair).
+int decode_mode(int kv_i8, int splitk) {
+  return splitk && kv_i8 != 3 ? pa::kModeSplit : pa::kModeStream;
+}
+
 size_t ws_bytes_for(const Shape& s, int mode, int B) {
   const long long cb = B < s.chunk_b ? B : s.chunk_b;
   const size_t off = pa::kWsPartOffset;
@@ -417,8 +424,7 @@ int decode_impl(int mode, int kv_i8, void* out, float* part_out, const void* q,
       ra.num_parts = 0;
       ra.piece_stride = s.SLOT;
       ra.seg_stride = (long long)s.s_max * s.SLOT;
-      e = fp4 ? pa::launch_reduce_fp4(s.GT, ra, act_bf16, s.s_max, st)
-              : pa::launch_reduce(s.GT, ra, s.s_max, st);
+      e = pa::launch_reduce(s.GT, ra, s.s_max, st);
       if (e != cudaSuccess) return cuda_fail(e, "reduce launch");
     }
   }
@@ -530,7 +536,7 @@ size_t pa_decode_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads, 
   Shape s;
   const int kv_i8 = kv_kind(kv_dtype);
   if (kv_i8 < 0) return 0;
-  const int mode = splitk ? pa::kModeSplit : pa::kModeStream;
+  const int mode = decode_mode(kv_i8, splitk);
   if (make_shape(kv_i8, mode, num_seqs, num_heads, num_kv_heads, head_dim, block_size,
                  max_blocks_per_seq, &s) != PA_OK)
     return 0;
@@ -649,7 +655,7 @@ int pa_decode_bf16q(void* out, const void* q, const void* k_cache, const void* v
   if (workspace_bytes < need)
     return fail(PA_ERR_WORKSPACE, "workspace too small: %zu < %zu bytes", workspace_bytes, need);
   if (kv_kind(kv_dtype) == 3)
-    return decode_impl(splitk ? pa::kModeSplit : pa::kModeStream, 3, out, nullptr, q, k_cache,
+    return decode_impl(pa::kModeStream, 3, out, nullptr, q, k_cache,
                        v_cache, nullptr, nullptr, block_table, context_lens, num_seqs, num_heads,
                        num_kv_heads, head_dim, num_blocks, block_size, max_blocks_per_seq, scale,
                        workspace, workspace_bytes, stream, nullptr, true);
@@ -726,7 +732,7 @@ int pa_splitk_fp4(void* out, const void* q, const void* k_cache, const void* v_c
                   int max_blocks_per_seq, float scale, void* workspace, size_t workspace_bytes,
                   void* stream) {
   const NvtxRange nvtx_range("pa_splitk_fp4");
-  return decode_impl(pa::kModeSplit, 3, out, nullptr, q, k_cache, v_cache, nullptr, nullptr,
+  return decode_impl(pa::kModeStream, 3, out, nullptr, q, k_cache, v_cache, nullptr, nullptr,
                      block_table, context_lens, num_seqs, num_heads, num_kv_heads, head_dim,
                      num_blocks, block_size, max_blocks_per_seq, scale, workspace,
                      workspace_bytes, stream);
@@ -764,7 +770,7 @@ int pa_decode_step(int kv_dtype, void* out, const void* q, const void* new_k,
     return fail(PA_ERR_INVALID_ARG, "fixed scales need an int8 cache and both of k and v");
   StepWrite sw{new_k, new_v, new_dtype, (long long)new_token_stride, k_fixed_scale,
                v_fixed_scale, fused != 0};
-  return decode_impl(splitk ? pa::kModeSplit : pa::kModeStream, kind, out, nullptr, q, k_cache,
+  return decode_impl(decode_mode(kind, splitk), kind, out, nullptr, q, k_cache,
                      v_cache, k_scales, v_scales, block_table, context_lens, num_seqs,
                      num_heads, num_kv_heads, head_dim, num_blocks, block_size,
                      max_blocks_per_seq, scale, workspace, workspace_bytes, stream, &sw);

@@ -342,40 +342,6 @@ __device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __
 }
 
 // ---------------------------------------------------------------------------------------
-// LSE reduce of the split-K pair: one CTA of kReduceThreads threads per (sequence, kv-head, head
-// tile) segment, merged cooperatively.
-// ---------------------------------------------------------------------------------------
-constexpr int kReduceThreads = 512;
-
-template <int D, int GT, bool BF>
-__global__ void __launch_bounds__(kReduceThreads, 1) reduce_fp4_kernel(const ReduceArgs a) {
-  extern __shared__ __align__(16) float rsm[];
-  const int SEGS = a.KVH * a.HT;
-  const int segid = blockIdx.x;
-  const int b = segid / SEGS;
-  const int seg = segid - b * SEGS;
-  const int kvh = seg / a.HT;
-  const int ht = seg - kvh * a.HT;
-  const int hbase = kvh * a.G + ht * GT;
-  const int hcnt = min(GT, a.G - ht * GT);
-  int c = __ldg(a.context_lens + b);
-  const int cap = a.max_blocks * a.bs;
-  c = c < 0 ? 0 : (c > cap ? cap : c);
-  const int pages = (c + kSubTokens - 1) / kSubTokens;
-  const int np = (pages + kSplitPages - 1) / kSplitPages;
-  __half* orow = a.out + ((size_t)b * a.H + hbase) * D;
-  if (np == 0) {
-    for (int i = threadIdx.x; i < hcnt * D; i += blockDim.x) orow[i] = __float2half_rn(0.f);
-    if (threadIdx.x == 0 && seg == 0) flag_error(a.status, PA_ERR_EMPTY_CONTEXT);
-    return;
-  }
-  const float* base = a.part + (size_t)segid * a.seg_stride;
-  coop_combine<D, GT, kReduceThreads, 16>(
-      [&](int k) { return base + (size_t)k * a.piece_stride; }, np, hcnt, orow, BF, nullptr,
-      a.status, rsm);
-}
-
-// ---------------------------------------------------------------------------------------
 // Decode step over a 4-bit cache: one warp quantises the new token's K and V rows (16-bit, at
 // src_k / src_v) and stores them into the cache, at token `off` of page row `row`, before it
 // loads the page. Only the calling warp reads the page.
@@ -537,17 +503,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
     seg = rel / pg;
     sp = rel - seg * pg;
   };
-  // Smallest split start >= p (split mode).
-  auto snap = [&](long long p) -> long long {
-    if (p >= T) return T;
-    int b, seg, sp;
-    locate((int)p, b, seg, sp);
-    const int pg = pages_of(b);
-    const int sp2 = (sp + kSplitPages - 1) / kSplitPages * kSplitPages;
-    if (sp2 >= pg) return (long long)s_pre[b] + (long long)(seg + 1) * pg;
-    return (long long)s_pre[b] + (long long)seg * pg + sp2;
-  };
-
   // ---- 2. This warp's page range ------------------------------------------------------------
   const long long Wt = min((long long)a.total_warps, (long long)T);
   const int wg = blockIdx.x * WARPS + warp;
@@ -555,10 +510,6 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
   if (wg < Wt) {
     p0 = (long long)wg * T / Wt;
     p1 = (long long)(wg + 1) * T / Wt;
-    if (a.mode == kModeSplit) {
-      p0 = snap(p0);
-      p1 = snap(p1);
-    }
   }
   const int n = (int)(p1 - p0);
   int nrec = 0;  // partials of segments shared with other warps
@@ -747,15 +698,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
   const int tau = 4 * (g >> 1) + (g & 1);  // token of K row g (row g + 8: + 2)
 
   int s = 0;  // ring stage of page j
-  const bool split = (a.mode == kModeSplit);
   int j = 0;
   while (j < n) {
-    // ---- one piece: the pages of this warp's range inside one segment (one split in split
-    // mode), pages [csp, csp + len) of sequence cb, segment cseg.
+    // ---- one piece: the pages of this warp's range inside one segment, pages
+    // [csp, csp + len) of sequence cb, segment cseg.
     const int piece_sp0 = csp;
-    int len = cpg - csp;
-    if (split) len = min(len, kSplitPages - csp % kSplitPages);
-    len = min(len, n - j);
+    const int len = min(cpg - csp, n - j);
     if (q_b != cb || q_seg != cseg) {
       fetch_q(cb, cseg);
       convert_q();
@@ -1059,9 +1007,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
         }
       };
 
-      if (split) {
-        write_slot(a.part + ((size_t)segid * a.s_max + piece_sp0 / kSplitPages) * SLOT, 0);
-      } else if (piece_sp0 == 0 && csp == cpg) {
+      if (piece_sp0 == 0 && csp == cpg) {
         // The whole segment was this warp's: normalise and store directly.
         if (a.mode == kModeStream) {
           // A lane holds values 16g .. 16g + 15 of its heads: 32 contiguous bytes each.
@@ -1271,29 +1217,6 @@ cudaError_t launch_decode_fp4(int gt, const DecodeFp4Args& a, int grid, cudaStre
   // weights' second parts: 8 MMAs a page instead of 16. 32/8 heads, 64 x 4096 tokens: 69.9 us
   // without, 65.1 with; 8 x 65536: 123.0 and 111.1.
   return a.G <= 4 ? launch_one<8, true>(a, grid, stream) : launch_one<8, false>(a, grid, stream);
-}
-
-cudaError_t launch_reduce_fp4(int gt, const ReduceArgs& a, bool bf16, int max_pieces,
-                              cudaStream_t stream) {
-  const int segs = a.B * a.KVH * a.HT;
-  if (segs == 0) return cudaSuccess;
-  auto launch = [&](auto kern, size_t floats) {
-    const size_t smem = floats * sizeof(float);
-    if (smem > 200 * 1024) return cudaErrorInvalidValue;  // contexts above 1.5 M tokens
-    cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return e;
-    kern<<<segs, kReduceThreads, smem, stream>>>(a);
-    return cudaGetLastError();
-  };
-  if (gt == 8) {
-    const size_t floats = Coop<128, 8, kReduceThreads, 16>::floats(max_pieces);
-    return bf16 ? launch(reduce_fp4_kernel<128, 8, true>, floats)
-                : launch(reduce_fp4_kernel<128, 8, false>, floats);
-  }
-  const size_t floats = Coop<128, 16, kReduceThreads, 16>::floats(max_pieces);
-  return bf16 ? launch(reduce_fp4_kernel<128, 16, true>, floats)
-              : launch(reduce_fp4_kernel<128, 16, false>, floats);
 }
 
 }  // namespace pa

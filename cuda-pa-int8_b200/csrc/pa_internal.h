@@ -86,8 +86,6 @@ struct DecodeFp4Args : DecodeArgs {
   int act_bf16;                // q and out are bf16
 };
 cudaError_t launch_decode_fp4(int gt, const DecodeFp4Args& a, int grid, cudaStream_t stream);
-cudaError_t launch_reduce_fp4(int gt, const ReduceArgs& a, bool bf16, int max_pieces,
-                              cudaStream_t stream);
 int decode_fp4_warps_per_cta(int gt);
 // Token-granular cache writes; kind selects the cache type.
 enum RowKind {

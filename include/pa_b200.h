@@ -151,8 +151,9 @@ int pa_splitk_fp8(void* out, const void* q, const void* k_cache, const void* v_c
 
 /* FP4 KV cache (layout above; written by pa_quantize_into_cache_fp4). Same arguments as
  * pa_decode_f16 / pa_splitk_f16. The other decode entry points (pa_decode_step, pa_decode_bf16q,
- * pa_decode_partial) take it as kv_dtype PA_DTYPE_FP4E2M1, without scales. No counterpart in the
- * reference. */
+ * pa_decode_partial) take it as kv_dtype PA_DTYPE_FP4E2M1, without scales. Both run the same
+ * kernel, which cuts long contexts itself (so does splitk elsewhere); pa_splitk_fp4 is there for
+ * callers that choose by shape whatever the cache. No counterpart in the reference. */
 int pa_decode_fp4(void* out, const void* q, const void* k_cache, const void* v_cache,
                   const int32_t* block_table, const int32_t* context_lens, int num_seqs,
                   int num_heads, int num_kv_heads, int head_dim, int num_blocks, int block_size,
