@@ -77,11 +77,11 @@ __device__ __forceinline__ void store4<float>(float* p, const float2 (&x)[2]) {
 // A row into the cache. The lane's chunks: values oa .. oa + 3 (x[0], x[1]) and ob .. ob + 3
 // (x[2], x[3]); `apart`: the chunks lie in different 16-value blocks, each shared by four
 // neighbouring lanes (else both in one block of two lanes; for the 4-bit cache rot is a multiple
-// of 32, so four neighbouring lanes agree). All sixteen lanes of the row call this together
-// (mask: the lanes of the warp that do).
+// of 32, so four neighbouring lanes agree). All lanes of the warp call this together; rows with
+// `ok` false are not stored.
 template <typename T, int KIND>
 __device__ __forceinline__ void cache_row(const float2 (&x)[4], int l, int oa, int ob, bool apart,
-                                          unsigned mask, bool is_v, void* cache, float* scales,
+                                          bool ok, bool is_v, void* cache, float* scales,
                                           size_t page, int off, int bs) {
   const float v[8] = {x[0].x, x[0].y, x[1].x, x[1].y, x[2].x, x[2].y, x[3].x, x[3].y};
   if constexpr (KIND == kRowsFP4) {
@@ -94,8 +94,8 @@ __device__ __forceinline__ void cache_row(const float2 (&x)[4], int l, int oa, i
     constexpr bool kWide = sizeof(T) == 4;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      uint32_t mc = max(m[c], __shfl_xor_sync(mask, m[c], 1));
-      const uint32_t far = __shfl_xor_sync(mask, mc, 2);
+      uint32_t mc = max(m[c], __shfl_xor_sync(0xffffffffu, m[c], 1));
+      const uint32_t far = __shfl_xor_sync(0xffffffffu, mc, 2);
       if (apart) mc = max(mc, far);
       const uint32_t sb = fp4::scale_byte<kWide>(mc);
       const float s = fp4::scale_value(sb), inv = fp4::scale_inverse<kWide>(sb);
@@ -103,9 +103,9 @@ __device__ __forceinline__ void cache_row(const float2 (&x)[4], int l, int oa, i
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e] = fp4::code_y<kWide>(v[4 * c + e], s, inv);
       const int o = c ? ob : oa;
-      *reinterpret_cast<uint16_t*>(grp + t * fp4::kCodeRow + o / 2) =
-          (uint16_t)(fp4::code_pair(y[0], y[1]) | (fp4::code_pair(y[2], y[3]) << 8));
-      if ((o & 15) == 0) grp[fp4::scale_offset(is_v, t, o / 16)] = (uint8_t)sb;
+      const uint32_t w = fp4::code_pair(y[0], y[1]) | (fp4::code_pair(y[2], y[3]) << 8);
+      if (ok) *reinterpret_cast<uint16_t*>(grp + t * fp4::kCodeRow + o / 2) = (uint16_t)w;
+      if (ok && (o & 15) == 0) grp[fp4::scale_offset(is_v, t, o / 16)] = (uint8_t)sb;
     }
   } else {
     float s = 0.f, inv = 0.f;
@@ -114,10 +114,11 @@ __device__ __forceinline__ void cache_row(const float2 (&x)[4], int l, int oa, i
 #pragma unroll
       for (int e = 0; e < 8; ++e) am = fmaxf(am, fabsf(v[e]));
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) am = fmaxf(am, __shfl_xor_sync(mask, am, o));
+      for (int o = 8; o > 0; o >>= 1) am = fmaxf(am, __shfl_xor_sync(0xffffffffu, am, o));
       s = KIND == kRowsI8 ? token_scale<T>(am) : __fdiv_rn(am, 448.f);
       inv = KIND == kRowsI8 ? __frcp_rn(s) : 0.f;
     }
+    if (!ok) return;
     constexpr int ES = KIND == kRowsF16 ? 2 : 1;
     uint8_t* c8 = static_cast<uint8_t*>(cache);
 #pragma unroll
@@ -172,7 +173,6 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeArgs a) {
   const int lane = threadIdx.x & 31;
   const int l = lane & 15;  // lane of the row
   const int half = lane >> 4;
-  const unsigned mask = 0xffffu << (16 * half);
   // Warps of a token: those of its q rows, then k, then v.
   const int qw = (a.H + 2 * kHeads - 1) / (2 * kHeads);
   const int kw = (a.KVH + 2 * kHeads - 1) / (2 * kHeads);
@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeArgs a) {
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
     const int h = h0 + 2 * i;
+    ra[i] = rb[i] = R{};  // the half-warp past an odd last head goes along with zeros
     if (h < heads) {
       ra[i] = load4(src + h * 128 + oa);
       rb[i] = load4(src + h * 128 + ob);
@@ -277,7 +278,8 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeArgs a) {
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
     const int h = h0 + 2 * i;
-    if (h >= heads) break;
+    if (h - half >= heads) break;
+    const bool ok = h < heads;
     float2 x[4];  // chunk a, chunk b
     {
       float2 xa[2], xb[2];
@@ -292,7 +294,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeArgs a) {
         for (int e = 1; e < 4; ++e) q2 = fma2(x[e], x[e], q2);
         float sum = q2.x + q2.y;
 #pragma unroll
-        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(mask, sum, o);
+        for (int o = 8; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const float r = rsqrtf(fmaf(sum, 1.f / 128.f, a.eps));
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] = mul2(x[e], make_float2(r, r));
@@ -321,15 +323,17 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeArgs a) {
       T* dst = is_q ? static_cast<T*>(a.q_out) + (size_t)n * a.qo_stride + h * 128
                     : static_cast<T*>(a.k_out) + (size_t)n * a.ko_stride + h * 128;
       const float2 lo[2] = {x[0], x[1]}, hi[2] = {x[2], x[3]};
-      store4(dst + oa, lo);
-      store4(dst + ob, hi);
+      if (ok) {
+        store4(dst + oa, lo);
+        store4(dst + ob, hi);
+      }
     } else if constexpr (kCache >= 0) {
       if (!is_v) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           x[e] = make_float2(In<T>::round_t(x[e].x), In<T>::round_t(x[e].y));
       }
-      cache_row<T, kCache>(x, l, oa, ob, apart, mask, is_v, is_v ? a.v_cache : a.k_cache,
+      cache_row<T, kCache>(x, l, oa, ob, apart, ok, is_v, is_v ? a.v_cache : a.k_cache,
                            is_v ? a.v_scales : a.k_scales, (size_t)page0 + h, off, a.bs);
     }
   }
