@@ -17,10 +17,11 @@
 //    half-warp, all loaded before the first is used. It folds the weights into the token's
 //    cosines and sines once: a' = r (a (c w_a) - b (s w_b)), r = 1/rms, three operations a value.
 //
-// Measured on a B200 (graph replay): 16384 tokens, 32/8 heads, bf16: 66 us, 5.2 TB/s, 0.79 of the
-// measured copy bandwidth (memory and issue slots both two thirds busy); 64 tokens: 2.4 us, a
-// launch and two dependent loads. CTAs of 256 threads instead of 128: 75 us; 40 registers a thread for
-// full occupancy: 80 us (spills).
+// Measured on a B200 (graph replay): 16384 tokens, 32/8 heads, bf16: 63.7 us, 5.4 TB/s, 0.82 of
+// the measured copy bandwidth (memory and issue slots both two thirds busy); 64 tokens: 2.4 us, a
+// launch and two dependent loads. CTAs of 256 threads instead of 128: 71 us; 40 registers a
+// thread for full occupancy: 76 us (spills); four rows' sums reduced together, with fewer
+// shuffles but all rows waited for at once: 65.6 us.
 //
 // The cache forms (kCache) round K to the rows' type first, so caches are bit for bit those of
 // the separate calls, then quantise as the cache writes do. One launch less for a step, and K's
@@ -359,7 +360,7 @@ cudaError_t launch_t(const RopeArgs& a, int sms, cudaStream_t st) {
   };
   // Four heads per half-warp where that still gives every SM sixteen warps, else one (each warp's
   // chain is then shorter). 32/8 heads, bf16, one and four heads: 256 tokens (1280 warps of four)
-  // 2.9 and 3.3 us, 512 tokens (2560) 4.5 and 3.7, 16384 tokens 105 and 66.
+  // 2.9 and 3.1 us, 512 tokens (2560) 4.5 and 3.8, 16384 tokens 102 and 62.
   if (warps(4) >= 16LL * sms) return launch_heads<T, kCache, 4>(a, warps(4), st);
   return launch_heads<T, kCache, 1>(a, warps(1), st);
 }
