@@ -62,11 +62,12 @@ struct Tile {
   static constexpr int PIECE = SLOT + D / 4;
   static constexpr size_t EARLY = (size_t)WARPS * PIECE * sizeof(float);
   static constexpr size_t SMEM = 128 + RING + EARLY;
-  static_assert((size_t)DEPTH * STAGE >= PIECE * sizeof(float), "a warp's ring holds its last piece");
+  static_assert((size_t)DEPTH * STAGE >= PIECE * sizeof(float),
+                "a warp's ring holds its last piece");
 };
 
-// Merges take bf16 output rows too, and pass NaN on (a block of the cache that holds one) instead of
-// taking it for an empty sequence. This file shares no code with decode.cu's: sharing it through a
+// Merges take bf16 output rows too, and pass NaN on (a block of the cache that holds one) instead
+// of taking it for an empty sequence. This file shares no code with decode.cu's: sharing it through a
 // header left its kernels' resources as they were but made the FP8 decode 2 % slower (66.3 -> 67.5
 // us at 64 x 8192 tokens, 12/2 heads).
 //
@@ -1180,7 +1181,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
 // Warps per CTA and ring stages per warp, by head tile (16 heads keep twice the accumulators).
 // 64 x 8192 / ragged 256 / 8 x 64-128 K tokens (12/2, 28/4 and 64/8 heads): 41.4 / 108.8 / 169.5 us
 // with sixteen warps of two stages (128 registers), 43.2 / 110.1 / 170.9 with twelve of two, 43.3 /
-// 110.7 / 171.6 with twelve of three, 43.2 / 119.7 / 184.2 with eight of four.
+// 110.7 / 171.6 with twelve of three, 43.2 / 119.7 / 184.2 with eight of four. Sixteen heads, 32/2,
+// 64 x 8192: 57.7 with eight warps (255 registers), 64.7 with twelve (spills).
 template <int GT> struct Shape;
 template <> struct Shape<8> { static constexpr int W = 16, DP = 2; };
 template <> struct Shape<16> { static constexpr int W = 8, DP = 4; };

@@ -268,10 +268,10 @@ def decode(out, q, k_cache, v_cache, block_table, context_lens, scale, block_siz
 
     The cache type follows the tensors: fp16; int8 or float8_e4m3fn, each with per-token fp32
     k_scales/v_scales (an int8 cache is assumed whenever scales are given); uint8 for a 4-bit
-    cache (fp4_cache), which holds its own scales. splitk
-    selects the partition + LSE-reduce kernel pair (512-token splits); otherwise, and always over
-    a 4-bit cache, the single-pass kernel with the fused combine runs. validate=False skips the one host sync
-    that checks context_lens (the kernels still flag bad lengths in the status word).
+    cache (fp4_cache), which holds its own scales. splitk selects the partition + LSE-reduce
+    kernel pair (512-token splits); otherwise, and always over a 4-bit cache, the single-pass
+    kernel with the fused combine runs. validate=False skips the one host sync that checks
+    context_lens (the kernels still flag bad lengths in the status word).
     kv_kind ('f16', 'i8', 'f8' or 'f4') pins the cache type instead of inferring it from the
     tensors, so a cache of another type is rejected (the reference-named ops use this).
     host_context_lens, a CPU tensor holding the same lengths (for instance the pinned copy the
