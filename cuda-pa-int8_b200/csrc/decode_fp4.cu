@@ -22,13 +22,13 @@
 //    error as the output's own.
 //  * steps of two full pages run in a loop with nothing to check; a step's scale and maximum are
 //    one multiply-add before the exponential (raw scores are compared with a threshold).
-// 277 warp instructions a page (479 with decode.cu's loop): 64 conversions, 64 multiplies, 24
+// 280 warp instructions a page (479 with decode.cu's loop): 64 conversions, 64 multiplies, 24
 // MMAs, 16 to pair the codes of neighbouring tokens for PV, the rest softmax, copies and loop.
 // Measured on a B200 (graph replay): 64 x 8192 tokens, 12/2 heads 41.3 us (3.67 TB/s); 8 x 64-128
-// K, 64/8 heads 167 us (5.43 TB/s, 0.83 of the measured copy bandwidth). With twelve warps the loop
-// took 467 cycles a page and scheduler, of which the ALU pipe (conversions, logic) was busy for
-// 255, the tensor pipe for 192 and the multiplies for 180; the three hardly overlap (a group of
-// one MMA and three of each takes 18.6 cycles where the MMA alone takes 8 and the others 8). The
+// K, 64/8 heads 167 us (5.43 TB/s, 0.83 of the measured copy bandwidth). That is 463 cycles a page
+// and scheduler, of which ALU instructions (conversions, logic) take 247, MMAs 192 and the FMA pipe
+// up to 189; they hardly overlap (a group of one MMA and three conversions and multiplies takes
+// 18.6 cycles where the MMA alone takes 8 and the others 8). Shifts turned into multiplies, the
 // QK of the next step issued between the PV of this one, two chains of QK MMAs a page instead of
 // one, and a choice of refill inside one loop for all full pages measured no better.
 
