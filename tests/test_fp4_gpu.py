@@ -568,3 +568,35 @@ def test_merges_inside_and_across_ctas(lens, H, KVH):
     _ops().merge_partials(merged, part[None], H, KVH)
     _close(merged, c)
     _ops().check_status(q.device)
+
+
+def test_empty_calls():
+    """No tokens, no sequences: nothing is launched or refused."""
+    ops = _ops()
+    kc, vc = ops.fp4_cache(2, 2)
+    half, i32 = dict(dtype=torch.float16, device="cuda"), dict(dtype=torch.int32, device="cuda")
+    rows, none = torch.zeros(0, 2, 128, **half), torch.zeros(0, **i32)
+    ops.quantize_into_cache_fp4(rows, rows, kc, vc, none)
+    k, v = ops.read_from_cache_fp4(kc, vc, none)
+    assert k.shape == v.shape == (0, 2, 128)
+    q, bt = torch.zeros(0, 4, 128, **half), torch.zeros(0, 3, **i32)
+    out = torch.empty_like(q)
+    ops.decode(out, q, kc, vc, bt, none, 0.1)
+    ops.decode_bf16(out.bfloat16(), q.bfloat16(), kc, vc, bt, none, 0.1)
+    ops.decode_step(out, q, rows, rows, kc, vc, bt, none, 0.1)
+    ops.decode_partial(q, kc, vc, bt, none, 0.1)
+    table = ops.rope_table(4)
+    q2, k2 = ops.qk_norm_rope(q, rows, None, None, none, table)
+    assert q2.shape == q.shape and k2.shape == rows.shape
+    ops.norm_rope_into_cache(q, rows, rows, None, None, none, table, kc, vc, none)
+    free, count = torch.arange(2, **i32), torch.full((1,), 2, **i32)
+    lens, n = ops.release_blocks(bt, none, none, free, count)
+    assert lens.numel() == 0 and n.item() == 2
+    slots, pos, start, lens, n = ops.extend_block_tables(bt, none, none, free, count, 2,
+                                                         max_tokens=0)
+    assert slots.numel() == pos.numel() == lens.numel() == 0
+    assert start.tolist() == [0] and n.item() == 2
+    slots, pos, *_ = ops.extend_block_tables(bt, none, none, free, count, 2, max_tokens=3)
+    assert slots.tolist() == pos.tolist() == [-1] * 3
+    assert bool((kc == 0).all()) and bool((vc == 0).all())
+    ops.check_status(kc.device)
