@@ -143,7 +143,7 @@ def _check_lengths(context_lens, capacity, host_context_lens=None):
         cl = context_lens.cpu()
     if cl.numel() == 0:
         return
-    if cl.numel() <= 32:  # a list costs less than numpy's reductions: 1.2 us against 3.4 for 4
+    if cl.dim() == 1 and cl.numel() <= 32:  # for 4 lengths 1.2 us; numpy's reductions 3.4
         v = cl.tolist()
         low, high = min(v), max(v)
     else:

@@ -198,3 +198,15 @@ def test_decodes_refuse_an_empty_block_size(lib):
         for bs in (0, -16):
             assert fn(P, P, P, P, P, P, 1, 8, 2, 128, 4, bs, 2, 0.1, P, 1 << 30,
                       None) == _lib.PA_ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("n", [1, 4, 32, 33, 200])
+def test_lengths_are_checked_alike_through_a_list_and_numpy(n):
+    good = torch.full((n,), 7, dtype=torch.int32)
+    for shape in ((n,), (n, 1)):
+        ops._check_lengths(good, 7, good.view(shape))
+        for bad in (0, 8, -1):
+            x = good.clone()
+            x[n // 2] = bad
+            with pytest.raises(RuntimeError):
+                ops._check_lengths(good, 7, x.view(shape))
