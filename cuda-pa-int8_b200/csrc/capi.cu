@@ -24,6 +24,12 @@ namespace {
 
 thread_local std::string g_err;
 
+// The status word that pa_device_status() gives out: one on every device, zero from the start and
+// never moved, so that a captured graph may hold its address.
+__device__ int g_device_status;
+
+__global__ void clear_bits_kernel(int* status, int bits) { atomicAnd(status, ~bits); }
+
 int vfail(int code, const char* fmt, va_list ap) {
   char buf[512];
   vsnprintf(buf, sizeof(buf), fmt, ap);
@@ -550,9 +556,24 @@ int pa_read_status(void* workspace, int* status_out, void* stream) {
   int h = 0;
   cudaError_t e = cudaMemcpyAsync(&h, workspace, sizeof(int), cudaMemcpyDeviceToHost, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-  if (e == cudaSuccess) e = cudaMemsetAsync(workspace, 0, sizeof(int), st);
+  if (e == cudaSuccess && h != 0) {
+    // Only the bits that are reported, so that none set since on another stream is lost, and
+    // before this returns, so that none set by later work is.
+    clear_bits_kernel<<<1, 1, 0, st>>>(static_cast<int*>(workspace), h);
+    e = cudaGetLastError();
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  }
   if (e != cudaSuccess) return cuda_fail(e, "status read");
   *status_out = h;
+  return PA_OK;
+}
+
+int pa_device_status(int** status_out) {
+  if (status_out == nullptr) return fail(PA_ERR_INVALID_ARG, "null pointer argument");
+  void* p = nullptr;
+  cudaError_t e = cudaGetSymbolAddress(&p, g_device_status);
+  if (e != cudaSuccess) return cuda_fail(e, "status word of the device");
+  *status_out = static_cast<int*>(p);
   return PA_OK;
 }
 

@@ -3,9 +3,10 @@
 Each op checks its arguments with the error conditions of the reference launchers
 (kernels/paged_attention_v4_splitk.cu:197-205, kernels/paged_attention_v6_splitk_int8.cu:
 201-221 and siblings) and raises RuntimeError like their TORCH_CHECKs, then calls the
-library on the current CUDA stream of the tensors' device. Temporaries (split partials,
-arrival counters, the device status word) live in a per-(device, stream) workspace that is
-zero-filled once when allocated and kept for later calls.
+library on the current CUDA stream of the tensors' device. Temporaries of the decodes (split
+partials, arrival counters, their status word) live in a per-(device, stream) workspace that is
+zero-filled once when allocated and kept for later calls; the other kernels set the library's own
+status word of the device.
 """
 
 import ctypes
@@ -24,6 +25,8 @@ _DTYPE_CODE = {
 }
 
 _workspaces = {}
+_outgrown = []      # (key, workspace) replaced inside a capture, where its status cannot be carried
+_status_words = {}  # device index -> address of the library's status word there
 
 
 def _ptr(t):
@@ -45,35 +48,66 @@ def workspace(device, nbytes):
 
     Growing replaces the buffer, and a CUDA graph keeps the address it captured: run the
     largest shape once on a stream before capturing graphs on it, so no later call on that
-    stream replaces the buffer a graph uses."""
+    stream replaces the buffer a graph uses. The status word moves along with a grown
+    workspace, so bits that were set and not read yet stay."""
     stream = _stream(device)
     key = (device.index, stream)
     ws = _workspaces.get(key)
     nbytes = max(int(nbytes), 256)
     if ws is None or ws.numel() < nbytes:
+        old = ws
         ws = torch.zeros(nbytes, dtype=torch.uint8, device=device)
+        if old is not None:
+            if torch.cuda.is_current_stream_capturing():
+                _outgrown.append((key, old))  # a captured copy would run again in every replay
+            else:
+                ws[:4].copy_(old[:4])
         _workspaces[key] = ws
     return ws
 
 
+def _status_word(device):
+    """Address of the library's own status word on `device`, the current one: for the kernels that
+    use nothing else of a workspace. It never moves, so graphs may hold it."""
+    p = _status_words.get(device.index)
+    if p is None:
+        out = ctypes.c_void_p()
+        _lib.check(_lib.lib().pa_device_status(ctypes.byref(out)), "pa_device_status")
+        p = _status_words[device.index] = out.value
+    return p
+
+
 def read_status(device=None):
-    """OR of the device status words of this device's workspaces, which are then cleared
-    (synchronises). Bits are the PA_ERR_* codes of include/pa_b200.h. A workspace that
-    reports an error also gets its arrival counters zeroed, since a kernel that stopped
-    part-way can leave some of them set."""
-    device = torch.device("cuda", torch.cuda.current_device()) if device is None else device
+    """OR of this device's status words (the library's own and those of its workspaces), which are
+    then cleared. Waits for all work on the device first. Bits are the PA_ERR_* codes of
+    include/pa_b200.h. A workspace that reports an error also gets its arrival counters zeroed,
+    since a kernel that stopped part-way can leave some of them set."""
+    if device is None or device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
     status = 0
     L = _lib.lib()
-    for (idx, stream), ws in list(_workspaces.items()):
-        if idx != device.index:
-            continue
-        out = ctypes.c_int(0)
-        _lib.check(L.pa_read_status(ws.data_ptr(), ctypes.byref(out), stream), "pa_read_status")
-        if out.value:
-            _lib.check(L.pa_reset_workspace(ws.data_ptr(), ws.numel(), stream),
-                       "pa_reset_workspace")
-            torch.cuda.synchronize(device)
-        status |= out.value
+    with _Guard(device):
+        # A graph runs on another stream than the one it was captured on, whose key its
+        # workspace has.
+        torch.cuda.synchronize(device)
+
+        def read(address, stream):
+            out = ctypes.c_int(0)
+            _lib.check(L.pa_read_status(address, ctypes.byref(out), stream), "pa_read_status")
+            return out.value
+
+        word = _status_words.get(device.index)
+        if word is not None:
+            status |= read(word, _stream(device))
+        for (idx, stream), ws in list(_workspaces.items()) + _outgrown:
+            if idx != device.index:
+                continue
+            bits = read(ws.data_ptr(), stream)
+            if bits:
+                _lib.check(L.pa_reset_workspace(ws.data_ptr(), ws.numel(), stream),
+                           "pa_reset_workspace")
+                torch.cuda.synchronize(device)
+            status |= bits
     return status
 
 
@@ -533,9 +567,9 @@ def merge_partials(out, partials, num_heads, num_kv_heads):
              "partials must be fp32 [num_parts, num_seqs, per_seq_floats]")
     _require(partials.device == out.device, "partials and out must be on the same device")
     with _Guard(out.device):
-        ws = workspace(out.device, 256)
+        status = _status_word(out.device)
         rc = _lib.lib().pa_merge_partials(out.data_ptr(), partials.data_ptr(), P, B, num_heads,
-                                          num_kv_heads, HEAD_DIM, ws.data_ptr(),
+                                          num_kv_heads, HEAD_DIM, status,
                                           _stream(out.device))
         _lib.check(rc, "merge partials")
     return out
@@ -612,20 +646,20 @@ def quantize_into_cache(key, value, k_cache, v_cache, k_scales, v_scales, slot_m
             _require(t.dtype == torch.float32 and t.numel() == 1 and t.device == key.device,
                      "fixed scales must be one fp32 element on the key's device")
     with _Guard(key.device):
-        ws = workspace(key.device, 256)
+        status = _status_word(key.device)
         if fp8:
             rc = _lib.lib().pa_quantize_into_cache_fp8(
                 key.data_ptr(), value.data_ptr(), _DTYPE_CODE[key.dtype], key.stride(0),
                 slot_mapping.data_ptr(), N, KVH, D, k_cache.data_ptr(), v_cache.data_ptr(),
                 k_scales.data_ptr(), v_scales.data_ptr(), k_cache.shape[0], block_size,
-                ws.data_ptr(), _stream(key.device))
+                status, _stream(key.device))
             _lib.check(rc, "quantize_into_cache (fp8)")
             return
         rc = _lib.lib().pa_quantize_into_cache(
             key.data_ptr(), value.data_ptr(), _DTYPE_CODE[key.dtype], key.stride(0),
             slot_mapping.data_ptr(), N, KVH, D, k_cache.data_ptr(), v_cache.data_ptr(),
             k_scales.data_ptr(), v_scales.data_ptr(), k_cache.shape[0], block_size,
-            _ptr(k_scale), _ptr(v_scale), ws.data_ptr(), _stream(key.device))
+            _ptr(k_scale), _ptr(v_scale), status, _stream(key.device))
         _lib.check(rc, "quantize_into_cache")
 
 
@@ -643,11 +677,11 @@ def write_into_cache(key, value, k_cache, v_cache, slot_mapping, block_size=16):
         _require(t.is_contiguous() and t.device == key.device,
                  "cache tensors must be contiguous and on the key's device")
     with _Guard(key.device):
-        ws = workspace(key.device, 256)
+        status = _status_word(key.device)
         rc = _lib.lib().pa_write_into_cache_f16(
             key.data_ptr(), value.data_ptr(), _DTYPE_CODE[key.dtype], key.stride(0),
             slot_mapping.data_ptr(), N, KVH, D, k_cache.data_ptr(), v_cache.data_ptr(),
-            k_cache.shape[0], block_size, ws.data_ptr(), _stream(key.device))
+            k_cache.shape[0], block_size, status, _stream(key.device))
         _lib.check(rc, "write_into_cache")
 
 
@@ -679,13 +713,13 @@ def prefill_into_cache(k, v, k_cache, v_cache, block_table, context_lens, block_
         _require(t.is_contiguous() and t.device == k.device,
                  "cache tensors must be contiguous and on k's device")
     with _Guard(k.device):
-        ws = workspace(k.device, 256)
+        status = _status_word(k.device)
         rc = _lib.lib().pa_prefill_into_cache(
             k.data_ptr(), v.data_ptr(), _DTYPE_CODE[k.dtype], S, Lmax, KVH, D,
             block_table.data_ptr(), context_lens.data_ptr(), block_table.shape[1],
             _lib.PA_DTYPE_I8 if int8 else _lib.PA_DTYPE_F16, k_cache.data_ptr(),
             v_cache.data_ptr(), _ptr(k_scales), _ptr(v_scales), k_cache.shape[0], block_size,
-            _ptr(k_scale), _ptr(v_scale), ws.data_ptr(), _stream(k.device))
+            _ptr(k_scale), _ptr(v_scale), status, _stream(k.device))
         _lib.check(rc, "prefill_into_cache")
 
 
@@ -744,7 +778,7 @@ def quantize_into_cache_fp4(key, value, k_cache, v_cache, slot_mapping, block_si
             key.data_ptr(), value.data_ptr(), _DTYPE_CODE[dt],
             stride[0] if N > 1 else KVH * D, slot_mapping.data_ptr(), N, KVH, D,
             k_cache.data_ptr(), v_cache.data_ptr(), NB,
-            block_size, workspace(dev, 256).data_ptr(), _stream(dev))
+            block_size, _status_word(dev), _stream(dev))
         _lib.check(rc, "quantize_into_cache (fp4)")
 
 
@@ -777,7 +811,7 @@ def read_from_cache_fp4(k_cache, v_cache, slot_mapping, block_size=16, *, dtype=
         rc = _lib.lib().pa_read_from_cache_fp4(
             key.data_ptr(), value.data_ptr(), _DTYPE_CODE[key.dtype], k_cache.data_ptr(),
             v_cache.data_ptr(), slot_mapping.data_ptr(), N, KVH, HEAD_DIM, NB, block_size,
-            workspace(dev, 256).data_ptr(), _stream(dev))
+            _status_word(dev), _stream(dev))
         _lib.check(rc, "read_from_cache (fp4)")
     return key, value
 
@@ -865,7 +899,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, table, *, eps=1e-6, interl
             q_out.data_ptr(), qos, k_out.data_ptr(), kos, q.data_ptr(), qs, k.data_ptr(), ks,
             _DTYPE_CODE[dt], _ptr(q_weight), _ptr(k_weight), eps, positions.data_ptr(),
             table.data_ptr(), table.shape[0], table.shape[1], 1 if interleaved else 0, N, H, KVH,
-            HEAD_DIM, workspace(dev, 256).data_ptr(), _stream(dev))
+            HEAD_DIM, _status_word(dev), _stream(dev))
         _lib.check(rc, "qk_norm_rope")
     return q_out, k_out
 
@@ -913,7 +947,7 @@ def norm_rope_into_cache(q, k, v, q_weight, k_weight, positions, table, k_cache,
             table.data_ptr(), table.shape[0], table.shape[1], 1 if interleaved else 0,
             slot_mapping.data_ptr(), N, H, KVH, HEAD_DIM, _KV_CODE[kind], k_cache.data_ptr(),
             v_cache.data_ptr(), _ptr(k_scales), _ptr(v_scales), NB, block_size,
-            workspace(dev, 256).data_ptr(), _stream(dev))
+            _status_word(dev), _stream(dev))
         _lib.check(rc, "norm_rope_into_cache")
     return q_out
 
@@ -966,11 +1000,11 @@ def release_blocks(block_table, context_lens, finished, free_blocks, free_count,
     else:
         _check_int(dev, ("free_count_out", count, 1))
     with _Guard(dev):
-        ws = workspace(dev, 256)
+        status = _status_word(dev)
         rc = _lib.lib().pa_release_blocks(
             block_table.data_ptr(), context_lens.data_ptr(), finished.data_ptr(),
             free_blocks.data_ptr(), free_count.data_ptr(), lens.data_ptr(), count.data_ptr(), S,
-            max_blocks, block_size, free_blocks.numel(), ws.data_ptr(), _stream(dev))
+            max_blocks, block_size, free_blocks.numel(), status, _stream(dev))
         _lib.check(rc, "release_blocks")
     return lens, count
 
@@ -1007,12 +1041,12 @@ def extend_block_tables(block_table, context_lens, new_lens, free_blocks, free_c
             _check_int(dev, (names[i], outs[i], n))
     slot_mapping, positions, query_start, lens, count = outs
     with _Guard(dev):
-        ws = workspace(dev, 256)
+        status = _status_word(dev)
         rc = _lib.lib().pa_extend_block_tables(
             block_table.data_ptr(), context_lens.data_ptr(), new_lens.data_ptr(),
             free_blocks.data_ptr(), free_count.data_ptr(), lens.data_ptr(), count.data_ptr(),
             slot_mapping.data_ptr(), positions.data_ptr(), query_start.data_ptr(), S, max_blocks,
-            block_size, free_blocks.numel(), num_blocks, max_tokens, ws.data_ptr(), _stream(dev))
+            block_size, free_blocks.numel(), num_blocks, max_tokens, status, _stream(dev))
         _lib.check(rc, "extend_block_tables")
     return slot_mapping, positions, query_start, lens, count
 

@@ -86,8 +86,14 @@ size_t pa_decode_workspace_bytes(int num_seqs, int num_heads, int num_kv_heads, 
                                  int max_blocks_per_seq, int block_size, int kv_dtype,
                                  int splitk);
 
-/* Read the device status word of a workspace (synchronises `stream`), then clear it. */
+/* Read the status word of a workspace (or another status word), then clear the bits that were
+ * set. Synchronises `stream`; work on other streams is not waited for. */
 int pa_read_status(void* workspace, int* status_out, void* stream);
+
+/* The library's own status word on the current device, for the calls below that take `status`
+ * and no workspace. Zero when the library is loaded; it stays in place until the process ends, so
+ * graphs may hold it. pa_read_status() reads it. */
+int pa_device_status(int** status_out);
 
 /* Zero a workspace's status word and arrival counters (its first min(workspace_bytes,
  * 256 B + 1 MiB) bytes) on `stream`. A decode that stopped part-way on a device error (a
