@@ -180,6 +180,8 @@ __device__ __noinline__ bool staged_combine(const float* part, int wf, int np, i
 // shared memory) and the denominators with every thread reading a different piece; pass 2
 // gives each thread one float4 of the [D][GT] output and U pieces' loads in flight per step,
 // so a merge costs a handful of dependent L2 round trips however many pieces there are.
+// pass_nan: a NaN among the sums reaches the output rows; else such a row reads as an empty
+// sequence, zeros and a flag, as in staged_combine.
 // ---------------------------------------------------------------------------------------
 template <int D, int GT, int NTHR, int U>
 struct Coop {
@@ -195,7 +197,8 @@ struct Coop {
 
 template <int D, int GT, int NTHR, int U, typename PieceFn>
 __device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __half* out_rows,
-                                             float* out_slot, int* status, float* sm) {
+                                             float* out_slot, int* status, float* sm,
+                                             bool pass_nan = false) {
   using CC = Coop<D, GT, NTHR, U>;
   static_assert(NTHR >= CC::OUT4 || CC::OUT4 % NTHR == 0, "outputs must tile the block");
   const int tid = threadIdx.x;
@@ -312,6 +315,7 @@ __device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __
       }
     }
   }
+  auto empty = [&](float L) { return pass_nan ? L == 0.f : !(L > 0.f); };
   if (pg == 0) {
 #pragma unroll
     for (int i = 0; i < CC::OPT; ++i) {
@@ -325,7 +329,7 @@ __device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __
           const int h = h0 + e;
           if (h < hcnt) {
             const float L = sL[h];
-            out_rows[(size_t)h * D + d] = __float2half_rn(L > 0.f ? a4[e] / L : 0.f);
+            out_rows[(size_t)h * D + d] = __float2half_rn(empty(L) ? 0.f : a4[e] / L);
           }
         }
       } else {
@@ -337,7 +341,7 @@ __device__ __forceinline__ void coop_combine(PieceFn piece, int np, int hcnt, __
     if (out_slot != nullptr) {
       out_slot[D * GT + tid] = sM[tid];
       out_slot[D * GT + GT + tid] = sL[tid];
-    } else if (tid < hcnt && !(sL[tid] > 0.f)) {
+    } else if (tid < hcnt && empty(sL[tid])) {
       flag_error(status, PA_ERR_EMPTY_CONTEXT);
     }
   }
@@ -1465,9 +1469,10 @@ __global__ void __launch_bounds__(kReduceThreads, 1) reduce_kernel(const ReduceA
     return;
   }
   const float* base = a.part + (size_t)segid * a.seg_stride;
+  // Partials from several GPUs may hold NaN (a 4-bit cache's block of a NaN or an infinity).
   coop_combine<D, GT, kReduceThreads, 16>(
       [&](int k) { return base + (size_t)k * a.piece_stride; }, np, hcnt, orow, nullptr,
-      a.status, rsm);
+      a.status, rsm, a.num_parts > 0);
 }
 
 // Launch shapes per (cache dtype, head tile): warps per CTA (one CTA per SM) and ring depth
