@@ -32,6 +32,8 @@
 #include "pa_internal.h"
 #include "pa_rows.cuh"
 
+#include <type_traits>
+
 namespace pa {
 namespace {
 
@@ -74,6 +76,24 @@ template <>
 __device__ __forceinline__ void store4<float>(float* p, const float2 (&x)[2]) {
   *reinterpret_cast<float4*>(p) = make_float4(x[0].x, x[0].y, x[1].x, x[1].y);
 }
+
+// a * b + c where `on`, else c, without a branch.
+__device__ __forceinline__ float2 fma2_if(bool on, float2 a, float2 b, float2 c) {
+  asm("{\n\t.reg .pred t;\n\t.reg .b64 x, y, z;\n\t"
+      "setp.ne.s32 t, %6, 0;\n\t"
+      "mov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%0, %1};\n\t"
+      "@t fma.rn.f32x2 z, x, y, z;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}"
+      : "+f"(c.x), "+f"(c.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "r"((int)on));
+  return c;
+}
+
+// CTAs an SM of the partly turned kernels of many 16-bit tokens, so that they keep to the 56
+// registers of the others (4099 tokens, 28/4 heads, half the head, interleaved: 18.3 us without the
+// bound, 17.6 with it).
+template <typename T, int kCache, int kHeads, bool kWhole>
+constexpr int kMinCtas = !kWhole && kCache < 0 && kHeads == 4 && sizeof(T) == 2 ? 9 : 0;
 
 // A row into the cache. The lane's chunks: values oa .. oa + 3 (x[0], x[1]) and ob .. ob + 3
 // (x[2], x[3]); `apart`: the chunks lie in different 16-value blocks, each shared by four
@@ -167,9 +187,14 @@ __device__ __forceinline__ void cache_row(const float2 (&x)[4], int l, int oa, i
 }
 
 // kCache: the cache's RowKind, or -1 for k rows written to k_out (and no V). kInter: pairs
-// (2i, 2i + 1).
-template <typename T, int kCache, int kHeads, bool kInter>
-__global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeArgs a) {
+// (2i, 2i + 1). kWhole: rot is 128, every lane's values turn. Where rot is less, the other lanes'
+// values are only scaled: with a sine of zero instead, a neighbour's infinity would make them NaN.
+// 16384 tokens, 32/8 heads, bf16, half the head: 64-66 us with a branch, 67.6 with a predicate
+// (interleaved, with the predicate, 62.7-65), 62-64 with the zero; whole heads, which need neither,
+// 62.4 and, by a kernel for both, 65-71.
+template <typename T, int kCache, int kHeads, bool kInter, bool kWhole>
+__global__ void __launch_bounds__(kThreads, kMinCtas<T, kCache, kHeads, kWhole>)
+norm_rope_kernel(const RopeArgs a) {
   using R = typename Raw<T>::type;
   const int lane = threadIdx.x & 31;
   const int l = lane & 15;  // lane of the row
@@ -190,7 +215,8 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeArgs a) {
 
   // The lane's chunks.
   const int turning = is_v ? 0 : a.rot >> 3;  // lanes whose values turn
-  const bool apart = !kInter && l < turning;
+  const bool turns = l < turning;
+  const bool apart = !kInter && turns;
   const int oa = apart ? 4 * l : 8 * l;
   const int ob = apart ? (a.rot >> 1) + 4 * l : 8 * l + 4;
 
@@ -247,7 +273,7 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeArgs a) {
       wa[0] = wa[1] = wb[0] = wb[1] = make_float2(1.f, 1.f);
     }
     float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (l < turning) {
+    if (turns) {
       const float* row = a.table + (size_t)pos * a.rot + 4 * l;
       c = __ldg(reinterpret_cast<const float4*>(row));
       s = __ldg(reinterpret_cast<const float4*>(row + (a.rot >> 1)));
@@ -305,10 +331,18 @@ __global__ void __launch_bounds__(kThreads) norm_rope_kernel(const RopeArgs a) {
         for (int e = 0; e < 2; ++e) {
           const float2 p = make_float2(x[2 * e].x, x[2 * e + 1].x);
           const float2 q = make_float2(x[2 * e].y, x[2 * e + 1].y);
-          const float2 u = fma2(q, su[e], mul2(p, cu[e]));
-          const float2 v = fma2(p, sv[e], mul2(q, cv[e]));
+          const float2 u = kWhole ? fma2(q, su[e], mul2(p, cu[e]))
+                                  : fma2_if(turns, q, su[e], mul2(p, cu[e]));
+          const float2 v = kWhole ? fma2(p, sv[e], mul2(q, cv[e]))
+                                  : fma2_if(turns, p, sv[e], mul2(q, cv[e]));
           x[2 * e] = make_float2(u.x, v.x);
           x[2 * e + 1] = make_float2(u.y, v.y);
+        }
+      } else if (!kWhole && !turns) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          x[e] = mul2(x[e], cu[e]);
+          x[2 + e] = mul2(x[2 + e], cv[e]);
         }
       } else {
 #pragma unroll
@@ -344,10 +378,16 @@ template <typename T, int kCache, int kHeads>
 cudaError_t launch_heads(const RopeArgs& a, long long warps, cudaStream_t st) {
   const long long grid = (warps + kThreads / 32 - 1) / (kThreads / 32);
   if (warps > 0x7fffffffLL) return cudaErrorInvalidValue;
-  if (a.interleaved) {
-    norm_rope_kernel<T, kCache, kHeads, true><<<(int)grid, kThreads, 0, st>>>(a);
+  auto launch = [&](auto inter, auto whole) {
+    norm_rope_kernel<T, kCache, kHeads, decltype(inter)::value, decltype(whole)::value>
+        <<<(int)grid, kThreads, 0, st>>>(a);
+  };
+  using Yes = std::true_type;
+  using No = std::false_type;
+  if (a.rot == 128) {
+    if (a.interleaved) launch(Yes{}, Yes{}); else launch(No{}, Yes{});
   } else {
-    norm_rope_kernel<T, kCache, kHeads, false><<<(int)grid, kThreads, 0, st>>>(a);
+    if (a.interleaved) launch(Yes{}, No{}); else launch(No{}, No{});
   }
   return cudaGetLastError();
 }
