@@ -47,6 +47,12 @@ template <typename T>
 __device__ __forceinline__ typename Raw<T>::type load4(const T* p) {
   return __ldg(reinterpret_cast<const typename Raw<T>::type*>(p));
 }
+// Of q, k and v rows: a plain load, since the outputs may be the inputs and __ldg is for memory
+// that nothing writes during the launch.
+template <typename T>
+__device__ __forceinline__ typename Raw<T>::type load4_row(const T* p) {
+  return *reinterpret_cast<const typename Raw<T>::type*>(p);
+}
 __device__ __forceinline__ void widen(uint2 u, const __half*, float2 (&x)[2]) {
   x[0] = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
   x[1] = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
@@ -229,8 +235,8 @@ norm_rope_kernel(const RopeArgs a) {
     const int h = h0 + 2 * i;
     ra[i] = rb[i] = R{};  // the half-warp past an odd last head goes along with zeros
     if (h < heads) {
-      ra[i] = load4(src + h * 128 + oa);
-      rb[i] = load4(src + h * 128 + ob);
+      ra[i] = load4_row(src + h * 128 + oa);
+      rb[i] = load4_row(src + h * 128 + ob);
     }
   }
 
