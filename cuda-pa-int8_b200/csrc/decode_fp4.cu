@@ -738,6 +738,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
         thr[nt][e] = neg_inf();
         fl[nt][e] = 0.f;
       }
+    bool far = false;  // a maximum past 2^18: see the step
     // One step: the two pages of stage s. FULL: all their tokens count; else valid0 and valid1 of
     // them do (where a piece begins or ends inside a stage, the page that is not its own has
     // none, and is met again by the other piece).
@@ -804,7 +805,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
       // The reference maximum moves only when a score passes it by 2^kLazy: weights then stay
       // below 2^(kPExp + kLazy) (far inside fp16), O and l carry the same factor, and most
       // steps need neither a reduction over the lanes nor a rescale.
-      constexpr float kLazy = 8.f;
+      constexpr float kLazy = 8.f, kFar = 0x1p18f;
       float tm[NT][2];
       bool up = false;
 #pragma unroll
@@ -816,6 +817,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
           up = up || tm[nt][e] > thr[nt][e];
         }
       if (__any_sync(0xffffffffu, up)) {
+        bool is_far = false;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float c[2];
@@ -824,10 +826,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
             float v = tm[nt][e];
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-            const float m = kPExp - fmb[nt][e], mn = fmaxf(m, ceilf(v * qs));
-            c[e] = mn > m ? ex2(m - mn) : 1.f;
-            fmb[nt][e] = kPExp - mn;
-            thr[nt][e] = __fdividef(mn + kLazy, qs);
+            // The maximum, as fmb, moves up only. From 2^kFar on, where the threshold's own
+            // rounding would let weights overflow, every new maximum moves it.
+            const float f = fminf(fmb[nt][e], kPExp - ceilf(__fmul_rn(v, qs)));
+            c[e] = f < fmb[nt][e] ? ex2(f - fmb[nt][e]) : 1.f;
+            fmb[nt][e] = f;
+            is_far = is_far || !(fabsf(f) < kFar);
+            thr[nt][e] = fabsf(f) < kFar ? __fdividef(kPExp - f + kLazy, qs)
+                                         : fmaxf(thr[nt][e], v);
             fl[nt][e] *= c[e];
             if constexpr (PACK) {  // columns 4-7 belong to the heads of columns 0-3
               const float other = __shfl_xor_sync(0xffffffffu, c[e], 2);
@@ -842,8 +848,18 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
             oacc[i][nt][3] *= c[1];
           }
         }
+        far = __any_sync(0xffffffffu, is_far);
       }
 
+      // Far: the product rounds as the maximum's did, so that even where scores have no bits below
+      // 1 left the largest weight is near 2^kPExp. (Scalar multiplications: packed ones and the
+      // addition would be fused.) The branch costs 0.8 % of 8 x 64-128 K tokens, 64/8 heads, two
+      // operations a score in every step 1.7 %.
+      auto weight_arg = [&](float a, float b, int nt) {
+        const float2 f = make_float2(fmb[nt][0], fmb[nt][1]);
+        if (far) return add2(make_float2(__fmul_rn(a, qs), __fmul_rn(b, qs)), f);
+        return fma2(make_float2(a, b), make_float2(qs, qs), f);
+      };
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         // Weights, as two fp16 parts each (about 22 significant bits, as for the other
@@ -854,8 +870,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
           float p[4];
 #pragma unroll
           for (int e = 0; e < 4; e += 2) {
-            const float2 v = fma2(make_float2(x[u][nt][e], x[u][nt][e + 1]),
-                                  make_float2(qs, qs), make_float2(fmb[nt][0], fmb[nt][1]));
+            const float2 v = weight_arg(x[u][nt][e], x[u][nt][e + 1], nt);
             p[e] = ex2(v.x);
             p[e + 1] = ex2(v.y);
             const float2 l = add2(make_float2(fl[nt][0], fl[nt][1]),
