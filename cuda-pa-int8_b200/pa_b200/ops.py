@@ -822,6 +822,7 @@ def read_from_cache_fp4(k_cache, v_cache, slot_mapping, block_size=16, *, dtype=
 def rope_table(num_positions, rot_dim=HEAD_DIM, base=10000.0, device="cuda"):
     """Rotation table [num_positions, rot_dim] fp32: cos(p * base^(-2i/rot_dim)) for i <
     rot_dim/2, then the sines. Angles are formed in 64 bits (far positions lose them in 32)."""
+    _require(rot_dim > 0 and rot_dim % 2 == 0, "rot_dim must be even: values turn in pairs")
     inv = float(base) ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64, device=device) /
                           rot_dim)
     ang = torch.arange(num_positions, dtype=torch.float64, device=device)[:, None] * inv
