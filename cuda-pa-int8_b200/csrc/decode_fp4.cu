@@ -738,11 +738,11 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
         thr[nt][e] = neg_inf();
         fl[nt][e] = 0.f;
       }
-    bool far = false;  // a maximum past 2^18: see the step
+    bool far = false;  // a maximum is far from zero: see the step
     // One step: the two pages of stage s. FULL: all their tokens count; else valid0 and valid1 of
     // them do (where a piece begins or ends inside a stage, the page that is not its own has
-    // none, and is met again by the other piece).
-    auto step = [&](auto full, int s, int valid0, int valid1) {
+    // none, and is met again by the other piece). False: nothing was done, the step needs !FULL.
+    auto step = [&](auto full, int s, int valid0, int valid1) -> bool {
       constexpr bool FULL = decltype(full)::value;
       const uint32_t st = my_ring + (uint32_t)s * (uint32_t)C::STAGE;
       const uint32_t ka = st + tau * fp4::kCodeRow + 16 * r;
@@ -805,6 +805,14 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
       // The reference maximum moves only when a score passes it by 2^kLazy: weights then stay
       // below 2^(kPExp + kLazy) (far inside fp16), O and l carry the same factor, and most
       // steps need neither a reduction over the lanes nor a rescale.
+      // Far from zero the weights' one multiply-add fails: fp32 scores of 2^27 have no bits below 1
+      // left, so the unrounded product may be off the rounded maximum by any power of two, and the
+      // threshold's own rounding lets as much through. Once a score that moves a maximum is 2^18
+      // (`far`, until the piece ends) the products are rounded as the maxima are, and every larger
+      // score moves its maximum. Steps of full pages leave that to the others: they stop before
+      // they have changed anything. (Heads of one tile: no time lost; of 9-16 heads 1-2 %, 12/1 5 %.
+      // With the branch inside them, one tile 0.4-2 %, 9-16 heads 4-9 %; two operations for every
+      // score 0.3-1.7 % of one tile.)
       constexpr float kLazy = 8.f, kFar = 0x1p18f;
       float tm[NT][2];
       bool up = false;
@@ -819,6 +827,17 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
       if (__any_sync(0xffffffffu, up)) {
         bool is_far = false;
 #pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float h = fabsf(tm[nt][e] * qs);
+            is_far = is_far || (h >= kFar && h != -neg_inf());
+          }
+        if (__any_sync(0xffffffffu, is_far)) {
+          far = true;
+          if constexpr (FULL) return false;
+        }
+#pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float c[2];
 #pragma unroll
@@ -826,14 +845,17 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
             float v = tm[nt][e];
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-            // The maximum, as fmb, moves up only. From 2^kFar on, where the threshold's own
-            // rounding would let weights overflow, every new maximum moves it.
-            const float f = fminf(fmb[nt][e], kPExp - ceilf(__fmul_rn(v, qs)));
-            c[e] = f < fmb[nt][e] ? ex2(f - fmb[nt][e]) : 1.f;
-            fmb[nt][e] = f;
-            is_far = is_far || !(fabsf(f) < kFar);
-            thr[nt][e] = fabsf(f) < kFar ? __fdividef(kPExp - f + kLazy, qs)
-                                         : fmaxf(thr[nt][e], v);
+            if constexpr (FULL) {
+              const float m = kPExp - fmb[nt][e], mn = fmaxf(m, ceilf(v * qs));
+              c[e] = mn > m ? ex2(m - mn) : 1.f;
+              fmb[nt][e] = kPExp - mn;
+              thr[nt][e] = __fdividef(mn + kLazy, qs);
+            } else {  // the maximum moves up, fmb down
+              const float f = fminf(fmb[nt][e], kPExp - ceilf(__fmul_rn(v, qs)));
+              c[e] = f < fmb[nt][e] ? ex2(f - fmb[nt][e]) : 1.f;
+              fmb[nt][e] = f;
+              thr[nt][e] = far ? fmaxf(thr[nt][e], v) : __fdividef(kPExp - f + kLazy, qs);
+            }
             fl[nt][e] *= c[e];
             if constexpr (PACK) {  // columns 4-7 belong to the heads of columns 0-3
               const float other = __shfl_xor_sync(0xffffffffu, c[e], 2);
@@ -848,16 +870,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
             oacc[i][nt][3] *= c[1];
           }
         }
-        far = __any_sync(0xffffffffu, is_far);
       }
 
-      // Far: the product rounds as the maximum's did, so that even where scores have no bits below
-      // 1 left the largest weight is near 2^kPExp. (Scalar multiplications: packed ones and the
-      // addition would be fused.) The branch costs 0.8 % of 8 x 64-128 K tokens, 64/8 heads, two
-      // operations a score in every step 1.7 %.
       auto weight_arg = [&](float a, float b, int nt) {
         const float2 f = make_float2(fmb[nt][0], fmb[nt][1]);
-        if (far) return add2(make_float2(__fmul_rn(a, qs), __fmul_rn(b, qs)), f);
+        // (Scalar multiplications: packed ones and the addition would be fused.)
+        if (!FULL && far) return add2(make_float2(__fmul_rn(a, qs), __fmul_rn(b, qs)), f);
         return fma2(make_float2(a, b), make_float2(qs, qs), f);
       };
 #pragma unroll
@@ -934,19 +952,20 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
           }
         }
       }
+      return true;
     };
     for (int k = 0; k < len;) {
       const int first = j & 1;
       // Steps with nothing to check: full pages whose refill lies inside the range and inside the
       // present batch of block ids.
-      if (first == 0 && !step_write) {
+      if (first == 0 && !step_write && !far) {
         const int jr = j + 2 * DEPTH;  // the next refill's first page
         int m = min(len - k, (cctx - (csp + k) * kSubTokens) / kSubTokens) / 2;
         m = min(min(m, (n - jr) / 2), (-jr & 31) / 2);
         for (int i = 0; i < m; ++i) {
           cp_async_wait_groups<DEPTH - 1>();
           __syncwarp();
-          step(std::true_type{}, s, kSubTokens, kSubTokens);
+          if (!step(std::true_type{}, s, kSubTokens, kSubTokens)) break;
           __syncwarp();
           const int e = (j + 2 * DEPTH) & 31;
           copy_pair(__shfl_sync(0xffffffffu, cur, e), __shfl_sync(0xffffffffu, cur, e + 1), s);
