@@ -22,11 +22,12 @@
 //    error as the output's own.
 //  * steps of two full pages run in a loop with nothing to check; a step's scale and maximum are
 //    one multiply-add before the exponential (raw scores are compared with a threshold).
-// 280 warp instructions a page (479 with decode.cu's loop): 64 conversions, 64 multiplies, 24
+// 281 warp instructions a page (479 with decode.cu's loop): 64 conversions, 64 multiplies, 24
 // MMAs, 16 to pair the codes of neighbouring tokens for PV, the rest softmax, copies and loop.
-// Measured on a B200 (graph replay): 64 x 8192 tokens, 12/2 heads 41.3 us (3.67 TB/s); 8 x 64-128
-// K, 64/8 heads 167 us (5.43 TB/s, 0.83 of the measured copy bandwidth). That is 463 cycles a page
-// and scheduler, of which ALU instructions (conversions, logic) take 247, MMAs 192 and the FMA pipe
+// Measured on a B200 (graph replay): 64 x 8192 tokens, 12/2 heads 41.2 us (3.68 TB/s); 8 x 64-128
+// K, 64/8 heads 167 us in a short run (5.44 TB/s, 0.83 of the measured copy bandwidth), 189-201 in
+// a loop of seconds, at the power cap of 1000 W and 1.65-1.75 GHz. That is 463 cycles a page
+// and scheduler, of which ALU instructions (conversions, logic) take 249, MMAs 192 and the FMA pipe
 // up to 189; they hardly overlap (a group of one MMA and three conversions and multiplies takes
 // 18.6 cycles where the MMA alone takes 8 and the others 8). Shifts turned into multiplies, the
 // QK of the next step issued between the PV of this one, two chains of QK MMAs a page instead of
@@ -1118,7 +1119,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
   // by side: first the CTA's own are merged in shared memory. A segment that it holds alone is
   // done; of others (at most two, the first and the last) the CTA leaves one partial in the
   // workspace, and the CTA that arrives last merges those. (With a partial of every warp in the
-  // workspace one segment of 8192 tokens was up to 512 of them: 1 x 8192 tokens took 60 us.)
+  // workspace one segment of 8192 tokens was up to 512 of them: 1 x 8192 tokens took 58 us.)
   if (lane == 0) s_npend[warp] = min(nrec, 2);
   __syncthreads();
   // Entry i = 2 * warp + e in lane i; groups of entries of one segment.
@@ -1215,8 +1216,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_fp4_kernel(const DecodeF
 // Warps per CTA and ring stages per warp, by head tile (16 heads keep twice the accumulators).
 // 64 x 8192 / ragged 256 / 8 x 64-128 K tokens (12/2, 28/4 and 64/8 heads): 41.4 / 108.8 / 169.5 us
 // with sixteen warps of two stages (128 registers), 43.2 / 110.1 / 170.9 with twelve of two, 43.3 /
-// 110.7 / 171.6 with twelve of three, 43.2 / 119.7 / 184.2 with eight of four. Sixteen heads, 32/2,
-// 64 x 8192: 57.7 with eight warps (255 registers), 64.7 with twelve (spills).
+// 110.7 / 171.6 with twelve of three, 43.2 / 119.7 / 184.2 with eight of four. The chosen one spills
+// 12 bytes of 5-8 heads, none of fewer. Sixteen heads, 32/2, 64 x 8192: 58.3 with eight warps (250
+// registers), 7 more with twelve (spills).
 template <int GT> struct Shape;
 template <> struct Shape<8> { static constexpr int W = 16, DP = 2; };
 template <> struct Shape<16> { static constexpr int W = 8, DP = 4; };

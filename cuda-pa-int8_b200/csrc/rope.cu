@@ -17,15 +17,24 @@
 //    half-warp, all loaded before the first is used. It folds the weights into the token's
 //    cosines and sines once: a' = r (a (c w_a) - b (s w_b)), r = 1/rms, three operations a value.
 //
-// Measured on a B200 (graph replay): 16384 tokens, 32/8 heads, bf16: 63.7 us, 5.4 TB/s, 0.82 of
-// the measured copy bandwidth (memory and issue slots both two thirds busy); 64 tokens: 2.4 us, a
-// launch and two dependent loads. CTAs of 256 threads instead of 128: 71 us; 40 registers a
-// thread for full occupancy: 76 us (spills); four rows' sums reduced together, with fewer
-// shuffles but all rows waited for at once: 65.6 us.
+// Measured on a B200 (graph replay): 16384 tokens, 32/8 heads, bf16: 62.4-65.5 us from one B200 to
+// the next, 5.3-5.5 TB/s, 0.80-0.84 of the measured copy bandwidth (memory and issue slots both
+// two thirds busy); 64 tokens: 2.4 us after another kernel of its graph, 4.2 as a graph of its
+// own, a launch and two dependent loads. With the same kernel at 63.7 us, CTAs of 256 threads
+// instead of 128: 71; 40 registers a thread for full occupancy: 76 (spills); four rows' sums
+// reduced together, with fewer shuffles but all rows waited for at once: 65.6.
 //
 // The cache forms (kCache) round K to the rows' type first, so caches are bit for bit those of
 // the separate calls, then quantise as the cache writes do. One launch less for a step, and K's
-// rows never go to memory and back.
+// rows never go to memory and back. A lane has eight values of a row, so V's page layout takes it
+// eight stores where the token write has 16-byte ones for runs of slots: for few tokens this form
+// is faster than the separate calls, for many slower. bf16, fused and separate, us:
+//   28/4 heads, 16 tokens     4-bit 3.1  4.1   fp16 3.1  4.6   int8 3.6  5.2
+//   28/4 heads, 1024 tokens   4-bit 7.2  7.2   fp16 12.3 13.3  int8 12.9 13.3
+//   28/4 heads, 4096 tokens   4-bit 19.5 16.9  fp16 30.9 35.8  int8 36.0 33.4
+//   32/8 heads, 16384 tokens  4-bit 99.9 76.8  fp16 179 91     int8 214 92 (prompts; 184 226 and
+//                             197 213 at scattered slots)
+// The int8 and fp8 kernels of four 16-bit heads a half-warp spill 8 to 24 bytes.
 
 #include "fp4.cuh"
 #include "pa_common.cuh"
@@ -406,7 +415,8 @@ cudaError_t launch_t(const RopeArgs& a, int sms, cudaStream_t st) {
   };
   // Four heads per half-warp where that still gives every SM sixteen warps, else one (each warp's
   // chain is then shorter). 32/8 heads, bf16, one and four heads: 256 tokens (1280 warps of four)
-  // 2.9 and 3.1 us, 512 tokens (2560) 4.5 and 3.8, 16384 tokens 102 and 62.
+  // 2.9 and 3.1 us, 512 tokens (2560) 4.5 and 3.8, 16384 tokens 102 and 62 (of 28 and 4 heads four
+  // leave a fifth of the row slots empty).
   if (warps(4) >= 16LL * sms) return launch_heads<T, kCache, 4>(a, warps(4), st);
   return launch_heads<T, kCache, 1>(a, warps(1), st);
 }
